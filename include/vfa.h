@@ -219,6 +219,98 @@ int vfa_bwd_head_splits(int batch, int num_heads, int num_heads_k, int max_seqle
                                 wave, hand-pipelined; dK/dV: 32 keys x all 256 columns per wave) */
 int vfa_dispatch_geometry(const vfa_params *p, int kernel);
 
+/* ---- Operators without a counterpart in the reference: a KV cache held in 8 bits, and the norm and
+ * rotation of query and key heads ---- */
+
+/* KV cache in 8 bits: e4m3 codes (OCP float8_e4m3fn) with one E8M0 scale byte (value 2^(byte - 127), 255 =
+ * NaN) per (block of scale_block tokens, KV head), for K and for V.  A code stands for code * scale, exactly.
+ *
+ * Common to the three entry points, in `a`: k / v = the codes, contiguous cache (num_pages, seqlen_k, h_k, d)
+ * or pages (num_pages, page_block_size, h_k, d) with block_table; strides in BYTES, multiples of 16, base
+ * pointers 16-byte aligned; b, h_k, d (a multiple of 16, at most 256); seqlen_k = the most tokens a sequence
+ * can have (a contiguous cache: its rows, a multiple of 16; pages: max_blocks * page_block_size);
+ * cu_seqlens_k = (b) int32, tokens in the cache before the call (lengths, not offsets), NULL = seqlen_k;
+ * cache_batch_idx (contiguous caches only).  Lengths are cut to [0, seqlen_k]; a page id outside
+ * [0, num_pages) is never followed: nothing is written there, and what is read from it is NaN. */
+typedef struct vfa_kv8_params {
+    vfa_params a;
+    void *k_scale, *v_scale;         /* (num_pages, rows / scale_block, h_k), strides in bytes */
+    int64_t k_scale_batch_stride, k_scale_row_stride, k_scale_head_stride;
+    int64_t v_scale_batch_stride, v_scale_row_stride, v_scale_head_stride;
+    int scale_block;                 /* a multiple of 16 that divides the rows of a page */
+    int num_pages;                   /* pages of the pool, or batch rows of a contiguous cache */
+    /* Writing: a.knew / a.vnew (16 bit, a.dtype) dense (b, a.seqlen_knew, h_k, d), or ragged
+     * (total, h_k, d) with cu_seqlens_new (b + 1) and a.seqlen_knew = the longest run. */
+    const int32_t *cu_seqlens_new;
+    /* Reading back: 16-bit outputs (a.dtype), dense (b, seqlen_out, h_k, d) or ragged (rows_out, h_k, d)
+     * with cu_seqlens_out (b + 1); strides in elements. */
+    void *k_out, *v_out;
+    int64_t ko_batch_stride, ko_row_stride, ko_head_stride;
+    int64_t vo_batch_stride, vo_row_stride, vo_head_stride;
+    const int32_t *cu_seqlens_out;
+    int64_t rows_out;
+    int seqlen_out;
+} vfa_kv8_params;
+
+/* Write new tokens at positions cu_seqlens_k[i] .. of every sequence.  A block's scale is the least power of
+ * two with max |x| <= 448 * scale over the tokens written to it (not under 2^-126); tokens that join a block
+ * which holds some already can only raise it, and what the block holds is then re-encoded.  A block that is
+ * written from its first token on starts anew.  Rounding is to nearest even; NaN and the infinities become
+ * NaN codes and do not count for the scale.  Rows behind the new tokens stay as they are.  Two sequences must
+ * not write to one block. */
+int vfa_kv8_quantize(const vfa_kv8_params *p);
+
+/* Read the first cu_seqlens_k[i] tokens of every sequence (ragged: at most the sequence's share of the
+ * output) in 16 bits; output rows without a token are zeros. */
+int vfa_kv8_dequantize(const vfa_kv8_params *p);
+
+/* Attention of q (dense (b, seqlen_q, h, d), or ragged with cu_seqlens_q) over the cache: a.q, a.out,
+ * a.softmax_lse, masks, ALiBi, a.num_splits with its scratch as for vfa_mha_fwd_kvcache.  With a.knew the new
+ * tokens (dense) are written first and attended. */
+int vfa_kv8_mha_fwd(const vfa_kv8_params *p);
+
+/* The num_splits that vfa_kv8_mha_fwd should be given: enough (batch, KV head group, 16- or 32-row block) work
+ * items to fill num_cus compute units, at least 256 keys each. */
+int vfa_kv8_num_splits(int batch, int num_heads, int num_heads_k, int head_size, int max_seqlen_k, int max_seqlen_q,
+                       int num_cus);
+
+/* RMS norm of every head of q (b, s, h, d) and k (b, s, h_k, d), times a weight (d), then the position rotation of its first
+ * rotary_dim columns (pairs (2i, 2i + 1) if interleaved, else (i, i + rotary_dim / 2)):
+ *   y = R(position) (x / sqrt(mean(x^2) + eps) * w).
+ * Ragged batches are b = 1.  Strides in elements, multiples of 8; base pointers 16-byte aligned; last dim
+ * contiguous.  positions (b, s) int32, NULL = the index in s; a negative position marks padding (output and
+ * gradients zero); one past the tables gives NaN.  The backward reads q / k again, needs nothing else from
+ * the forward, and gives the same bits on every run. */
+typedef struct vfa_qk_norm_rotary_params {
+    int dtype;                       /* VFA_FP16 | VFA_BF16: q, k, outputs, gradients */
+    int weight_fp32, table_fp32;     /* 1: fp32; 0: dtype */
+    int b, s, h, h_k, d;             /* d: a multiple of 8, at most 256 */
+    const void *q, *k;
+    int64_t q_batch_stride, q_row_stride, q_head_stride;
+    int64_t k_batch_stride, k_row_stride, k_head_stride;
+    const void *q_weight, *k_weight;
+    const void *rotary_cos, *rotary_sin;   /* (table_rows, rotary_dim / 2), contiguous */
+    int table_rows, rotary_dim, is_rotary_interleaved;   /* rotary_dim: a multiple of 16, at most d */
+    const int32_t *positions;
+    int64_t positions_batch_stride;
+    float eps;
+    /* forward: the outputs; backward: dq and dk (either may be NULL) */
+    void *q_out, *k_out;
+    int64_t qo_batch_stride, qo_row_stride, qo_head_stride;
+    int64_t ko_batch_stride, ko_row_stride, ko_head_stride;
+    /* backward */
+    const void *dq_out, *dk_out;     /* gradients of the outputs */
+    int64_t dqo_batch_stride, dqo_row_stride, dqo_head_stride;
+    int64_t dko_batch_stride, dko_row_stride, dko_head_stride;
+    void *dq_weight, *dk_weight;     /* (d), the weights' type; either may be NULL */
+    float *workspace;                /* vfa_qk_norm_rotary_bwd_workspace() floats, not needed without dq_weight / dk_weight */
+    void *stream;
+} vfa_qk_norm_rotary_params;
+
+int vfa_qk_norm_rotary_fwd(const vfa_qk_norm_rotary_params *p);
+int vfa_qk_norm_rotary_bwd(const vfa_qk_norm_rotary_params *p);
+size_t vfa_qk_norm_rotary_bwd_workspace(const vfa_qk_norm_rotary_params *p);   /* floats */
+
 /* sizeof(vfa_params) of the built library, for foreign-function bindings to check their mirror of
  * the struct against (no counterpart in the reference: its boundary is typed by pybind). */
 size_t vfa_params_sizeof(void);

@@ -13,6 +13,8 @@
 #include "../../include/vfa.h"
 #include "vfa_kernel_params.h"
 #include "vfa_dispatch.h"
+#include "vfa_kv8.h"
+#include "vfa_qk_norm.h"
 
 namespace vfa {
 hipError_t run_fwd_prefill(const KParams &p, hipStream_t stream);
@@ -26,6 +28,12 @@ hipError_t run_fwd_prefill_pack(const KParams &p, hipStream_t stream);
 bool fwd_prefill_split_ok(const KParams &p);
 hipError_t run_fwd_combine(const KParams &p, hipStream_t stream);
 hipError_t run_bwd_dropout(const KParams &p, hipStream_t stream, hipEvent_t *stage_events);
+hipError_t run_kv8_quantize(const KV8Params &a, hipStream_t stream);             // kv8_cache.hip
+hipError_t run_kv8_dequantize(const KV8Params &a, hipStream_t stream);
+hipError_t run_fwd_kv8(const KV8Params &a, hipStream_t stream);                  // fwd_kv8.hip
+int kv8_heads_per_wg(int d, int h_k);
+hipError_t run_qk_norm_rotary(const QKNormParams &p, bool bwd, hipStream_t stream);   // qk_norm_rotary.hip
+void qk_norm_bwd_blocks(QKNormParams &p, int cus);
 }  // namespace vfa
 
 using vfa::KParams;
@@ -526,6 +534,211 @@ extern "C" int vfa_dispatch_geometry(const vfa_params *p, int kernel) {
     k.hsplit = p->bwd_head_splits > 1 ? p->bwd_head_splits : 0;
     const int cus = num_cus();
     return kernel == 0 ? vfa::fwd_geometry(k, cus) : kernel == 1 ? vfa::dkdv_geometry(k, cus) : vfa::dq_geometry(k, cus);
+}
+
+// ---------------------------------------------------------------------------------------------
+// 8-bit KV cache
+static bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
+
+static int kv8_fill(const vfa_kv8_params *p, vfa::KV8Params &k) {
+    VFA_CHECK(p != nullptr, "null params");
+    const vfa_params &a = p->a;
+    VFA_CHECK(a.dtype == VFA_FP16 || a.dtype == VFA_BF16, "FlashAttention only support fp16 and bf16 data type");
+    VFA_CHECK(a.k && a.v && p->k_scale && p->v_scale, "null cache or scale pointer");
+    VFA_CHECK(a.b > 0, "batch size must be postive");
+    VFA_CHECK(a.h_k > 0, "number of heads must be positive");
+    VFA_CHECK(a.d > 0 && a.d <= 256 && a.d % 16 == 0, "8-bit KV cache: head dimension must be a multiple of 16, at most 256");
+    VFA_CHECK(!(a.block_table && a.cache_batch_idx), "Paged KVcache does not support cache_batch_idx");
+    const int rows = a.block_table ? a.page_block_size : a.seqlen_k;
+    VFA_CHECK(p->num_pages > 0 && rows > 0 && a.seqlen_k > 0, "8-bit KV cache: empty cache");
+    VFA_CHECK(p->scale_block > 0 && p->scale_block % 16 == 0 && rows % p->scale_block == 0,
+              "8-bit KV cache: the tokens per scale must be a multiple of 16 that divides the rows of a page");
+    VFA_CHECK(a.block_table || a.cache_batch_idx || a.b <= p->num_pages, "8-bit KV cache: batch size exceeds the cache's");
+    VFA_CHECK(aligned16(a.k) && aligned16(a.v) && a.k_batch_stride % 16 == 0 && a.k_row_stride % 16 == 0 && a.k_head_stride % 16 == 0 &&
+                  a.v_batch_stride % 16 == 0 && a.v_row_stride % 16 == 0 && a.v_head_stride % 16 == 0,
+              "8-bit KV cache: codes must be 16-byte aligned, strides multiples of 16 bytes");
+    fill_common(&a, k.p, a.seqlen_q, a.seqlen_k);
+    k.p.k_cumulative = 0;
+    k.ks = (unsigned char *)p->k_scale; k.vs = (unsigned char *)p->v_scale;
+    k.ks_bs = p->k_scale_batch_stride; k.ks_rs = p->k_scale_row_stride; k.ks_hs = p->k_scale_head_stride;
+    k.vs_bs = p->v_scale_batch_stride; k.vs_rs = p->v_scale_row_stride; k.vs_hs = p->v_scale_head_stride;
+    k.blk = p->scale_block;
+    k.page_rows = rows;
+    k.num_pages = p->num_pages;
+    k.cap = a.seqlen_k;
+    vfa::kv8_div_magic(rows / 16, k.page_mul, k.page_sh);
+    vfa::kv8_div_magic(k.blk / 16, k.blk_mul, k.blk_sh);
+    if (a.knew) {
+        VFA_CHECK(a.vnew, "If key is supplied, value must also be passed in");
+        VFA_CHECK(aligned16(a.knew) && aligned16(a.vnew) && a.knew_batch_stride % 8 == 0 && a.knew_row_stride % 8 == 0 &&
+                      a.knew_head_stride % 8 == 0 && a.vnew_batch_stride % 8 == 0 && a.vnew_row_stride % 8 == 0 && a.vnew_head_stride % 8 == 0,
+                  "new keys and values must be 16-byte aligned, strides multiples of 8 elements");
+        k.p.knew = a.knew; k.p.vnew = a.vnew; k.p.seqlen_knew = a.seqlen_knew;
+        k.p.knew_bs = a.knew_batch_stride; k.p.knew_rs = a.knew_row_stride; k.p.knew_hs = a.knew_head_stride;
+        k.p.vnew_bs = a.vnew_batch_stride; k.p.vnew_rs = a.vnew_row_stride; k.p.vnew_hs = a.vnew_head_stride;
+        VFA_CHECK(a.seqlen_knew >= 0, "negative number of new tokens");
+    }
+    k.cu_new = p->cu_seqlens_new;
+    return VFA_OK;
+}
+
+extern "C" int vfa_kv8_quantize(const vfa_kv8_params *p) {
+    g_err.clear();
+    vfa::KV8Params k;
+    std::memset(&k, 0, sizeof(k));
+    int rc = kv8_fill(p, k);
+    if (rc) return rc;
+    VFA_CHECK(p->a.knew, "no new tokens");
+    if ((rc = check_arch())) return rc;
+    hipError_t e = vfa::run_kv8_quantize(k, (hipStream_t)p->a.stream);
+    if (e != hipSuccess) return hip_fail(e, "kv8 quantize launch");
+    return VFA_OK;
+}
+
+extern "C" int vfa_kv8_dequantize(const vfa_kv8_params *p) {
+    g_err.clear();
+    vfa::KV8Params k;
+    std::memset(&k, 0, sizeof(k));
+    int rc = kv8_fill(p, k);
+    if (rc) return rc;
+    if (p->rows_out == 0) return VFA_OK;
+    VFA_CHECK(p->k_out && p->v_out, "null output pointer");
+    VFA_CHECK(p->rows_out > 0 && (p->cu_seqlens_out || p->seqlen_out > 0), "8-bit KV cache: no shape for the output");
+    VFA_CHECK(aligned16(p->k_out) && aligned16(p->v_out) && p->ko_batch_stride % 8 == 0 && p->ko_row_stride % 8 == 0 &&
+                  p->ko_head_stride % 8 == 0 && p->vo_batch_stride % 8 == 0 && p->vo_row_stride % 8 == 0 && p->vo_head_stride % 8 == 0,
+              "outputs must be 16-byte aligned, strides multiples of 8 elements");
+    if ((rc = check_arch())) return rc;
+    k.k_out = p->k_out; k.v_out = p->v_out;
+    k.ko_bs = p->ko_batch_stride; k.ko_rs = p->ko_row_stride; k.ko_hs = p->ko_head_stride;
+    k.vo_bs = p->vo_batch_stride; k.vo_rs = p->vo_row_stride; k.vo_hs = p->vo_head_stride;
+    k.cu_out = p->cu_seqlens_out; k.rows_out = p->rows_out; k.seqlen_out = p->seqlen_out;
+    hipError_t e = vfa::run_kv8_dequantize(k, (hipStream_t)p->a.stream);
+    if (e != hipSuccess) return hip_fail(e, "kv8 dequantize launch");
+    return VFA_OK;
+}
+
+extern "C" int vfa_kv8_num_splits(int batch, int num_heads, int num_heads_k, int head_size, int max_seqlen_k, int max_seqlen_q,
+                                  int num_cus_) {
+    if (num_heads_k <= 0 || num_heads % num_heads_k != 0 || head_size <= 0 || batch <= 0) return 1;
+    const int hpw = vfa::kv8_heads_per_wg(head_size, num_heads_k), parts = 8 / hpw;
+    const long long items = (long long)batch * (num_heads_k / hpw) * (((long long)max_seqlen_q * (num_heads / num_heads_k) + 31) / 32);
+    // two workgroups per CU; a wave keeps at least 4 of its steps of 32 keys
+    const long long most = std::max(1LL, (long long)max_seqlen_k / (32LL * 4 * parts));
+    const long long want = (2LL * num_cus_ + items - 1) / std::max(1LL, items);
+    return (int)std::max(1LL, std::min({want, most, 128LL}));
+}
+
+extern "C" int vfa_kv8_mha_fwd(const vfa_kv8_params *p) {
+    g_err.clear();
+    vfa::KV8Params k;
+    std::memset(&k, 0, sizeof(k));
+    int rc = kv8_fill(p, k);
+    if (rc) return rc;
+    const vfa_params &a = p->a;
+    if ((rc = common_checks(&a))) return rc;
+    VFA_CHECK(a.p_dropout == 0.f, "fwd_kvcache has no dropout");
+    VFA_CHECK(a.softmax_scale > 0.f, "softmax_scale must be positive");
+    VFA_CHECK(!(a.knew && (a.cu_seqlens_q || p->cu_seqlens_new)), "8-bit KV cache: new tokens go with a dense query batch");
+    VFA_CHECK(aligned16(a.q) && aligned16(a.out) && a.q_batch_stride % 8 == 0 && a.q_row_stride % 8 == 0 && a.q_head_stride % 8 == 0 &&
+                  a.o_batch_stride % 8 == 0 && a.o_row_stride % 8 == 0 && a.o_head_stride % 8 == 0,
+              "q and out must be 16-byte aligned, strides multiples of 8 elements");
+    if ((rc = check_arch())) return rc;
+    if (a.seqlen_q <= 0) return VFA_OK;
+    hipStream_t stream = (hipStream_t)a.stream;
+    hipError_t e;
+    if (a.knew) {
+        e = vfa::run_kv8_quantize(k, stream);
+        if (e != hipSuccess) return hip_fail(e, "kv8 quantize launch");
+    }
+    if (a.num_splits > 1) {
+        VFA_CHECK(a.num_splits <= 128, "num_splits > 128 not supported");
+        VFA_CHECK(a.oaccum && a.softmax_lseaccum, "split-KV needs oaccum / softmax_lseaccum scratch");
+        k.p.num_splits = a.num_splits;
+        k.p.oaccum = a.oaccum;
+        k.p.lseaccum = a.softmax_lseaccum;
+    }
+    k.heads_per_wg = vfa::kv8_heads_per_wg(a.d, a.h_k);
+    e = vfa::run_fwd_kv8(k, stream);
+    if (e == hipSuccess && a.num_splits > 1) e = vfa::run_fwd_combine(k.p, stream);
+    if (e != hipSuccess) return hip_fail(e, "kv8 attention launch");
+    return VFA_OK;
+}
+
+// ---------------------------------------------------------------------------------------------
+// q / k norm + rotation
+static int qk_norm_fill(const vfa_qk_norm_rotary_params *p, vfa::QKNormParams &k, bool bwd) {
+    VFA_CHECK(p != nullptr, "null params");
+    VFA_CHECK(p->dtype == VFA_FP16 || p->dtype == VFA_BF16, "qk_norm_rotary only supports fp16 and bf16 data type");
+    VFA_CHECK(p->b >= 0 && p->s >= 0 && p->h > 0 && p->h_k > 0, "negative size, or no heads");
+    VFA_CHECK(p->d > 0 && p->d <= 256 && p->d % 8 == 0, "qk_norm_rotary: head dimension must be a multiple of 8, at most 256");
+    VFA_CHECK(p->rotary_dim > 0 && p->rotary_dim % 16 == 0, "Only rotary dimensions divisible by 16 are currently supported");
+    VFA_CHECK(p->rotary_dim <= p->d, "rotary_dim must be <= headdim");
+    VFA_CHECK(p->table_rows > 0 && p->rotary_cos && p->rotary_sin, "rotary tables are required");
+    VFA_CHECK(p->positions || p->s <= p->table_rows, "cos/sin seqlen must be at least the seqlen of q");
+    VFA_CHECK(p->q_weight && p->k_weight, "null weight pointer");
+    const bool tokens = (int64_t)p->b * p->s > 0;
+    VFA_CHECK(!tokens || (p->q && p->k), "null tensor pointer");
+    std::memset(&k, 0, sizeof(k));
+    auto side = [&](int i, const void *x, int64_t bs, int64_t rs, int64_t hs, const void *w, int h, void *y, int64_t ybs, int64_t yrs,
+                    int64_t yhs, const void *dy, int64_t dbs, int64_t drs, int64_t dhs, void *dw) {
+        vfa::QKNormTensor &t = k.t[i];
+        t.x = x; t.x_bs = bs; t.x_rs = rs; t.x_hs = hs; t.w = w; t.h = h;
+        t.y = y; t.y_bs = ybs; t.y_rs = yrs; t.y_hs = yhs;
+        t.dy = dy; t.dy_bs = dbs; t.dy_rs = drs; t.dy_hs = dhs; t.dw = dw;
+        return aligned16(x) && aligned16(y) && aligned16(dy) && bs % 8 == 0 && rs % 8 == 0 && hs % 8 == 0 && ybs % 8 == 0 &&
+               yrs % 8 == 0 && yhs % 8 == 0 && dbs % 8 == 0 && drs % 8 == 0 && dhs % 8 == 0;
+    };
+    const bool ok_q = side(0, p->q, p->q_batch_stride, p->q_row_stride, p->q_head_stride, p->q_weight, p->h, p->q_out, p->qo_batch_stride,
+                           p->qo_row_stride, p->qo_head_stride, p->dq_out, p->dqo_batch_stride, p->dqo_row_stride, p->dqo_head_stride,
+                           p->dq_weight);
+    const bool ok_k = side(1, p->k, p->k_batch_stride, p->k_row_stride, p->k_head_stride, p->k_weight, p->h_k, p->k_out, p->ko_batch_stride,
+                           p->ko_row_stride, p->ko_head_stride, p->dk_out, p->dko_batch_stride, p->dko_row_stride, p->dko_head_stride,
+                           p->dk_weight);
+    VFA_CHECK(ok_q && ok_k, "tensors must be 16-byte aligned, strides multiples of 8 elements");
+    if (!bwd) VFA_CHECK(!tokens || (p->q_out && p->k_out), "null output pointer");
+    else VFA_CHECK(!tokens || (p->dq_out && p->dk_out), "null gradient pointer");
+    k.b = p->b; k.s = p->s; k.d = p->d;
+    k.positions = p->positions; k.pos_bs = p->positions_batch_stride;
+    k.cos = p->rotary_cos; k.sin = p->rotary_sin;
+    k.table_rows = p->table_rows; k.rd = p->rotary_dim; k.interleaved = p->is_rotary_interleaved;
+    k.eps = p->eps;
+    k.is_bf16 = p->dtype == VFA_BF16; k.table_f32 = p->table_fp32; k.w_f32 = p->weight_fp32;
+    return VFA_OK;
+}
+
+extern "C" int vfa_qk_norm_rotary_fwd(const vfa_qk_norm_rotary_params *p) {
+    g_err.clear();
+    vfa::QKNormParams k;
+    int rc = qk_norm_fill(p, k, false);
+    if (rc) return rc;
+    if ((rc = check_arch())) return rc;
+    hipError_t e = vfa::run_qk_norm_rotary(k, false, (hipStream_t)p->stream);
+    if (e != hipSuccess) return hip_fail(e, "qk_norm_rotary launch");
+    return VFA_OK;
+}
+
+extern "C" size_t vfa_qk_norm_rotary_bwd_workspace(const vfa_qk_norm_rotary_params *p) {
+    if (!p || p->d <= 0 || p->h <= 0 || p->h_k <= 0) return 0;
+    vfa::QKNormParams k;
+    std::memset(&k, 0, sizeof(k));
+    k.t[0].h = p->h; k.t[1].h = p->h_k;
+    k.b = p->b; k.s = p->s; k.d = p->d;
+    vfa::qk_norm_bwd_blocks(k, num_cus());
+    return (size_t)(k.blocks_q + k.blocks_k) * (size_t)p->d;
+}
+
+extern "C" int vfa_qk_norm_rotary_bwd(const vfa_qk_norm_rotary_params *p) {
+    g_err.clear();
+    vfa::QKNormParams k;
+    int rc = qk_norm_fill(p, k, true);
+    if (rc) return rc;
+    VFA_CHECK(!(p->dq_weight || p->dk_weight) || p->workspace, "qk_norm_rotary: the weights' gradients need the workspace");
+    if ((rc = check_arch())) return rc;
+    k.dw_part = p->workspace;
+    vfa::qk_norm_bwd_blocks(k, num_cus());
+    hipError_t e = vfa::run_qk_norm_rotary(k, true, (hipStream_t)p->stream);
+    if (e != hipSuccess) return hip_fail(e, "qk_norm_rotary backward launch");
+    return VFA_OK;
 }
 
 extern "C" size_t vfa_params_sizeof(void) { return sizeof(vfa_params); }

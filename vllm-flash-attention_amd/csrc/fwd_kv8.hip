@@ -1,0 +1,391 @@
+// Attention over an 8-bit KV cache (format: vfa_kv8.h): a few query rows per KV head against a long key
+// range -- decode, drafted tokens, short chunks.
+//
+// The keys and values are the exact 16-bit values that the codes stand for (the conversion instruction
+// applies the power-of-two scale), so the result is that of the 16-bit cache path on the cache read back,
+// up to the order of sums.
+//
+// HBM-bound: 2 d bytes per key and KV head against 4 d rows flops.  A workgroup is 8 waves; each wave owns
+// one KV head (of heads_per_wg adjacent ones, whose rows are adjacent in memory) and every parts-th step of
+// 32 keys, with a running maximum, sum and output of its own.  Waves share nothing until the end, so the key
+// loop has no barrier:
+//   * the 16 NR rows of a workgroup are (query position, query head of the group) pairs: the heads that share
+//     a KV head read it once;
+//   * S^T = K Q^T by 16x16x32 MFMAs with the key on the accumulator's rows and the query row on the lane.  A
+//     lane's K operand is 16 consecutive codes of one key: two k-steps, loaded straight from memory to
+//     registers (which columns a k-step takes is free as long as Q agrees);
+//   * P^T of 32 keys is, in the registers it is computed in, the B operand of O^T += V^T P^T if V^T takes its
+//     keys in the order {4g .. 4g+3, 16+4g .. 16+4g+3} for lane group g: ds_read_b64_tr_b8 reads any 8 rows,
+//     so V goes through a wave-private LDS image as codes and comes back transposed, to be converted there.
+#include "vfa_kv8.h"
+
+namespace vfa {
+
+constexpr int A_NW = 8, A_NT = A_NW * 64;
+constexpr int A_STEP = 32;                   // keys of a step
+
+template <int DP, int NR>
+struct Kv8Cfg {
+    static constexpr int VB = A_STEP * DP;               // V image of a wave
+    static constexpr int O_ROWB = DP * 4 + 16;
+    static constexpr int O_BYTES = A_NW * 16 * O_ROWB;   // merge area: 16 rows of every wave
+    static constexpr int MAIN = A_NW * VB > O_BYTES ? A_NW * VB : O_BYTES;
+    static constexpr int ML = A_NW * 16 * NR * 2 * 4;    // maxima and sums
+    static constexpr int LDS_BYTES = MAIN + ML;
+};
+
+template <bool BF16>
+__device__ __forceinline__ f32x4 mma16(i32x4 a, i32x4 b, f32x4 c) {
+    if constexpr (BF16)
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+// combined over the four lanes that hold one row (l, l ^ 16, l ^ 32, l ^ 48)
+__device__ __forceinline__ float quad_max(float x) {
+    auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return half_swap_max(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])));
+}
+__device__ __forceinline__ float quad_sum(float x) {
+    auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return half_swap_sum(__uint_as_float(r[0]) + __uint_as_float(r[1]));
+}
+// 16-byte chunk of row `row` of the V image: the 16 rows that 32 lanes of a transposed read touch lie in
+// different banks
+template <int DP>
+__device__ __forceinline__ int kv8_swz(int row) {
+    if constexpr (DP == 64) return ((row >> 2) & 1) | ((row >> 4) & 1) << 1;
+    else if constexpr (DP == 128) return ((row >> 1) & 3) | ((row >> 4) & 1) << 2;
+    else return (row & 7) | ((row >> 4) & 1) << 3;
+}
+
+// Columns from p.d to DP are zero in Q, and their K and V codes are not loaded (zeros).
+template <int DP, bool BF16, int NR>
+__global__ void __launch_bounds__(A_NT, (NR == 1 && DP == 64) ? 4 : 2)
+fwd_kv8_kernel(const KV8Params a, const int n_mblocks) {
+    using Cfg = Kv8Cfg<DP, NR>;
+    constexpr int NJ = DP / 64;              // 64-column groups of K: one 16-byte load per lane and key tile
+    constexpr int NDB = DP / 16;             // 16-column blocks of O
+    constexpr int CPR = DP / 16;             // 16-byte chunks of a V row
+    constexpr int NV = A_STEP * CPR / 64;    // V loads per lane and step
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    const KParams &p = a.p;
+
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int c = lane & 15, g = lane >> 4;
+    const int hpw = a.heads_per_wg, parts = A_NW / hpw;
+    const int whead = wave & (hpw - 1), part = wave / hpw;
+
+    // blocks of one (batch, head group) -- its splits and row blocks -- run on one XCD at about the same time
+    int L = blockIdx.x;
+    if (p.num_splits > 1 || n_mblocks > 1) {
+        const int per_xcd = gridDim.x / 8;
+        if (L < per_xcd * 8) L = (L % 8) * per_xcd + L / 8;
+    }
+    const int n_hblocks = p.h_k / hpw;
+    const int m_block = L % n_mblocks; L /= n_mblocks;
+    const int hblock = L % n_hblocks; L /= n_hblocks;
+    const int split = L % p.num_splits; L /= p.num_splits;
+    const int bidb = L;
+    const int hk = hblock * hpw + whead;
+    const int ratio = p.h_ratio;
+    const bool is_split = p.num_splits > 1;
+
+    const BlockInfo bi(p, bidb);
+    const int sq = bi.sq;
+    const int sk = min(kv8_cached(a, bidb) + (p.knew ? p.seqlen_knew : 0), a.cap);
+    const int rows = sq * ratio;
+    const int q0 = m_block * 16 * NR;
+    if (q0 >= rows) return;
+    const int pos_lo = q0 / ratio, pos_hi = min(rows - 1, q0 + 16 * NR - 1) / ratio;
+
+    // keys that some row of the block sees, then this split's share of their steps
+    const bool edge_r = p.is_causal || p.is_local;
+    const int vis_lo = p.is_local ? max(0, pos_lo + sk - sq - p.wl) : 0;
+    const int vis_hi = edge_r ? min(sk, pos_hi + 1 + sk - sq + p.wr) : sk;
+    int n0 = vis_lo / A_STEP, n1 = vis_hi > vis_lo ? (vis_hi + A_STEP - 1) / A_STEP : n0;
+    if (is_split) {
+        const int per = (n1 - n0 + p.num_splits - 1) / p.num_splits;
+        n0 += split * per;
+        n1 = min(n1, n0 + per);
+    }
+
+    const unsigned short *qg = (const unsigned short *)p.q + bi.q_off(p.q_bs, p.q_rs, bidb);
+    unsigned short *og = (unsigned short *)p.o + bi.q_off(p.o_bs, p.o_rs, bidb);
+    // row i of KV head `head`: query position i / ratio, query head head * ratio + i % ratio
+    auto stat_at = [&](int head, int i) -> int64_t {
+        const int64_t bh = (int64_t)bidb * p.h + head * ratio + i % ratio;
+        return ((is_split ? (int64_t)split * p.b * p.h : 0) + bh) * p.seqlen_q + i / ratio;
+    };
+    float *lse = is_split ? p.lseaccum : p.lse;
+
+    if (n1 <= n0) {
+        for (int i = tid; i < hpw * 16 * NR * (DP / 8); i += A_NT) {
+            const int ch = i % (DP / 8), rr = i / (DP / 8) % (16 * NR), head = hblock * hpw + i / (DP / 8) / (16 * NR);
+            const int row = q0 + rr;
+            if (row >= rows || ch * 8 >= p.d) continue;
+            if (is_split) {
+                float *dst = p.oaccum + stat_at(head, row) * p.d + ch * 8;
+                *(f32x4 *)dst = f32x4{0, 0, 0, 0};
+                *(f32x4 *)(dst + 4) = f32x4{0, 0, 0, 0};
+            } else {
+                *(i32x4 *)(og + (int64_t)(row / ratio) * p.o_rs + (int64_t)(head * ratio + row % ratio) * p.o_hs + ch * 8) = i32x4{0, 0, 0, 0};
+            }
+            if (ch == 0) lse[stat_at(head, row)] = is_split ? -INFINITY : INFINITY;
+        }
+        return;
+    }
+
+    // Q operand: columns 64 j + 16 g + 8 s .. of k-step 2 j + s
+    i32x4 qf[NR][2 * NJ];
+    int pos[NR];
+    float slope[NR];
+#pragma unroll
+    for (int r = 0; r < NR; r++) {
+        const int row = min(q0 + 16 * r + c, rows - 1);
+        pos[r] = row / ratio;
+        const int head = hk * ratio + row % ratio;
+        slope[r] = p.alibi_slopes ? p.alibi_slopes[(int64_t)bidb * p.alibi_bs + head] / p.scale : 0.f;
+        const unsigned short *qr = qg + (int64_t)pos[r] * p.q_rs + (int64_t)head * p.q_hs;
+#pragma unroll
+        for (int s = 0; s < 2 * NJ; s++) {
+            const int col = 64 * (s >> 1) + 16 * g + 8 * (s & 1);
+            qf[r][s] = col < p.d ? *(const i32x4 *)(qr + col) : i32x4{0, 0, 0, 0};
+        }
+    }
+
+    const unsigned char *kbase = (const unsigned char *)p.k + (int64_t)hk * p.k_hs;
+    const unsigned char *vbase = (const unsigned char *)p.v + (int64_t)hk * p.v_hs;
+    const unsigned char *ksb = a.ks + (int64_t)hk * a.ks_hs, *vsb = a.vs + (int64_t)hk * a.vs_hs;
+
+    i32x4 kreg[2][NJ], vreg[NV];
+    unsigned ksc[2], vsc[2];
+    // Loads of the step n.  A tile of 16 keys lies in one page and one block of the scales (both are multiples
+    // of 16 rows); one that starts past the sequence's end takes the sequence's last tile (its keys are masked).
+    auto load_step = [&](int n) __attribute__((always_inline)) {
+#pragma unroll
+        for (int t = 0; t < 2; t++) {
+            const int key = min(n * A_STEP + 16 * t, (sk - 1) & ~15);
+            const int page = __builtin_amdgcn_readfirstlane(kv8_page(a, bidb, key));
+            const int row = kv8_row_in_page(a, key);
+            const int64_t pg = max(page, 0);
+            const int blk = kv8_div(row >> 4, a.blk_mul, a.blk_sh);
+            // (a page outside the pool: NaN, from the scale)
+            ksc[t] = page < 0 ? 255u : ksb[pg * a.ks_bs + blk * a.ks_rs];
+            vsc[t] = page < 0 ? 255u : vsb[pg * a.vs_bs + blk * a.vs_rs];
+            const unsigned char *kp = kbase + pg * p.k_bs + (int64_t)(row + c) * p.k_rs + 16 * g;
+            const unsigned char *vp = vbase + pg * p.v_bs + (int64_t)row * p.v_rs;
+#pragma unroll
+            for (int j = 0; j < NJ; j++)
+                kreg[t][j] = 64 * j + 16 * g < p.d ? *(const i32x4 *)(kp + 64 * j) : i32x4{0, 0, 0, 0};
+#pragma unroll
+            for (int i = 0; i < NV / 2; i++) {
+                const int ci = lane + 64 * i, vr = ci / CPR, vc = ci % CPR * 16;
+                vreg[t * (NV / 2) + i] = vc < p.d ? *(const i32x4 *)(vp + (int64_t)vr * p.v_rs + vc) : i32x4{0, 0, 0, 0};
+            }
+        }
+    };
+
+    f32x4 o[NR][NDB];
+    float m_run[NR], l_run[NR];
+#pragma unroll
+    for (int r = 0; r < NR; r++) {
+        m_run[r] = -INFINITY;
+        l_run[r] = 0.f;
+#pragma unroll
+        for (int db = 0; db < NDB; db++) o[r][db] = f32x4{0, 0, 0, 0};
+    }
+    const float c2 = p.scale_log2;
+    char *vimg = smem + wave * Cfg::VB;
+    // transposed read: lane i of group g names row {4g + j, 16 + 4g + j - 4}[j = (i >> 1)], half i & 1 of a chunk
+    const int tj = c >> 1, trow = (tj < 4 ? 4 * g + tj : 12 + 4 * g + tj);
+    const char *tr_base = vimg + trow * DP + (c & 1) * 8;
+    const int tr_swz = kv8_swz<DP>(trow) << 4;
+
+    const int first = n0 + part;
+    if (first < n1) load_step(first);
+    for (int n = first; n < n1; n += parts) {
+        const int k0 = n * A_STEP;
+        const bool tail = k0 < vis_lo || k0 + A_STEP > vis_hi;   // keys that no row sees: V must not count, whatever stands there
+#pragma unroll
+        for (int i = 0; i < NV; i++) {
+            const int ci = lane + 64 * (i % (NV / 2)), vr = ci / CPR + 16 * (i / (NV / 2)), ch = ci % CPR;
+            if (tail && (k0 + vr < vis_lo || k0 + vr >= vis_hi)) vreg[i] = i32x4{0, 0, 0, 0};
+            *(i32x4 *)(vimg + vr * DP + ((ch ^ kv8_swz<DP>(vr)) << 4)) = vreg[i];
+        }
+        const float ks[2] = {e8m0_to_f32(ksc[0]), e8m0_to_f32(ksc[1])}, vs[2] = {e8m0_to_f32(vsc[0]), e8m0_to_f32(vsc[1])};
+        f32x4 s[NR][2];
+#pragma unroll
+        for (int t = 0; t < 2; t++) {
+#pragma unroll
+            for (int r = 0; r < NR; r++) s[r][t] = f32x4{0, 0, 0, 0};
+#pragma unroll
+            for (int j = 0; j < NJ; j++) {
+                const i32x4 k_lo = kv8_to16<BF16>(i32x2{kreg[t][j][0], kreg[t][j][1]}, ks[t]);
+                const i32x4 k_hi = kv8_to16<BF16>(i32x2{kreg[t][j][2], kreg[t][j][3]}, ks[t]);
+#pragma unroll
+                for (int r = 0; r < NR; r++) {
+                    s[r][t] = mma16<BF16>(k_lo, qf[r][2 * j], s[r][t]);
+                    s[r][t] = mma16<BF16>(k_hi, qf[r][2 * j + 1], s[r][t]);
+                }
+            }
+        }
+        if (n + parts < n1) load_step(n + parts);
+
+        bool need = p.alibi_slopes || k0 + A_STEP > sk;
+        if (edge_r) need = need || (k0 + A_STEP > pos_lo + 1 + sk - sq + p.wr);
+        if (p.is_local) need = need || (k0 < pos_hi + sk - sq - p.wl);
+        i32x4 pf[NR];
+#pragma unroll
+        for (int r = 0; r < NR; r++) {
+            if (need) {
+                const int lo = p.is_local ? max(0, pos[r] + sk - sq - p.wl) : 0;
+                const int hi = edge_r ? min(sk, pos[r] + 1 + sk - sq + p.wr) : sk;
+#pragma unroll
+                for (int t = 0; t < 2; t++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const int key = k0 + 16 * t + 4 * g + i;
+                        float x = s[r][t][i];
+                        if (p.alibi_slopes)
+                            x = p.is_causal ? x + slope[r] * (float)key : x - slope[r] * fabsf((float)(pos[r] + sk - sq - key));
+                        s[r][t][i] = (key >= lo && key < hi) ? x : -INFINITY;
+                    }
+            }
+            float mx = fmaxf(fmaxf(fmaxf(s[r][0][0], s[r][0][1]), fmaxf(s[r][0][2], s[r][0][3])),
+                             fmaxf(fmaxf(s[r][1][0], s[r][1][1]), fmaxf(s[r][1][2], s[r][1][3])));
+            mx = quad_max(mx);
+            // the reference point of the exponentials follows the maximum lazily (P stays under 2^4)
+            if (__any((mx - m_run[r]) * c2 > 4.f)) {
+                const float m_new = fmaxf(m_run[r], mx);
+                const float alpha = __builtin_amdgcn_exp2f((m_run[r] - (m_new == -INFINITY ? 0.f : m_new)) * c2);
+                l_run[r] *= alpha;
+#pragma unroll
+                for (int db = 0; db < NDB; db++) o[r][db] *= alpha;
+                m_run[r] = m_new;
+            }
+            const float mc = (m_run[r] == -INFINITY ? 0.f : m_run[r]) * c2;
+            float sum = 0.f;
+#pragma unroll
+            for (int t = 0; t < 2; t++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r][t][i], c2, -mc));
+                    s[r][t][i] = e;
+                    sum += e;
+                }
+            l_run[r] += sum;
+#pragma unroll
+            for (int t = 0; t < 2; t++) {
+                pf[r][2 * t] = pack2<BF16>(s[r][t][0], s[r][t][1]);
+                pf[r][2 * t + 1] = pack2<BF16>(s[r][t][2], s[r][t][3]);
+            }
+        }
+#pragma unroll
+        for (int db = 0; db < NDB; db++) {
+            const i32x2 vt = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+                (__attribute__((address_space(3))) i32x2 *)(tr_base + ((db << 4) ^ tr_swz)));
+            i32x4 vf;
+            const i32x4 lo = kv8_to16<BF16>(i32x2{vt[0], 0}, vs[0]), hi = kv8_to16<BF16>(i32x2{vt[1], 0}, vs[1]);
+            vf[0] = lo[0]; vf[1] = lo[1]; vf[2] = hi[0]; vf[3] = hi[1];
+#pragma unroll
+            for (int r = 0; r < NR; r++) o[r][db] = mma16<BF16>(vf, pf[r], o[r][db]);
+        }
+    }
+
+    // ---- merge the waves of a head: weights from the maxima and sums, then 16 rows at a time ----
+    float *ml = (float *)(smem + Cfg::MAIN);     // [wave][row][2]
+#pragma unroll
+    for (int r = 0; r < NR; r++) {
+        const float l = quad_sum(l_run[r]);
+        if (g == 0) {
+            ml[((wave * NR + r) * 16 + c) * 2] = m_run[r];
+            ml[((wave * NR + r) * 16 + c) * 2 + 1] = l;
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < NR; r++) {
+        __syncthreads();                          // statistics written; V images and the rows before are done with
+        float m_all = -INFINITY, l_all = 0.f;
+        for (int w = 0; w < parts; w++) m_all = fmaxf(m_all, ml[(((w * hpw + whead) * NR + r) * 16 + c) * 2]);
+        const float m_fin = m_all == -INFINITY ? 0.f : m_all;
+        for (int w = 0; w < parts; w++) {
+            const float *e = ml + (((w * hpw + whead) * NR + r) * 16 + c) * 2;
+            l_all += e[1] * __builtin_amdgcn_exp2f((e[0] - m_fin) * c2);
+        }
+        const bool none = m_all == -INFINITY && l_all == 0.f;
+        const float f = none ? 0.f : __builtin_amdgcn_exp2f((m_run[r] - m_fin) * c2) / l_all;
+        char *ob = smem + wave * 16 * Cfg::O_ROWB + c * Cfg::O_ROWB + g * 16;
+#pragma unroll
+        for (int db = 0; db < NDB; db++) *(f32x4 *)(ob + db * 64) = o[r][db] * f;
+        const int row = q0 + 16 * r + c;
+        if (part == 0 && g == 0 && row < rows)
+            lse[stat_at(hk, row)] = none ? (is_split ? -INFINITY : INFINITY) : m_all * p.scale + __logf(l_all);
+        __syncthreads();
+        for (int i = tid; i < hpw * 16 * (DP / 8); i += A_NT) {
+            const int ch = i % (DP / 8), rr = i / (DP / 8) % 16, hs = i / (DP / 8) / 16;
+            const int orow = q0 + 16 * r + rr, head = hblock * hpw + hs;
+            if (orow >= rows || ch * 8 >= p.d) continue;
+            f32x4 a0 = {0, 0, 0, 0}, a1 = {0, 0, 0, 0};
+            for (int w = 0; w < parts; w++) {
+                const char *src = smem + ((w * hpw + hs) * 16 + rr) * Cfg::O_ROWB + ch * 32;
+                a0 += *(const f32x4 *)src;
+                a1 += *(const f32x4 *)(src + 16);
+            }
+            if (is_split) {
+                float *dst = p.oaccum + stat_at(head, orow) * p.d + ch * 8;
+                *(f32x4 *)dst = a0;
+                *(f32x4 *)(dst + 4) = a1;
+            } else {
+                i32x4 w;
+                w[0] = pack2<BF16>(a0[0], a0[1]); w[1] = pack2<BF16>(a0[2], a0[3]);
+                w[2] = pack2<BF16>(a1[0], a1[1]); w[3] = pack2<BF16>(a1[2], a1[3]);
+                *(i32x4 *)(og + (int64_t)(orow / ratio) * p.o_rs + (int64_t)(head * ratio + orow % ratio) * p.o_hs + ch * 8) = w;
+            }
+        }
+    }
+}
+
+template <int DP, bool BF16, int NR>
+static hipError_t launch_kv8(const KV8Params &a, hipStream_t stream) {
+    const KParams &p = a.p;
+    const int n_mblocks = (p.seqlen_q * p.h_ratio + 16 * NR - 1) / (16 * NR);
+    const long long blocks = (long long)n_mblocks * p.b * (p.h_k / a.heads_per_wg) * p.num_splits;
+    if (blocks <= 0) return hipSuccess;
+    if (blocks > 0x7fffffffLL) return hipErrorInvalidValue;
+    auto kern = fwd_kv8_kernel<DP, BF16, NR>;
+    constexpr int lds = Kv8Cfg<DP, NR>::LDS_BYTES;
+    static std::atomic<uint64_t> lds_set{0};
+    if (hipError_t e = set_dyn_lds_once((const void *)kern, lds, lds_set); e != hipSuccess) return e;
+    hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3(A_NT), lds, stream, a, n_mblocks);
+    return hipGetLastError();
+}
+
+template <int DP, bool BF16>
+static hipError_t launch_kv8_rows(const KV8Params &a, hipStream_t stream) {
+    const int rows = a.p.seqlen_q * a.p.h_ratio;
+    if constexpr (DP == 256) {
+        return launch_kv8<DP, BF16, 1>(a, stream);   // (the accumulators of 32 rows do not fit beside the loads)
+    } else {
+        if (rows <= 16) return launch_kv8<DP, BF16, 1>(a, stream);
+        return launch_kv8<DP, BF16, 2>(a, stream);
+    }
+}
+
+// Adjacent KV heads of a workgroup: a key's codes of one head are d bytes, and reads of 512 contiguous bytes
+// are what keeps HBM busy.
+int kv8_heads_per_wg(int d, int h_k) {
+    int n = 1;
+    while (n < 8 && n * d < 512 && h_k % (2 * n) == 0) n *= 2;
+    return n;
+}
+
+hipError_t run_fwd_kv8(const KV8Params &a, hipStream_t stream) {
+    const bool bf = a.p.is_bf16;
+    if (a.p.d <= 64) return bf ? launch_kv8_rows<64, true>(a, stream) : launch_kv8_rows<64, false>(a, stream);
+    if (a.p.d <= 128) return bf ? launch_kv8_rows<128, true>(a, stream) : launch_kv8_rows<128, false>(a, stream);
+    return bf ? launch_kv8_rows<256, true>(a, stream) : launch_kv8_rows<256, false>(a, stream);
+}
+
+}  // namespace vfa

@@ -1,0 +1,263 @@
+// Writing tokens to an 8-bit KV cache and reading it back (see vfa_kv8.h for the format).
+//
+// Both are copies: 2 bytes in and 1 out per element, or 1 in and 2 out, bound by HBM (by the launch for a
+// decode step's few tokens).
+#include "vfa_kv8.h"
+#include <algorithm>
+
+namespace vfa {
+
+constexpr int Q_NT = 256, Q_NW = Q_NT / 64;
+constexpr int Q_KEEP = 8;        // rows a wave keeps in registers between the maximum and the encoding
+
+// exponent of the least power-of-two scale that brings `amax` to at most 448 = 1.75 * 2^8
+__device__ __forceinline__ int kv8_exponent(float amax) {
+    const unsigned u = __float_as_uint(amax);
+    const int x = (int)(u >> 23) - 127;
+    return max(KV8_EMIN, x - 8 + ((u & 0x7fffffu) > 0x600000u ? 1 : 0));
+}
+__device__ __forceinline__ float exp2_int(int e) { return __uint_as_float((unsigned)(e + 127) << 23); }
+
+// 8 values of 16 bits times `inv` -> 8 codes, rounded to nearest even once (the product is exact).  NaN and
+// the infinities become NaN codes (e4m3 has no infinity).  `lim`: 448, or 240 where the next code would
+// stand for 2^16 (fp16) or 2^128 (bf16) and could not be read back as a finite value.
+template <bool BF16>
+__device__ __forceinline__ i32x2 kv8_encode(i32x4 x, float inv, float lim) {
+    float y[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        const unsigned short h = (unsigned short)((unsigned)x[i >> 1] >> (16 * (i & 1)));
+        const float v = to_f32<BF16>(h) * inv;
+        const float m = fabsf(v);
+        y[i] = (m > lim && m < INFINITY) ? copysignf(lim, v) : v;
+    }
+    i32x2 c;
+#pragma unroll
+    for (int w = 0; w < 2; w++) {
+        int t = __builtin_amdgcn_cvt_pk_fp8_f32(y[4 * w], y[4 * w + 1], 0, false);
+        c[w] = __builtin_amdgcn_cvt_pk_fp8_f32(y[4 * w + 2], y[4 * w + 3], t, true);
+    }
+    return c;
+}
+
+// 8 codes times `f` (a power of two <= 1): the block's scale has grown
+__device__ __forceinline__ i32x2 kv8_recode(i32x2 c, float f) {
+    i32x2 o;
+#pragma unroll
+    for (int w = 0; w < 2; w++) {
+        typedef float f32x2 __attribute__((ext_vector_type(2)));
+        const f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8(c[w], false), hi = __builtin_amdgcn_cvt_pk_f32_fp8(c[w], true);
+        int t = __builtin_amdgcn_cvt_pk_fp8_f32(lo[0] * f, lo[1] * f, 0, false);
+        o[w] = __builtin_amdgcn_cvt_pk_fp8_f32(hi[0] * f, hi[1] * f, t, true);
+    }
+    return o;
+}
+
+// largest finite magnitude of 8 values, as a bit pattern (16-bit floats order like their bits)
+template <bool BF16>
+__device__ __forceinline__ int amax_bits(i32x4 x, int m) {
+    constexpr int INF = BF16 ? 0x7f80 : 0x7c00;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const int a = x[i] & 0x7fff, b = (x[i] >> 16) & 0x7fff;
+        m = max(m, a < INF ? a : 0);
+        m = max(m, b < INF ? b : 0);
+    }
+    return m;
+}
+
+// One workgroup per (sequence, touched block of tokens, group of heads, K or V).  LPR lanes hold one head's
+// row (8 elements each), so a wave covers 64 / LPR adjacent heads of a token, whose rows are adjacent in
+// memory; the four waves take the block's rows in turn.  The block belongs to this workgroup alone, so its
+// scale is found (maximum over lanes, then over waves through LDS) and its codes are written without
+// atomics, and nothing depends on the order of workgroups.
+template <bool BF16, int LPR>
+__global__ void __launch_bounds__(Q_NT)
+kv8_quantize_kernel(const KV8Params a, const int n_blocks, const int n_hgroups) {
+    const KParams &p = a.p;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    int64_t L = blockIdx.x;
+    const bool is_v = L & 1; L >>= 1;
+    const int hg = (int)(L % n_hgroups); L /= n_hgroups;
+    const int j = (int)(L % n_blocks);
+    const int bidb = (int)(L / n_blocks);
+
+    const int start = kv8_cached(a, bidb);
+    int64_t src0;                        // first new token's row
+    int n_new;
+    if (a.cu_new) { src0 = a.cu_new[bidb]; n_new = a.cu_new[bidb + 1] - a.cu_new[bidb]; }
+    else { src0 = 0; n_new = p.seqlen_knew; }
+    const int end = (int)min((int64_t)start + max(n_new, 0), (int64_t)a.cap);
+    const int lo = kv8_div(start >> 4, a.blk_mul, a.blk_sh) * a.blk + j * a.blk;
+    if (lo >= end || end <= start) return;
+    const int r0 = max(start, lo), r1 = min(end, lo + a.blk);
+    const int page = kv8_page(a, bidb, lo);
+    if (page < 0) return;                // the table names no page of the pool: nothing is written
+
+    const int head = hg * (64 / LPR) + lane / LPR, ch = lane % LPR;
+    const bool ok = ch * 8 < p.d && head < p.h_k;
+    const int hsafe = min(head, p.h_k - 1), csafe = ch * 8 < p.d ? ch * 8 : 0;
+    const int in_page = kv8_row_in_page(a, lo);
+    const int64_t rs = is_v ? p.v_rs : p.k_rs;
+    unsigned char *codes = (unsigned char *)(is_v ? p.v : p.k) + (int64_t)page * (is_v ? p.v_bs : p.k_bs) +
+                           (int64_t)in_page * rs + (int64_t)hsafe * (is_v ? p.v_hs : p.k_hs) + csafe;   // row lo
+    unsigned char *scale = (is_v ? a.vs : a.ks) + (int64_t)page * (is_v ? a.vs_bs : a.ks_bs) +
+                           (int64_t)kv8_div(in_page >> 4, a.blk_mul, a.blk_sh) * (is_v ? a.vs_rs : a.ks_rs) +
+                           (int64_t)hsafe * (is_v ? a.vs_hs : a.ks_hs);
+    const int64_t nrs = is_v ? p.vnew_rs : p.knew_rs;
+    const unsigned short *src = (const unsigned short *)(is_v ? p.vnew : p.knew) +
+                                (a.cu_new ? src0 * nrs : (int64_t)bidb * (is_v ? p.vnew_bs : p.knew_bs)) -
+                                (int64_t)start * nrs + (int64_t)hsafe * (is_v ? p.vnew_hs : p.knew_hs) + csafe;   // row of token 0
+
+    const bool holds = start > lo;       // the block has tokens already: its scale only grows
+    const int e_old = holds ? (int)*scale - 127 : KV8_EMIN;
+
+    i32x4 x[Q_KEEP];
+    int m = 0;
+#pragma unroll
+    for (int i = 0; i < Q_KEEP; i++) {
+        const int row = r0 + wave + Q_NW * i;
+        x[i] = (ok && row < r1) ? *(const i32x4 *)(src + row * nrs) : i32x4{0, 0, 0, 0};
+    }
+#pragma unroll
+    for (int i = 0; i < Q_KEEP; i++) m = amax_bits<BF16>(x[i], m);
+    for (int row = r0 + wave + Q_NW * Q_KEEP; row < r1; row += Q_NW)
+        m = amax_bits<BF16>(ok ? *(const i32x4 *)(src + row * nrs) : i32x4{0, 0, 0, 0}, m);
+#pragma unroll
+    for (int off = LPR / 2; off > 0; off >>= 1) m = max(m, __shfl_xor(m, off));
+    __shared__ int s_m[Q_NW][64 / LPR];
+    if (ch == 0) s_m[wave][lane / LPR] = m;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < Q_NW; w++) m = max(m, s_m[w][lane / LPR]);
+    if (!ok) return;
+
+    int e = kv8_exponent(to_f32<BF16>((unsigned short)m));
+    if (holds) e = max(e, e_old);
+    // past this exponent the largest code would stand for a value the 16-bit type does not have
+    constexpr int E_TOP = BF16 ? 120 : 8;
+    const float inv = exp2_int(-e), lim = e >= E_TOP ? 240.f : 448.f;
+    if (holds && e > e_old) {
+        const float f = e - e_old > 126 ? 0.f : exp2_int(e_old - e);
+        for (int row = wave; row < start - lo; row += Q_NW) {
+            i32x2 *c = (i32x2 *)(codes + row * rs);
+            *c = kv8_recode(*c, f);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < Q_KEEP; i++) {
+        const int row = r0 + wave + Q_NW * i;
+        if (row < r1) *(i32x2 *)(codes + (row - lo) * rs) = kv8_encode<BF16>(x[i], inv, lim);
+    }
+    for (int row = r0 + wave + Q_NW * Q_KEEP; row < r1; row += Q_NW)
+        *(i32x2 *)(codes + (row - lo) * rs) = kv8_encode<BF16>(*(const i32x4 *)(src + row * nrs), inv, lim);
+    if (wave == 0 && ch == 0) *scale = (unsigned char)(e + 127);
+}
+
+hipError_t run_kv8_quantize(const KV8Params &a, hipStream_t stream) {
+    const KParams &p = a.p;
+    if (p.seqlen_knew <= 0) return hipSuccess;
+    const int lpr = p.d <= 64 ? 8 : p.d <= 128 ? 16 : 32;
+    const int n_hgroups = (p.h_k + 64 / lpr - 1) / (64 / lpr);
+    const int n_blocks = (p.seqlen_knew + a.blk - 2) / a.blk + 1;   // a run of n tokens touches at most so many
+    const long long blocks = 2LL * p.b * n_blocks * n_hgroups;
+    if (blocks > 0x7fffffffLL) return hipErrorInvalidValue;
+    const dim3 grid((unsigned)blocks), wg(Q_NT);
+#define VFA_Q(LPR)                                                                                                          \
+    if (p.is_bf16) hipLaunchKernelGGL((kv8_quantize_kernel<true, LPR>), grid, wg, 0, stream, a, n_blocks, n_hgroups);       \
+    else hipLaunchKernelGGL((kv8_quantize_kernel<false, LPR>), grid, wg, 0, stream, a, n_blocks, n_hgroups)
+    if (lpr == 8) { VFA_Q(8); } else if (lpr == 16) { VFA_Q(16); } else { VFA_Q(32); }
+#undef VFA_Q
+    return hipGetLastError();
+}
+
+constexpr int D_NT = 256;
+
+// A workgroup takes `tpw` output rows (tokens): its first threads find each row's sequence (ragged: by
+// bisection of the offsets), page and scale row, then all threads copy 16 codes at a time, adjacent threads
+// adjacent chunks of a token's heads.  Rows behind a sequence's tokens are zeros.
+struct RowOf {
+    int64_t k, v, ks, vs, out_k, out_v;   // k < 0: no token here
+};
+
+template <bool BF16>
+__global__ void __launch_bounds__(D_NT)
+kv8_dequantize_kernel(const KV8Params a, const int tpw, const int cph) {
+    __shared__ RowOf s_row[64];
+    const KParams &p = a.p;
+    const int tid = threadIdx.x;
+    const int64_t first = (int64_t)blockIdx.x * tpw;
+    if (tid < tpw && first + tid < a.rows_out) {
+        const int64_t t = first + tid;
+        int seq;
+        int64_t tok;
+        RowOf r;
+        if (a.cu_out) {
+            int lo = 0, hi = p.b;          // last sequence that starts at or before t
+            while (hi - lo > 1) {
+                const int mid = (lo + hi) >> 1;
+                if (a.cu_out[mid] <= t) lo = mid; else hi = mid;
+            }
+            seq = lo;
+            tok = t - a.cu_out[seq];
+            if (t >= a.cu_out[p.b]) tok = a.cap;   // behind the last sequence
+            r.out_k = t * a.ko_rs; r.out_v = t * a.vo_rs;
+        } else {
+            seq = (int)(t / a.seqlen_out);
+            tok = t - (int64_t)seq * a.seqlen_out;
+            r.out_k = seq * a.ko_bs + tok * a.ko_rs; r.out_v = seq * a.vo_bs + tok * a.vo_rs;
+        }
+        r.k = -1; r.v = r.ks = r.vs = 0;
+        if (tok >= 0 && tok < kv8_cached(a, seq)) {
+            const int page = kv8_page(a, seq, (int)tok);
+            if (page >= 0) {
+                const int row = kv8_row_in_page(a, (int)tok), blk = kv8_div(row >> 4, a.blk_mul, a.blk_sh);
+                r.k = page * p.k_bs + row * p.k_rs;   r.v = page * p.v_bs + row * p.v_rs;
+                r.ks = page * a.ks_bs + blk * a.ks_rs; r.vs = page * a.vs_bs + blk * a.vs_rs;
+            } else {
+                r.k = -2;                             // a page outside the pool: NaN
+            }
+        }
+        s_row[tid] = r;
+    }
+    __syncthreads();
+    const int per = p.h_k * cph;                      // chunks of 16 elements of a token
+    const int n = (int)min((int64_t)tpw, a.rows_out - first) * per;
+    for (int i = tid; i < n; i += D_NT) {
+        const int t = i / per, c = i - t * per;
+        const int head = c / cph, col = (c - head * cph) * 16;
+        const RowOf &r = s_row[t];
+        i32x4 k = {0, 0, 0, 0}, v = k;
+        float ks = 1.f, vs = 1.f;
+        if (r.k >= 0) {
+            k = *(const i32x4 *)((const unsigned char *)p.k + r.k + head * p.k_hs + col);
+            v = *(const i32x4 *)((const unsigned char *)p.v + r.v + head * p.v_hs + col);
+            ks = e8m0_to_f32(a.ks[r.ks + head * a.ks_hs]);
+            vs = e8m0_to_f32(a.vs[r.vs + head * a.vs_hs]);
+        } else if (r.k == -2) {
+            k = i32x4{0x7f7f7f7f, 0x7f7f7f7f, 0x7f7f7f7f, 0x7f7f7f7f};
+            v = k;
+        }
+        unsigned short *ko = (unsigned short *)a.k_out + r.out_k + head * a.ko_hs + col;
+        unsigned short *vo = (unsigned short *)a.v_out + r.out_v + head * a.vo_hs + col;
+        *(i32x4 *)ko = kv8_to16<BF16>(i32x2{k[0], k[1]}, ks);
+        *(i32x4 *)(ko + 8) = kv8_to16<BF16>(i32x2{k[2], k[3]}, ks);
+        *(i32x4 *)vo = kv8_to16<BF16>(i32x2{v[0], v[1]}, vs);
+        *(i32x4 *)(vo + 8) = kv8_to16<BF16>(i32x2{v[2], v[3]}, vs);
+    }
+}
+
+hipError_t run_kv8_dequantize(const KV8Params &a, hipStream_t stream) {
+    const KParams &p = a.p;
+    if (a.rows_out <= 0) return hipSuccess;
+    const int cph = p.d / 16, per = p.h_k * cph;
+    // enough rows that every thread has a chunk or more, at most the 64 whose places fit in LDS
+    const int tpw = std::min(64, std::max(1, 4 * D_NT / per));
+    const long long blocks = (a.rows_out + tpw - 1) / tpw;
+    if (blocks > 0x7fffffffLL) return hipErrorInvalidValue;
+    if (p.is_bf16) hipLaunchKernelGGL(kv8_dequantize_kernel<true>, dim3((unsigned)blocks), dim3(D_NT), 0, stream, a, tpw, cph);
+    else hipLaunchKernelGGL(kv8_dequantize_kernel<false>, dim3((unsigned)blocks), dim3(D_NT), 0, stream, a, tpw, cph);
+    return hipGetLastError();
+}
+
+}  // namespace vfa

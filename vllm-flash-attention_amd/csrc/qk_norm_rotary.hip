@@ -1,0 +1,323 @@
+// RMS norm of every query / key head and the position rotation in one pass, forward and backward.
+//
+//   forward   r = 1 / sqrt(mean(x^2) + eps),  n = x r w,  y = R n
+//   backward  g = R^T dy,  dx = r (g w - x r^2 mean(g w x)),  dw = sum over rows of g x r
+//
+// R turns the pairs (2i, 2i + 1) (interleaved) or (i, i + rd / 2) by the token's angles and leaves the
+// columns from rd on alone.  Everything is fp32 from the 16-bit inputs to the one rounding of the result:
+// the normalised value is not rounded in front of the rotation.
+//
+// HBM-bound: the forward reads and writes q and k once; the backward reads x and dy and writes dx, and
+// needs nothing else from the forward (r is recomputed from the x it reads anyway).  A head row is held by
+// LPR lanes, 8 elements (16 bytes) each, so that sums over the row are log2(LPR) lane exchanges and the
+// partner of a rotation pair (rd / 16 lanes away, as rd is a multiple of 16) is one exchange of the packed
+// 16-bit words.  A wave stays with one token while it walks that token's heads: angles and weights are
+// loaded once per wave and the rows of adjacent heads are adjacent in memory.
+#include "vfa_qk_norm.h"
+#include <algorithm>
+
+namespace vfa {
+
+constexpr int N_NT = 256, N_NW = N_NT / 64;
+
+template <bool BF16>
+__device__ __forceinline__ void unpack8(i32x4 x, float f[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; i++) f[i] = to_f32<BF16>((unsigned short)((unsigned)x[i >> 1] >> (16 * (i & 1))));
+}
+template <bool BF16>
+__device__ __forceinline__ i32x4 pack8(const float f[8]) {
+    i32x4 w;
+#pragma unroll
+    for (int i = 0; i < 4; i++) w[i] = pack2<BF16>(f[2 * i], f[2 * i + 1]);
+    return w;
+}
+// element i of a table or weight held in fp32 or in the tensors' type
+template <bool BF16>
+__device__ __forceinline__ float ld_f(const void *p, int64_t i, int f32) {
+    return f32 ? ((const float *)p)[i] : to_f32<BF16>(((const unsigned short *)p)[i]);
+}
+template <int LPR>
+__device__ __forceinline__ float row_sum(float x) {
+#pragma unroll
+    for (int off = LPR / 2; off > 0; off >>= 1) x += __shfl_xor(x, off);
+    return x;
+}
+
+// What a lane needs of the rotation for its 8 columns of a token.
+struct Turn {
+    float c[8], s[8];            // interleaved: the first 4 of each; outside rd: 1 and 0
+    int partner;                 // lane that holds the other half's columns (pairs (i, i + rd / 2)), or own
+};
+
+template <bool BF16>
+__device__ __forceinline__ void load_turn(const QKNormParams &p, int pos, int ch, int lane, Turn &t) {
+    const int col = ch * 8, half = p.rd / 2;
+    t.partner = lane;
+#pragma unroll
+    for (int i = 0; i < 8; i++) { t.c[i] = 1.f; t.s[i] = 0.f; }
+    if (col >= p.rd) return;
+    if (pos >= p.table_rows) {                 // no such row: loud, and nothing is read
+#pragma unroll
+        for (int i = 0; i < 8; i++) t.c[i] = t.s[i] = __uint_as_float(0x7fc00000u);
+    }
+    const int64_t row = (int64_t)pos * half;
+    if (p.interleaved) {
+        if (pos < p.table_rows)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                t.c[i] = ld_f<BF16>(p.cos, row + col / 2 + i, p.table_f32);
+                t.s[i] = ld_f<BF16>(p.sin, row + col / 2 + i, p.table_f32);
+            }
+    } else {
+        const bool left = col < half;
+        t.partner = left ? lane + half / 8 : lane - half / 8;
+        if (pos < p.table_rows)
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                t.c[i] = ld_f<BF16>(p.cos, row + (left ? col : col - half) + i, p.table_f32);
+                t.s[i] = ld_f<BF16>(p.sin, row + (left ? col : col - half) + i, p.table_f32);
+            }
+        if (left)
+#pragma unroll
+            for (int i = 0; i < 8; i++) t.s[i] = -t.s[i];   // y = n c + partner s
+    }
+}
+
+// f turned (fwd) or turned back, with `o` the partner columns' values (pairs (i, i + rd / 2) only)
+__device__ __forceinline__ void turn8(const QKNormParams &p, const Turn &t, bool inside, float f[8], const float o[8], float sign) {
+    if (!inside) return;
+    if (p.interleaved) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const float a = f[2 * i], b = f[2 * i + 1], s = sign * t.s[i];
+            f[2 * i] = a * t.c[i] - b * s;
+            f[2 * i + 1] = a * s + b * t.c[i];
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++) f[i] = f[i] * t.c[i] + o[i] * (sign * t.s[i]);
+    }
+}
+
+__device__ __forceinline__ i32x4 from_lane(i32x4 x, int src) {
+    i32x4 o;
+#pragma unroll
+    for (int i = 0; i < 4; i++) o[i] = __shfl(x[i], src);
+    return o;
+}
+
+// item -> (token, part): a wave's U passes over 64 / LPR head rows each, of one token of q or of k
+struct Item {
+    int64_t tok;
+    int bi, si, head0, pos;
+};
+__device__ __forceinline__ Item find_item(const QKNormParams &p, int64_t item, int parts, int rows) {
+    Item it;
+    it.tok = item / parts;
+    it.head0 = (int)(item - it.tok * parts) * rows;
+    it.bi = (int)(it.tok / p.s);
+    it.si = (int)(it.tok - (int64_t)it.bi * p.s);
+    it.pos = p.positions ? p.positions[it.bi * p.pos_bs + it.si] : it.si;
+    return it;
+}
+
+template <bool BF16, int LPR, int U>
+__global__ void __launch_bounds__(N_NT)
+qk_norm_fwd_kernel(const QKNormParams p, const int64_t items_q, const int64_t items, const int parts_q, const int parts_k) {
+    constexpr int RPW = 64 / LPR;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    int64_t item = (int64_t)blockIdx.x * N_NW + wave;
+    if (item >= items) return;
+    const bool is_k = item >= items_q;
+    const QKNormTensor &t = p.t[is_k];
+    const Item it = find_item(p, is_k ? item - items_q : item, is_k ? parts_k : parts_q, RPW * U);
+    const int sub = lane / LPR, ch = lane % LPR, col = ch * 8;
+    const bool col_ok = col < p.d;
+
+    const unsigned short *xp = (const unsigned short *)t.x + it.bi * t.x_bs + it.si * t.x_rs + (col_ok ? col : 0);
+    unsigned short *yp = (unsigned short *)t.y + it.bi * t.y_bs + it.si * t.y_rs + col;
+    i32x4 x[U];
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        const int head = it.head0 + u * RPW + sub;
+        x[u] = (col_ok && head < t.h) ? *(const i32x4 *)(xp + head * t.x_hs) : i32x4{0, 0, 0, 0};
+    }
+    if (it.pos < 0) {                          // padding: zeros, whatever stands there
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int head = it.head0 + u * RPW + sub;
+            if (col_ok && head < t.h) *(i32x4 *)(yp + head * t.y_hs) = i32x4{0, 0, 0, 0};
+        }
+        return;
+    }
+    Turn tr;
+    load_turn<BF16>(p, it.pos, ch, lane, tr);
+    const bool inside = col < p.rd, pairs = inside && !p.interleaved;
+    float w[8], wo[8];
+    const int pcol = (tr.partner % LPR) * 8;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        w[i] = col_ok ? ld_f<BF16>(t.w, col + i, p.w_f32) : 0.f;
+        wo[i] = pairs ? ld_f<BF16>(t.w, pcol + i, p.w_f32) : 0.f;
+    }
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        const int head = it.head0 + u * RPW + sub;
+        float f[8], o[8], ss = 0.f;
+        unpack8<BF16>(x[u], f);
+#pragma unroll
+        for (int i = 0; i < 8; i++) ss += f[i] * f[i];
+        const float r = 1.f / sqrtf(row_sum<LPR>(ss) / (float)p.d + p.eps);
+        unpack8<BF16>(from_lane(x[u], tr.partner), o);
+#pragma unroll
+        for (int i = 0; i < 8; i++) { f[i] *= r * w[i]; o[i] *= r * wo[i]; }
+        turn8(p, tr, inside, f, o, 1.f);
+        if (col_ok && head < t.h) *(i32x4 *)(yp + head * t.y_hs) = pack8<BF16>(f);
+    }
+}
+
+// Backward.  The first blocks_q workgroups walk q's items, the others k's, so that a workgroup's partial dw
+// (registers over its items, then lanes and waves in a fixed order) is one side's; a second kernel adds the
+// partials in workgroup order: the same bits on every run.
+template <bool BF16, int LPR, int U>
+__global__ void __launch_bounds__(N_NT)
+qk_norm_bwd_kernel(const QKNormParams p, const int64_t items_q, const int64_t items_k, const int parts_q, const int parts_k) {
+    constexpr int RPW = 64 / LPR;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const bool is_k = (int)blockIdx.x >= p.blocks_q;
+    const QKNormTensor &t = p.t[is_k];
+    const int blk = is_k ? blockIdx.x - p.blocks_q : blockIdx.x, n_blk = is_k ? p.blocks_k : p.blocks_q;
+    const int64_t items = is_k ? items_k : items_q;
+    const int parts = is_k ? parts_k : parts_q;
+    const int sub = lane / LPR, ch = lane % LPR, col = ch * 8;
+    const bool col_ok = col < p.d, inside = col < p.rd;
+    float w[8], acc[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        w[i] = col_ok ? ld_f<BF16>(t.w, col + i, p.w_f32) : 0.f;
+        acc[i] = 0.f;
+    }
+    for (int64_t item = (int64_t)blk * N_NW + wave; item < items; item += (int64_t)n_blk * N_NW) {
+        const Item it = find_item(p, item, parts, RPW * U);
+        const unsigned short *xp = (const unsigned short *)t.x + it.bi * t.x_bs + it.si * t.x_rs + (col_ok ? col : 0);
+        const unsigned short *gp = (const unsigned short *)t.dy + it.bi * t.dy_bs + it.si * t.dy_rs + (col_ok ? col : 0);
+        unsigned short *yp = (unsigned short *)t.y + it.bi * t.y_bs + it.si * t.y_rs + col;
+        const bool pad = it.pos < 0;
+        i32x4 x[U], g[U];
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int head = it.head0 + u * RPW + sub;
+            const bool ok = col_ok && head < t.h && !pad;
+            x[u] = ok ? *(const i32x4 *)(xp + head * t.x_hs) : i32x4{0, 0, 0, 0};
+            g[u] = ok ? *(const i32x4 *)(gp + head * t.dy_hs) : i32x4{0, 0, 0, 0};
+        }
+        Turn tr;
+        load_turn<BF16>(p, pad ? 0 : it.pos, ch, lane, tr);
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int head = it.head0 + u * RPW + sub;
+            float f[8], q[8], o[8];
+            unpack8<BF16>(x[u], f);
+            unpack8<BF16>(g[u], q);
+            unpack8<BF16>(from_lane(g[u], tr.partner), o);
+            turn8(p, tr, inside, q, o, -1.f);             // g = R^T dy
+            float ss = 0.f, sg = 0.f;
+#pragma unroll
+            for (int i = 0; i < 8; i++) { ss += f[i] * f[i]; sg += q[i] * w[i] * f[i]; }
+            const float r = 1.f / sqrtf(row_sum<LPR>(ss) / (float)p.d + p.eps);
+            const float m = row_sum<LPR>(sg) / (float)p.d * r * r;
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                if (col_ok && head < t.h && !pad) acc[i] += q[i] * f[i] * r;
+                f[i] = r * (q[i] * w[i] - f[i] * m);
+            }
+            if (t.y && col_ok && head < t.h) *(i32x4 *)(yp + head * t.y_hs) = pad ? i32x4{0, 0, 0, 0} : pack8<BF16>(f);
+        }
+    }
+    if (!t.dw) return;
+    __shared__ float s_acc[N_NW][LPR * 8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+#pragma unroll
+        for (int off = 32; off >= LPR; off >>= 1) acc[i] += __shfl_xor(acc[i], off);
+        if (sub == 0) s_acc[wave][col + i] = acc[i];
+    }
+    __syncthreads();
+    for (int c = threadIdx.x; c < p.d; c += N_NT) {
+        float sum = 0.f;
+#pragma unroll
+        for (int v = 0; v < N_NW; v++) sum += s_acc[v][c];
+        p.dw_part[(int64_t)blockIdx.x * p.d + c] = sum;
+    }
+}
+
+// dw of q (blockIdx.y 0) and of k (1): 8 columns per workgroup, 32 threads a column, partials in a fixed order
+template <bool BF16>
+__global__ void __launch_bounds__(N_NT)
+qk_norm_dw_kernel(const QKNormParams p) {
+    const QKNormTensor &t = p.t[blockIdx.y];
+    if (!t.dw) return;
+    const int c = blockIdx.x * 8 + (threadIdx.x & 7), part = threadIdx.x >> 3;
+    const int first = blockIdx.y ? p.blocks_q : 0, n = blockIdx.y ? p.blocks_k : p.blocks_q;
+    float sum = 0.f;
+    for (int i = part; i < n; i += N_NT / 8) sum += p.dw_part[(int64_t)(first + i) * p.d + c];
+    __shared__ float s[N_NT];
+    s[threadIdx.x] = sum;
+    __syncthreads();
+    if (threadIdx.x < 8) {
+        for (int i = 1; i < N_NT / 8; i++) sum += s[i * 8 + threadIdx.x];
+        if (p.w_f32) ((float *)t.dw)[c] = sum;
+        else ((unsigned short *)t.dw)[c] = (unsigned short)(pack2<BF16>(sum, 0.f) & 0xffff);
+    }
+}
+
+static int lanes_per_row(int d) { return d <= 64 ? 8 : d <= 128 ? 16 : 32; }
+constexpr int N_U = 2;           // passes of a wave over a token's heads
+
+static int head_parts(const QKNormParams &p, int side) {
+    const int rows = 64 / lanes_per_row(p.d) * N_U;
+    return (p.t[side].h + rows - 1) / rows;
+}
+
+// Workgroups of the backward per side: enough that every CU has work, few enough that the partial sums of
+// dw stay small beside q and k.
+void qk_norm_bwd_blocks(QKNormParams &p, int cus) {
+    for (int side = 0; side < 2; side++) {
+        const long long items = (long long)p.b * p.s * head_parts(p, side);
+        const long long want = (items + N_NW - 1) / N_NW;
+        (side ? p.blocks_k : p.blocks_q) = (int)std::max(1LL, std::min(want, 4LL * cus));
+    }
+}
+
+template <bool BF16, int LPR>
+static hipError_t launch(const QKNormParams &p, bool bwd, hipStream_t stream) {
+    const int parts_q = head_parts(p, 0), parts_k = head_parts(p, 1);
+    const int64_t items_q = (int64_t)p.b * p.s * parts_q, items_k = (int64_t)p.b * p.s * parts_k;
+    if (!bwd) {
+        const int64_t blocks = (items_q + items_k + N_NW - 1) / N_NW;
+        if (blocks > 0x7fffffff) return hipErrorInvalidValue;
+        hipLaunchKernelGGL((qk_norm_fwd_kernel<BF16, LPR, N_U>), dim3((unsigned)blocks), dim3(N_NT), 0, stream, p, items_q,
+                           items_q + items_k, parts_q, parts_k);
+        return hipGetLastError();
+    }
+    hipLaunchKernelGGL((qk_norm_bwd_kernel<BF16, LPR, N_U>), dim3((unsigned)(p.blocks_q + p.blocks_k)), dim3(N_NT), 0, stream, p,
+                       items_q, items_k, parts_q, parts_k);
+    if (p.t[0].dw || p.t[1].dw) {
+        if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+        hipLaunchKernelGGL(qk_norm_dw_kernel<BF16>, dim3((unsigned)(p.d / 8), 2), dim3(N_NT), 0, stream, p);
+    }
+    return hipGetLastError();
+}
+
+hipError_t run_qk_norm_rotary(const QKNormParams &p, bool bwd, hipStream_t stream) {
+    if ((int64_t)p.b * p.s <= 0) {
+        // no token: the weights' gradients are zero, and the backward's kernels write that
+        if (!bwd) return hipSuccess;
+    }
+    const int lpr = lanes_per_row(p.d);
+    if (p.is_bf16) return lpr == 8 ? launch<true, 8>(p, bwd, stream) : lpr == 16 ? launch<true, 16>(p, bwd, stream) : launch<true, 32>(p, bwd, stream);
+    return lpr == 8 ? launch<false, 8>(p, bwd, stream) : lpr == 16 ? launch<false, 16>(p, bwd, stream) : launch<false, 32>(p, bwd, stream);
+}
+
+}  // namespace vfa

@@ -17,6 +17,7 @@
 #include <limits>
 #include <optional>
 #include <vector>
+#include <torch/csrc/Dtype.h>
 
 #include "vfa.h"
 
@@ -836,6 +837,366 @@ std::vector<Tensor> varlen_bwd(const Tensor &dout, const Tensor &q, const Tensor
                     is_causal, window_size_left, window_size_right, deterministic, gen_, rng_state);
 }
 
+// ---------------------------------------------------------------------------------------------
+// 8-bit KV cache (vfa_kv8_params) and the q / k norm + rotation: no counterpart in the reference
+
+// Strides of dims that hold one index mean nothing and need not be aligned.
+int64_t stride_of(const Tensor &t, int64_t dim) { return t.size(dim) > 1 ? t.stride(dim) : 0; }
+
+// A 16-bit tensor as the kernels read it: last dim contiguous, 16-byte aligned rows; copied if it is not.
+Tensor aligned_rows(const Tensor &t) {
+    bool ok = ((uintptr_t)t.data_ptr() & 15) == 0 && (t.size(-1) <= 1 || t.stride(-1) == 1);
+    for (int64_t i = 0; i + 1 < t.dim(); i++) ok = ok && stride_of(t, i) % 8 == 0;
+    return ok ? t : t.clone(at::MemoryFormat::Contiguous);
+}
+
+void expect_with(const Tensor &t, const char *name, const Tensor &other) {
+    expect_gpu(t, name);
+    TORCH_CHECK(t.device() == other.device(), name, " must be on the device of the other tensors, ", other.device(), ", got ", t.device());
+}
+void expect_int32(const Tensor &t, const char *name, const Tensor &other) {
+    TORCH_CHECK(t.scalar_type() == at::kInt, name, " must have dtype int32");
+    expect_with(t, name, other);
+    expect_contig(t, name);
+}
+
+// Cache, scales, lengths and pages; returns the batch size.
+int64_t set_kv8_cache(vfa_kv8_params &P, const Tensor &kc, const Tensor &vc, const Tensor &ks, const Tensor &vs, int64_t b,
+                      const OptTensor &seqlens_, const OptTensor &cache_batch_idx_, const OptTensor &block_table_) {
+    for (const Tensor *t : {&kc, &vc}) {
+        TORCH_CHECK(t->scalar_type() == at::kFloat8_e4m3fn, "k_cache and v_cache must have dtype float8_e4m3fn");
+        TORCH_CHECK(t->dim() == 4, "k_cache and v_cache must be 4-dimensional");
+        TORCH_CHECK(t->size(-1) <= 1 || t->stride(-1) == 1, "k_cache and v_cache must have contiguous last dimension");
+    }
+    expect_gpu(kc, "k_cache");
+    expect_with(vc, "v_cache", kc);
+    const bool paged = block_table_.has_value();
+    const int64_t pages = kc.size(0), rows = kc.size(1), hk = kc.size(2), d = kc.size(3);
+    TORCH_CHECK(pages > 0 && rows > 0 && hk > 0 && d > 0, "k_cache must not be empty");
+    TORCH_CHECK(vc.sizes() == kc.sizes(), "v_cache must have the shape of k_cache, ", kc.sizes(), ", got ", vc.sizes());
+    TORCH_CHECK(d <= 256 && d % 16 == 0, "8-bit KV cache: head dimension must be a multiple of 16, at most 256");
+    for (const Tensor *t : {&ks, &vs}) {
+        TORCH_CHECK(t->scalar_type() == at::kFloat8_e8m0fnu, "k_scale and v_scale must have dtype float8_e8m0fnu");
+        expect_with(*t, "k_scale / v_scale", kc);
+        TORCH_CHECK(t->dim() == 3 && t->size(0) == pages && t->size(2) == hk && t->sizes() == ks.sizes(),
+                    "k_scale and v_scale must have shape (", pages, ", blocks of tokens, ", hk, "), got ", t->sizes());
+    }
+    const int64_t nblk = ks.size(1);
+    TORCH_CHECK(nblk > 0 && rows % nblk == 0 && (rows / nblk) % 16 == 0,
+                "8-bit KV cache: the tokens per scale must be a multiple of 16 that divides the rows of a page (", rows, " rows, ", nblk, " scales)");
+    TORCH_CHECK(rows <= (1 << 30) && pages <= (1 << 30), "8-bit KV cache: too large");
+    P.a.k = kc.data_ptr(); P.a.v = vc.data_ptr();
+    P.a.k_batch_stride = stride_of(kc, 0); P.a.k_row_stride = stride_of(kc, 1); P.a.k_head_stride = stride_of(kc, 2);
+    P.a.v_batch_stride = stride_of(vc, 0); P.a.v_row_stride = stride_of(vc, 1); P.a.v_head_stride = stride_of(vc, 2);
+    P.k_scale = ks.data_ptr(); P.v_scale = vs.data_ptr();
+    P.k_scale_batch_stride = stride_of(ks, 0); P.k_scale_row_stride = stride_of(ks, 1); P.k_scale_head_stride = stride_of(ks, 2);
+    P.v_scale_batch_stride = stride_of(vs, 0); P.v_scale_row_stride = stride_of(vs, 1); P.v_scale_head_stride = stride_of(vs, 2);
+    P.scale_block = (int)(rows / nblk);
+    P.num_pages = (int)pages;
+    if (b < 0) {
+        TORCH_CHECK(seqlens_.has_value(), "cache_seqlens must be passed in");
+        b = seqlens_.value().numel();
+    }
+    TORCH_CHECK(b > 0, "batch size must be postive");
+    P.a.b = (int)b; P.a.h_k = (int)hk; P.a.d = (int)d;
+    if (seqlens_.has_value()) {
+        const Tensor &s = seqlens_.value();
+        expect_int32(s, "cache_seqlens", kc);
+        expect_shape(s, "cache_seqlens", {b});
+        P.a.cu_seqlens_k = s.data_ptr<int32_t>();
+    }
+    if (cache_batch_idx_.has_value()) {
+        TORCH_CHECK(!paged, "Paged KVcache does not support cache_batch_idx");
+        expect_int32(cache_batch_idx_.value(), "cache_batch_idx", kc);
+        expect_shape(cache_batch_idx_.value(), "cache_batch_idx", {b});
+        P.a.cache_batch_idx = cache_batch_idx_.value().data_ptr<int32_t>();
+    }
+    if (paged) {
+        const Tensor &bt = block_table_.value();
+        TORCH_CHECK(bt.scalar_type() == at::kInt, "block_table must have dtype torch.int32");
+        expect_with(bt, "block_table", kc);
+        TORCH_CHECK(bt.dim() == 2 && bt.size(0) == b && bt.size(1) > 0, "block_table must have shape (batch_size, max_blocks)");
+        TORCH_CHECK(bt.size(1) <= 1 || bt.stride(-1) == 1, "block_table must have contiguous last dimension");
+        TORCH_CHECK(bt.size(1) * rows <= (1 << 30), "8-bit KV cache: too large");
+        P.a.block_table = bt.data_ptr<int32_t>();
+        P.a.block_table_batch_stride = stride_of(bt, 0);
+        P.a.page_block_size = (int)rows;
+        P.a.seqlen_k = (int)(bt.size(1) * rows);
+    } else {
+        TORCH_CHECK(cache_batch_idx_.has_value() || b <= pages, "batch size exceeds the cache's");
+        P.a.seqlen_k = (int)rows;
+    }
+    return b;
+}
+
+// New tokens (dense or ragged); the returned pair keeps copies alive until the launch.
+std::pair<Tensor, Tensor> set_kv8_new(vfa_kv8_params &P, const Tensor &k_, const Tensor &v_, const Tensor &kc, const OptTensor &cu_, int64_t max_seqlen) {
+    const int dt = dtype_code(k_);
+    TORCH_CHECK(v_.scalar_type() == k_.scalar_type(), "k and v must have the same dtype");
+    expect_with(k_, "k", kc);
+    expect_with(v_, "v", kc);
+    TORCH_CHECK(k_.dim() == (cu_.has_value() ? 3 : 4), cu_.has_value() ? "k and v must be (total, nheads_k, headdim) with cu_seqlens"
+                                                                       : "k and v must be (batch_size, seqlen, nheads_k, headdim), or ragged with cu_seqlens");
+    TORCH_CHECK(k_.sizes() == v_.sizes(), "k and v must have the same shape");
+    TORCH_CHECK(k_.size(-2) == P.a.h_k && k_.size(-1) == P.a.d, "k and v must have the heads and the head size of the cache, (", P.a.h_k, ", ", P.a.d, "), got ", k_.sizes());
+    Tensor k = aligned_rows(k_), v = aligned_rows(v_);
+    P.a.dtype = dt;
+    P.a.knew = k.data_ptr(); P.a.vnew = v.data_ptr();
+    P.a.knew_row_stride = stride_of(k, -3); P.a.knew_head_stride = stride_of(k, -2);
+    P.a.vnew_row_stride = stride_of(v, -3); P.a.vnew_head_stride = stride_of(v, -2);
+    if (cu_.has_value()) {
+        expect_int32(cu_.value(), "cu_seqlens", kc);
+        expect_shape(cu_.value(), "cu_seqlens", {(int64_t)P.a.b + 1});
+        TORCH_CHECK(max_seqlen >= 0 && max_seqlen <= (1 << 30), "max_seqlen out of range");
+        P.cu_seqlens_new = cu_.value().data_ptr<int32_t>();
+        P.a.seqlen_knew = (int)std::min<int64_t>(max_seqlen, k.size(0));
+    } else {
+        TORCH_CHECK(k.size(0) == P.a.b, "k and v must have the batch size ", P.a.b, ", got ", k.size(0));
+        TORCH_CHECK(k.size(1) <= (1 << 30), "too many new tokens");
+        P.a.knew_batch_stride = stride_of(k, 0); P.a.vnew_batch_stride = stride_of(v, 0);
+        P.a.seqlen_knew = (int)k.size(1);
+    }
+    return {k, v};
+}
+
+void kv8_quantize(const Tensor &k, const Tensor &v, const Tensor &kc, const Tensor &vc, const Tensor &ks, const Tensor &vs,
+                  const Tensor &seqlens, const OptTensor &cache_batch_idx, const OptTensor &block_table, const OptTensor &cu_seqlens,
+                  int64_t max_seqlen) {
+    vfa_kv8_params P{};
+    set_kv8_cache(P, kc, vc, ks, vs, -1, seqlens, cache_batch_idx, block_table);
+    at::hip::HIPGuardMasqueradingAsCUDA device_guard{(c10::DeviceIndex)kc.get_device()};
+    const auto keep = set_kv8_new(P, k, v, kc, cu_seqlens, max_seqlen);
+    if (keep.first.numel() == 0) return;
+    P.a.stream = current_stream();
+    run(vfa_kv8_quantize(&P));
+}
+
+std::vector<Tensor> kv8_dequantize(const Tensor &kc, const Tensor &vc, const Tensor &ks, const Tensor &vs, const Tensor &seqlens,
+                                   const OptTensor &cache_batch_idx, const OptTensor &block_table, const OptTensor &cu_seqlens,
+                                   int64_t rows, at::ScalarType dtype) {
+    vfa_kv8_params P{};
+    const int64_t b = set_kv8_cache(P, kc, vc, ks, vs, -1, seqlens, cache_batch_idx, block_table);
+    TORCH_CHECK(dtype == at::kHalf || dtype == at::kBFloat16, "FlashAttention only support fp16 and bf16 data type");
+    TORCH_CHECK(rows >= 0 && rows <= (1 << 30), "max_seqlen / total_seqlen out of range");
+    at::hip::HIPGuardMasqueradingAsCUDA device_guard{(c10::DeviceIndex)kc.get_device()};
+    const int64_t hk = P.a.h_k, d = P.a.d;
+    Tensor k, v;
+    if (cu_seqlens.has_value()) {
+        expect_int32(cu_seqlens.value(), "cu_seqlens", kc);
+        expect_shape(cu_seqlens.value(), "cu_seqlens", {b + 1});
+        P.cu_seqlens_out = cu_seqlens.value().data_ptr<int32_t>();
+        P.rows_out = rows;
+        k = torch::empty({rows, hk, d}, kc.options().dtype(dtype));
+    } else {
+        P.seqlen_out = (int)rows;
+        P.rows_out = b * rows;
+        k = torch::empty({b, rows, hk, d}, kc.options().dtype(dtype));
+    }
+    v = torch::empty_like(k);
+    if (k.numel() == 0) return {k, v};
+    P.a.dtype = dtype == at::kBFloat16 ? VFA_BF16 : VFA_FP16;
+    P.k_out = k.data_ptr(); P.v_out = v.data_ptr();
+    P.ko_batch_stride = P.vo_batch_stride = rows * hk * d;
+    P.ko_row_stride = P.vo_row_stride = hk * d;
+    P.ko_head_stride = P.vo_head_stride = d;
+    P.a.stream = current_stream();
+    run(vfa_kv8_dequantize(&P));
+    return {k, v};
+}
+
+std::vector<Tensor> fwd_kv8(const Tensor &q_, const Tensor &kc, const Tensor &vc, const Tensor &ks, const Tensor &vs, OptTensor &k_,
+                            OptTensor &v_, OptTensor &seqlens, OptTensor &cache_batch_idx, OptTensor &block_table, OptTensor &alibi_slopes,
+                            OptTensor &out_, OptTensor &cu_seqlens_q, int64_t max_seqlen_q, const double softmax_scale, bool is_causal,
+                            int64_t window_size_left, int64_t window_size_right, int64_t num_splits) {
+    const int dt = dtype_code(q_);
+    const bool ragged = cu_seqlens_q.has_value();
+    TORCH_CHECK(q_.dim() == (ragged ? 3 : 4), ragged ? "q must be (total_q, nheads, headdim) with cu_seqlens_q"
+                                                     : "q must be (batch_size, seqlen_q, nheads, headdim), or ragged with cu_seqlens_q");
+    if (ragged) TORCH_CHECK(cu_seqlens_q.value().dim() == 1 && cu_seqlens_q.value().numel() > 1, "cu_seqlens_q must have shape (batch_size + 1)");
+    const int64_t b = ragged ? cu_seqlens_q.value().numel() - 1 : q_.size(0);
+    vfa_kv8_params P{};
+    TORCH_CHECK(b > 0, "batch size must be postive");
+    set_kv8_cache(P, kc, vc, ks, vs, b, seqlens, cache_batch_idx, block_table);
+    expect_with(q_, "q", kc);
+    at::hip::HIPGuardMasqueradingAsCUDA device_guard{(c10::DeviceIndex)kc.get_device()};
+    const int64_t h = q_.size(-2), d = P.a.d, hk = P.a.h_k, sq = ragged ? max_seqlen_q : q_.size(1);
+    TORCH_CHECK(q_.size(-1) == d, "q must have the head size of the cache, ", d, ", got ", q_.size(-1));
+    TORCH_CHECK(h > 0 && h % hk == 0, "Number of heads in key/value must divide number of heads in query");
+    TORCH_CHECK(sq >= 0 && sq * h <= (1 << 30), "max_seqlen_q out of range");
+    std::pair<Tensor, Tensor> keep;
+    if (k_.has_value() || v_.has_value()) {
+        TORCH_CHECK(k_.has_value() && v_.has_value(), "If key is supplied, value must also be passed in");
+        TORCH_CHECK(seqlens.has_value(), "If key is supplied, seqlens_k must also be passed in");
+        TORCH_CHECK(!ragged, "new keys and values go with a dense query batch: write them with quantize_kvcache first");
+        TORCH_CHECK(k_.value().scalar_type() == q_.scalar_type(), "Key must have the same dtype as query");
+        keep = set_kv8_new(P, k_.value(), v_.value(), kc, std::nullopt, 0);
+    }
+    const Tensor q = aligned_rows(q_);
+    Tensor out;
+    if (out_.has_value()) {
+        const Tensor &o = out_.value();
+        TORCH_CHECK(o.scalar_type() == q.scalar_type(), "Output must have the same dtype as inputs");
+        expect_with(o, "out", kc);
+        TORCH_CHECK(o.sizes() == q.sizes(), "out must have the shape of q, ", q.sizes(), ", got ", o.sizes());
+        TORCH_CHECK(o.size(-1) <= 1 || o.stride(-1) == 1, "Output tensor must have contiguous last dimension");
+        bool fits = ((uintptr_t)o.data_ptr() & 15) == 0;
+        for (int64_t i = 0; i + 1 < o.dim(); i++) fits = fits && stride_of(o, i) % 8 == 0;
+        out = fits ? o : torch::empty(q.sizes(), q.options());
+    } else {
+        out = torch::empty(q.sizes(), q.options());
+    }
+    auto opts = q.options();
+    Tensor lse = torch::empty({b, h, sq}, opts.dtype(at::kFloat));
+    if (q.numel() == 0 || sq == 0) {
+        // no query: the new tokens still enter the cache
+        if (k_.has_value() && keep.first.numel() > 0) { P.a.stream = current_stream(); run(vfa_kv8_quantize(&P)); }
+        return {out, lse};
+    }
+    P.a.dtype = dt;
+    P.a.q = q.data_ptr(); P.a.out = out.data_ptr(); P.a.softmax_lse = lse.data_ptr<float>();
+    P.a.q_row_stride = stride_of(q, -3); P.a.q_head_stride = stride_of(q, -2);
+    P.a.o_row_stride = stride_of(out, -3); P.a.o_head_stride = stride_of(out, -2);
+    P.a.h = (int)h; P.a.seqlen_q = (int)sq;
+    if (ragged) {
+        expect_int32(cu_seqlens_q.value(), "cu_seqlens_q", kc);
+        P.a.cu_seqlens_q = cu_seqlens_q.value().data_ptr<int32_t>();
+        P.a.total_q = (int)q.size(0);
+    } else {
+        P.a.q_batch_stride = stride_of(q, 0); P.a.o_batch_stride = stride_of(out, 0);
+    }
+    if (keep.first.defined() && keep.first.numel() == 0) P.a.knew = P.a.vnew = nullptr;
+    P.a.softmax_scale = (float)softmax_scale;
+    P.a.is_causal = is_causal;
+    P.a.window_size_left = (int)std::clamp<int64_t>(window_size_left, -1, 1 << 30);
+    P.a.window_size_right = (int)std::clamp<int64_t>(window_size_right, -1, 1 << 30);
+    if (alibi_slopes.has_value()) expect_with(alibi_slopes.value(), "alibi_slopes", kc);
+    set_alibi(P.a, alibi_slopes, b, h);
+    SplitScratch scratch;
+    if (num_splits < 1) num_splits = vfa_kv8_num_splits((int)b, (int)h, (int)hk, (int)d, P.a.seqlen_k, (int)sq, cu_count());
+    plan_splits(P.a, scratch, (int)std::min<int64_t>(num_splits, 1 << 20), b, h, d, P.a.seqlen_k, sq, opts);
+    P.a.stream = current_stream();
+    run(vfa_kv8_mha_fwd(&P));
+    if (out_.has_value() && out.data_ptr() != out_.value().data_ptr()) {
+        out_.value().copy_(out);
+        out = out_.value();
+    }
+    return {out, lse};
+}
+
+struct QKNormHeld { std::vector<Tensor> t; };
+
+void set_qk_norm(vfa_qk_norm_rotary_params &P, QKNormHeld &held, const Tensor &q_, const Tensor &k_, const Tensor &wq, const Tensor &wk,
+                 const Tensor &cos, const Tensor &sin, const OptTensor &positions, double eps, bool interleaved) {
+    P.dtype = dtype_code(q_);
+    TORCH_CHECK(k_.scalar_type() == q_.scalar_type(), "q and k must have the same dtype");
+    expect_gpu(q_, "q");
+    expect_with(k_, "k", q_);
+    TORCH_CHECK(q_.dim() == 4 && k_.dim() == 4 && q_.size(0) == k_.size(0) && q_.size(1) == k_.size(1) && q_.size(3) == k_.size(3),
+                "q and k must have the same tokens and head size, got ", q_.sizes(), " and ", k_.sizes());
+    const int64_t b = q_.size(0), s = q_.size(1), h = q_.size(2), hk = k_.size(2), d = q_.size(3);
+    TORCH_CHECK(h > 0 && hk > 0, "q and k must have heads");
+    TORCH_CHECK(d > 0 && d <= 256 && d % 8 == 0, "qk_norm_rotary: head dimension must be a multiple of 8, at most 256");
+    TORCH_CHECK(b <= (1 << 30) && s <= (1 << 30) && h <= (1 << 20) && hk <= (1 << 20), "qk_norm_rotary: too large");
+    for (const Tensor *w : {&wq, &wk}) {
+        expect_with(*w, "weight", q_);
+        TORCH_CHECK(w->scalar_type() == q_.scalar_type() || w->scalar_type() == at::kFloat, "q_weight and k_weight must have the dtype of q or fp32");
+        TORCH_CHECK(w->scalar_type() == wq.scalar_type(), "q_weight and k_weight must have the same dtype");
+        expect_shape(*w, "q_weight / k_weight", {d});
+        expect_contig(*w, "q_weight / k_weight");
+    }
+    TORCH_CHECK(cos.dim() == 2, "rotary_cos must be 2-dimensional");
+    for (const Tensor *c : {&cos, &sin}) {
+        expect_with(*c, "rotary_cos / rotary_sin", q_);
+        TORCH_CHECK(c->scalar_type() == q_.scalar_type() || c->scalar_type() == at::kFloat, "rotary_cos and rotary_sin must have the dtype of q or fp32");
+        TORCH_CHECK(c->scalar_type() == cos.scalar_type(), "rotary_cos and rotary_sin must have the same dtype");
+        expect_shape(*c, "rotary_cos / rotary_sin", {cos.size(0), cos.size(1)});
+        expect_contig(*c, "rotary_cos / rotary_sin");
+    }
+    const int64_t rd = 2 * cos.size(1);
+    TORCH_CHECK(cos.size(0) > 0 && cos.size(0) <= (1 << 30), "rotary_cos must have rows");
+    TORCH_CHECK(rd > 0 && rd % 16 == 0, "Only rotary dimensions divisible by 16 are currently supported");
+    TORCH_CHECK(rd <= d, "rotary_dim must be <= headdim");
+    if (positions.has_value()) {
+        const Tensor &p = positions.value();
+        TORCH_CHECK(p.scalar_type() == at::kInt, "positions must have dtype int32");
+        expect_with(p, "positions", q_);
+        expect_shape(p, "positions", {b, s});
+        TORCH_CHECK(s <= 1 || p.stride(1) == 1, "positions must have contiguous last dimension");
+        P.positions = p.data_ptr<int32_t>();
+        P.positions_batch_stride = stride_of(p, 0);
+    } else {
+        TORCH_CHECK(s <= cos.size(0), "cos/sin seqlen must be at least the seqlen of q");
+    }
+    P.weight_fp32 = wq.scalar_type() == at::kFloat;
+    P.table_fp32 = cos.scalar_type() == at::kFloat;
+    P.b = (int)b; P.s = (int)s; P.h = (int)h; P.h_k = (int)hk; P.d = (int)d;
+    const Tensor q = aligned_rows(q_), k = aligned_rows(k_);
+    held.t.push_back(q); held.t.push_back(k);
+    P.q = q.data_ptr(); P.k = k.data_ptr();
+    P.q_batch_stride = stride_of(q, 0); P.q_row_stride = stride_of(q, 1); P.q_head_stride = stride_of(q, 2);
+    P.k_batch_stride = stride_of(k, 0); P.k_row_stride = stride_of(k, 1); P.k_head_stride = stride_of(k, 2);
+    P.q_weight = wq.data_ptr(); P.k_weight = wk.data_ptr();
+    P.rotary_cos = cos.data_ptr(); P.rotary_sin = sin.data_ptr();
+    P.table_rows = (int)cos.size(0); P.rotary_dim = (int)rd; P.is_rotary_interleaved = interleaved;
+    P.eps = (float)eps;
+}
+
+void set_qk_out(vfa_qk_norm_rotary_params &P, const Tensor &q, const Tensor &k) {   // contiguous (b, s, heads, d)
+    P.q_out = q.defined() ? q.data_ptr() : nullptr;
+    P.k_out = k.defined() ? k.data_ptr() : nullptr;
+    const int64_t s = P.s, d = P.d;
+    P.qo_batch_stride = s * P.h * d; P.qo_row_stride = P.h * d; P.qo_head_stride = d;
+    P.ko_batch_stride = s * P.h_k * d; P.ko_row_stride = P.h_k * d; P.ko_head_stride = d;
+}
+
+std::vector<Tensor> qk_norm_rotary_fwd(const Tensor &q, const Tensor &k, const Tensor &wq, const Tensor &wk, const Tensor &cos,
+                                       const Tensor &sin, const OptTensor &positions, double eps, bool interleaved) {
+    vfa_qk_norm_rotary_params P{};
+    QKNormHeld held;
+    expect_gpu(q, "q");
+    at::hip::HIPGuardMasqueradingAsCUDA device_guard{(c10::DeviceIndex)q.get_device()};
+    set_qk_norm(P, held, q, k, wq, wk, cos, sin, positions, eps, interleaved);
+    Tensor qo = torch::empty(q.sizes(), q.options()), ko = torch::empty(k.sizes(), k.options());
+    if (q.size(0) * q.size(1) == 0) return {qo, ko};
+    set_qk_out(P, qo, ko);
+    P.stream = current_stream();
+    run(vfa_qk_norm_rotary_fwd(&P));
+    return {qo, ko};
+}
+
+std::vector<Tensor> qk_norm_rotary_bwd(const Tensor &dqo_, const Tensor &dko_, const Tensor &q, const Tensor &k, const Tensor &wq,
+                                       const Tensor &wk, const Tensor &cos, const Tensor &sin, const OptTensor &positions, double eps,
+                                       bool interleaved, bool need_q, bool need_k, bool need_wq, bool need_wk) {
+    vfa_qk_norm_rotary_params P{};
+    QKNormHeld held;
+    expect_gpu(q, "q");
+    at::hip::HIPGuardMasqueradingAsCUDA device_guard{(c10::DeviceIndex)q.get_device()};
+    set_qk_norm(P, held, q, k, wq, wk, cos, sin, positions, eps, interleaved);
+    expect_with(dqo_, "dq_out", q);
+    expect_with(dko_, "dk_out", q);
+    TORCH_CHECK(dqo_.sizes() == q.sizes() && dko_.sizes() == k.sizes(), "gradients must have the shapes of the outputs");
+    TORCH_CHECK(dqo_.scalar_type() == q.scalar_type() && dko_.scalar_type() == q.scalar_type(), "gradients must have the dtype of the outputs");
+    const Tensor dqo = aligned_rows(dqo_), dko = aligned_rows(dko_);
+    P.dq_out = dqo.data_ptr(); P.dk_out = dko.data_ptr();
+    P.dqo_batch_stride = stride_of(dqo, 0); P.dqo_row_stride = stride_of(dqo, 1); P.dqo_head_stride = stride_of(dqo, 2);
+    P.dko_batch_stride = stride_of(dko, 0); P.dko_row_stride = stride_of(dko, 1); P.dko_head_stride = stride_of(dko, 2);
+    Tensor dq, dk, dwq, dwk, work;
+    if (need_q) dq = torch::empty(q.sizes(), q.options());
+    if (need_k) dk = torch::empty(k.sizes(), k.options());
+    if (need_wq) dwq = torch::empty_like(wq);
+    if (need_wk) dwk = torch::empty_like(wk);
+    set_qk_out(P, dq, dk);
+    if (need_wq) P.dq_weight = dwq.data_ptr();
+    if (need_wk) P.dk_weight = dwk.data_ptr();
+    if (need_wq || need_wk) {
+        work = torch::empty({(int64_t)vfa_qk_norm_rotary_bwd_workspace(&P)}, q.options().dtype(at::kFloat));
+        P.workspace = work.data_ptr<float>();
+    }
+    P.stream = current_stream();
+    run(vfa_qk_norm_rotary_bwd(&P));
+    return {dq, dk, dwq, dwk};
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -856,4 +1217,15 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("bwd", &bwd, "Backward pass");
     m.def("varlen_bwd", &varlen_bwd, "Backward pass (variable length)");
     m.def("fwd_kvcache", &fwd_kvcache, "Forward pass, with KV-cache");
+    // No counterpart in the reference: a KV cache in 8 bits, and the norm and rotation of q and k heads.
+    m.def("kv8_quantize", &kv8_quantize, "Write tokens to an 8-bit KV cache");
+    m.def("kv8_dequantize", [](const Tensor &kc, const Tensor &vc, const Tensor &ks, const Tensor &vs, const Tensor &seqlens,
+                               const OptTensor &cache_batch_idx, const OptTensor &block_table, const OptTensor &cu_seqlens, int64_t rows,
+                               const py::object &dtype) {
+        return kv8_dequantize(kc, vc, ks, vs, seqlens, cache_batch_idx, block_table, cu_seqlens, rows,
+                              torch::python::detail::py_object_to_dtype(dtype));
+    }, "Read an 8-bit KV cache in 16 bits");
+    m.def("fwd_kv8", &fwd_kv8, "Forward pass, with an 8-bit KV cache");
+    m.def("qk_norm_rotary_fwd", &qk_norm_rotary_fwd, "RMS norm and rotation of query and key heads");
+    m.def("qk_norm_rotary_bwd", &qk_norm_rotary_bwd, "Backward of qk_norm_rotary_fwd");
 }

@@ -1,0 +1,91 @@
+// A KV cache held in 8 bits: e4m3 codes with one power-of-two scale per (block of tokens, KV head), in
+// E8M0 bytes (value 2^(byte - 127), 255 = NaN).  Parameter block and device helpers shared by the kernels
+// that write such a cache, read it back and attend over it.
+//
+// Why a power of two.  e4m3 is a floating format: a block's scale only has to bring the block's largest
+// magnitude under 448; within the format's normal range a value keeps its 3 mantissa bits whatever the
+// scale.  With 2^e every product with the scale is exact, so the value a code stands for is exact in
+// bf16 / fp16, the conversion instructions apply it (v_cvt_scalef32_pk_{bf16,f16}_fp8 take the exponent of
+// a float), and re-encoding a block whose scale has grown rounds only what falls among the subnormals.
+#pragma once
+#include "vfa_kernel_params.h"
+
+namespace vfa {
+
+constexpr int KV8_EMIN = -126;   // smallest exponent of a scale (2^126 is still a normal float)
+
+struct KV8Params {
+    KParams p;                   // k / v: the codes (strides in bytes); lengths, pages, masks, q, out as elsewhere
+    unsigned char *ks, *vs;      // scales
+    int64_t ks_bs, ks_rs, ks_hs; // page (batch row), block of tokens, head
+    int64_t vs_bs, vs_rs, vs_hs;
+    int blk;                     // tokens per scale: a multiple of 16 that divides page_rows
+    int page_rows;               // rows of a page; of a contiguous cache: its capacity
+    int num_pages;               // pages; batch rows of a contiguous cache
+    int cap;                     // most tokens a sequence can have
+    int heads_per_wg;            // attention: adjacent KV heads per workgroup (1, 2, 4, 8)
+    unsigned page_mul, blk_mul;  // n / (page_rows / 16) = n * page_mul >> page_sh for n < 2^27 (and so for blk)
+    int page_sh, blk_sh;
+    // writing: new tokens are p.knew / p.vnew, dense (b, seqlen_knew) or ragged
+    const int *cu_new;
+    // reading back
+    void *k_out, *v_out;
+    int64_t ko_bs, ko_rs, ko_hs, vo_bs, vo_rs, vo_hs;
+    const int *cu_out;           // ragged: (b + 1); else (b, seqlen_out)
+    int64_t rows_out;            // output rows in all
+    int seqlen_out;
+};
+
+// multiplier and shift of the exact division of n < 2^27 by d: M = floor(2^k / d) + 1 with k = 27 + ceil(log2 d)
+// has an error under 2^-27 relative, less than a unit of the quotient's fraction
+inline void kv8_div_magic(int d, unsigned &mul, int &shift) {
+    int l = 0;
+    while ((1 << l) < d) l++;
+    shift = 27 + l;
+    mul = (unsigned)((1ull << shift) / (unsigned)d + 1);
+}
+__device__ __forceinline__ int kv8_div(int n, unsigned mul, int shift) {
+    return (int)(((unsigned long long)(unsigned)n * mul) >> shift);
+}
+
+// tokens in the cache of sequence bidb before the call
+__device__ __forceinline__ int kv8_cached(const KV8Params &a, int bidb) {
+    const int n = a.p.cu_seqlens_k ? a.p.cu_seqlens_k[bidb] : a.p.seqlen_k;
+    return min(max(n, 0), a.cap);
+}
+
+// Page that holds token `tok` of sequence bidb (a contiguous cache: its batch row); -1 if the table names
+// none of the pool.  tok < cap.
+__device__ __forceinline__ int kv8_page(const KV8Params &a, int bidb, int tok) {
+    int page;
+    if (a.p.block_table) page = a.p.block_table[(int64_t)bidb * a.p.bt_bs + kv8_div(tok >> 4, a.page_mul, a.page_sh)];
+    else page = a.p.cache_batch_idx ? a.p.cache_batch_idx[bidb] : bidb;
+    return (unsigned)page < (unsigned)a.num_pages ? page : -1;
+}
+__device__ __forceinline__ int kv8_row_in_page(const KV8Params &a, int tok) {
+    return a.p.block_table ? tok - kv8_div(tok >> 4, a.page_mul, a.page_sh) * a.page_rows : tok;
+}
+
+__device__ __forceinline__ float e8m0_to_f32(unsigned byte) {
+    return __uint_as_float(byte == 255u ? 0x7fc00000u : byte << 23);
+}
+
+// 8 codes -> 8 values of 16 bits, times 2^e
+template <bool BF16>
+__device__ __forceinline__ i32x4 kv8_to16(i32x2 c, float scale) {
+    i32x4 w;
+    if constexpr (BF16) {
+        w[0] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c[0], scale, false));
+        w[1] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c[0], scale, true));
+        w[2] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c[1], scale, false));
+        w[3] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c[1], scale, true));
+    } else {
+        w[0] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(c[0], scale, false));
+        w[1] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(c[0], scale, true));
+        w[2] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(c[1], scale, false));
+        w[3] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(c[1], scale, true));
+    }
+    return w;
+}
+
+}  // namespace vfa
