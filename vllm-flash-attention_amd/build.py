@@ -27,7 +27,7 @@ LIB = os.path.join(HERE, "libvfa_hip.so")
 HIP_SOURCES = ["api.hip", "fwd_prefill.hip", "fwd_splitkv.hip", "bwd.hip", "fwd_prefill_drop.hip",
                "bwd_drop.hip", "fwd_prefill_split.hip", "bwd_dkdv_w64.hip", "fwd_prefill_persist.hip", "bwd_dq_persist.hip",
                "bwd_dkdv_wide.hip", "fwd_prefill_wide.hip", "bwd_dq_ilp.hip", "fwd_prefill_d64.hip", "fwd_prefill_pack.hip", "fwd_prefill_d96.hip", "bwd_d96.hip", "fwd_prefill_wide_paged.hip",
-               "fwd_kv8.hip", "kv8_cache.hip", "qk_norm_rotary.hip"]
+               "fwd_kv8.hip", "fwd_prefill_kv8.hip", "kv8_cache.hip", "qk_norm_rotary.hip"]
 # The development library (libvfa_hip_dev.so, -DVFA_DEV) adds the kernels no shipped dispatch takes
 # and the kernel-variant switches (vfa_debug_set_tuning) that select them; the A/B tools and the
 # tests that check a shipped kernel against its alternative load it.  The product never does.
@@ -41,7 +41,7 @@ DEV_LIB = os.path.join(HERE, "libvfa_hip_dev.so")
 NO_PACKED_FP32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 # Kernels built for one wave per SIMD (up to 512 registers): MFMA results that vector instructions
 # consume must be allocated in the arch VGPRs, not forced into the accumulator half of the file.
-EXTRA_FLAGS = {"fwd_kv8.hip": NO_PACKED_FP32, "kv8_cache.hip": NO_PACKED_FP32, "qk_norm_rotary.hip": NO_PACKED_FP32,
+EXTRA_FLAGS = {"fwd_kv8.hip": NO_PACKED_FP32, "fwd_prefill_kv8.hip": NO_PACKED_FP32, "kv8_cache.hip": NO_PACKED_FP32, "qk_norm_rotary.hip": NO_PACKED_FP32,
                "bwd_dkdv_w64.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
                "bwd_dkdv_wide.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
                "fwd_prefill_wide.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
@@ -61,7 +61,7 @@ EXTRA_FLAGS = {"fwd_kv8.hip": NO_PACKED_FP32, "kv8_cache.hip": NO_PACKED_FP32, "
                "fwd_prefill_d64.hip": ["-fno-slp-vectorize"]}
 # the dropout translation units are one-line includes of the kernel sources
 EXTRA_DEPS = {"fwd_prefill_drop.hip": ["fwd_prefill.hip"], "bwd_drop.hip": ["bwd.hip"], "bwd_d96.hip": ["bwd.hip"], "fwd_prefill_wide_paged.hip": ["fwd_prefill_wide.hip"], "bwd_dq_ilp.hip": ["bwd.hip"], "fwd_prefill_d64.hip": ["fwd_prefill.hip"], "fwd_prefill_d96.hip": ["fwd_prefill.hip"], "fwd_prefill_pack.hip": ["fwd_prefill.hip"],
-              "fwd_prefill_split.hip": ["fwd_prefill.hip"]}
+              "fwd_prefill_split.hip": ["fwd_prefill.hip"], "fwd_prefill_kv8.hip": ["fwd_prefill.hip"]}
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 HIP_FLAGS = ["--offload-arch=gfx950", "-O3", "-fPIC", "-fvisibility=hidden", "-std=c++17", "-I", INCLUDE, "-I", CSRC]
 

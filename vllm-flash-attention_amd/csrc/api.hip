@@ -32,6 +32,7 @@ hipError_t run_kv8_quantize(const KV8Params &a, hipStream_t stream);            
 hipError_t run_kv8_dequantize(const KV8Params &a, hipStream_t stream);
 hipError_t run_fwd_kv8(const KV8Params &a, hipStream_t stream);                  // fwd_kv8.hip
 int kv8_heads_per_wg(int d, int h_k);
+bool kv8_takes_prefill(int d, int h_ratio, int seqlen_q);
 hipError_t run_qk_norm_rotary(const QKNormParams &p, bool bwd, hipStream_t stream);   // qk_norm_rotary.hip
 void qk_norm_bwd_blocks(QKNormParams &p, int cus);
 }  // namespace vfa
@@ -620,8 +621,17 @@ extern "C" int vfa_kv8_dequantize(const vfa_kv8_params *p) {
 extern "C" int vfa_kv8_num_splits(int batch, int num_heads, int num_heads_k, int head_size, int max_seqlen_k, int max_seqlen_q,
                                   int num_cus_) {
     if (num_heads_k <= 0 || num_heads % num_heads_k != 0 || head_size <= 0 || batch <= 0) return 1;
+    const int ratio = num_heads / num_heads_k;
+    if (vfa::kv8_takes_prefill(head_size, ratio, max_seqlen_q)) {
+        // 128-row blocks, two workgroups per CU; split only what would fill less than a quarter of them (the
+        // rule of the 16-bit path's packed rows), at least four 64-key tiles each
+        const long long blocks = (long long)batch * num_heads_k * (((long long)max_seqlen_q * ratio + 127) / 128);
+        const long long chunks = ((long long)max_seqlen_k + 255) / 256;
+        if (blocks * 4 > 2LL * num_cus_ || chunks < 2) return 1;
+        return (int)std::min({chunks, 2LL * num_cus_ / blocks, 128LL});
+    }
     const int hpw = vfa::kv8_heads_per_wg(head_size, num_heads_k), parts = 8 / hpw;
-    const long long items = (long long)batch * (num_heads_k / hpw) * (((long long)max_seqlen_q * (num_heads / num_heads_k) + 31) / 32);
+    const long long items = (long long)batch * (num_heads_k / hpw) * (((long long)max_seqlen_q * ratio + 31) / 32);
     // two workgroups per CU; a wave keeps at least 4 of its steps of 32 keys
     const long long most = std::max(1LL, (long long)max_seqlen_k / (32LL * 4 * parts));
     const long long want = (2LL * num_cus_ + items - 1) / std::max(1LL, items);

@@ -381,7 +381,13 @@ int kv8_heads_per_wg(int d, int h_k) {
     return n;
 }
 
+hipError_t run_fwd_kv8_prefill(const KV8Params &a, hipStream_t stream);   // fwd_prefill_kv8.hip
+
+// Whether a call's rows take the prefill kernel's 128-row blocks: from there on the products bound it.
+bool kv8_takes_prefill(int d, int h_ratio, int seqlen_q) { return (long long)seqlen_q * h_ratio > 32; }
+
 hipError_t run_fwd_kv8(const KV8Params &a, hipStream_t stream) {
+    if (kv8_takes_prefill(a.p.d, a.p.h_ratio, a.p.seqlen_q)) return run_fwd_kv8_prefill(a, stream);
     const bool bf = a.p.is_bf16;
     if (a.p.d <= 64) return bf ? launch_kv8_rows<64, true>(a, stream) : launch_kv8_rows<64, false>(a, stream);
     if (a.p.d <= 128) return bf ? launch_kv8_rows<128, true>(a, stream) : launch_kv8_rows<128, false>(a, stream);

@@ -16,6 +16,7 @@
 //     tiles that need them (wave-uniform test).
 #include "vfa_kernel_params.h"
 #include "vfa_dispatch.h"
+#include "vfa_kv8.h"
 #include <type_traits>
 
 namespace vfa {
@@ -122,6 +123,10 @@ struct PrefillCfg {
 // XOR swizzle places at its slot.  No staging registers, no ds_write, and the wave does not wait
 // for its own loads before the tile's last barrier.  (Out-of-range lanes write zeros.)
 // LD = 0: generic per-row addressing (any strides, any page size).
+// LD = 5: an 8-bit cache (vfa_kv8.h; the kernel's argument is then a KV8Params), contiguous or paged.
+// The codes go through staging registers, 16 of a row per load, and are converted once per workgroup
+// on their way to the 16-bit tile in LDS; from there on the kernel is the same.  The rows of a wave's load
+// lie in one group of 16, so in one page and one block of the scales.
 //
 // DROP: dropout on P (flash_fwd_kernel.h:324-337, dropout.h) with the reference's Philox pattern,
 // and the optional Return_softmax output.  The reference point of the exponentials then follows
@@ -138,9 +143,14 @@ struct PrefillCfg {
 // heads).  For a few query tokens per sequence against a long cache (chunked prefill, draft-token
 // verification): 16 tokens of 4 grouped heads fill half a 128-row block and sweep the keys once,
 // where one block per query head sweeps them four times at an eighth of the rows each.
+__device__ __forceinline__ const KParams &base_params(const KParams &p) { return p; }
+__device__ __forceinline__ const KParams &base_params(const KV8Params &a) { return a.p; }
+
 template <int DP, bool BF16, int NW, int LD, bool DROP, bool SPLIT = false, bool PACK = false, int DV = DP>
 __global__ void __launch_bounds__(NW * 64, (NW == 8 || DP == 256) ? 1 : 2)
-fwd_prefill_kernel(const KParams p, const int n_mblocks) {
+fwd_prefill_kernel(const std::conditional_t<LD == 5, KV8Params, KParams> args, const int n_mblocks) {
+    constexpr bool KV8 = LD == 5;                    // 8-bit codes, converted on their way into LDS
+    const KParams &p = base_params(args);
     static_assert(!PACK || (NW == 4 && !DROP), "packed grouped heads: 4-wave geometry, no dropout");
     constexpr bool DIRECT = LD == 3;                 // contiguous K/V, loaded straight into LDS
     constexpr bool PDIRECT = LD == 4;                // paged K/V (per-page descriptors), loaded straight into LDS
@@ -167,7 +177,9 @@ fwd_prefill_kernel(const KParams p, const int n_mblocks) {
     const int ratio = PACK ? p.pack_gqa : 1;
 
     const BlockInfo bi(p, bidb);
-    const int sq = bi.sq, sk = bi.sk;
+    int sk_ = bi.sk;
+    if constexpr (KV8) sk_ = min(kv8_cached(args, bidb) + (p.knew ? p.seqlen_knew : 0), args.cap);
+    const int sq = bi.sq, sk = sk_;
     const int sq_rows = sq * ratio;    // rows of this (batch, head): query positions (x grouped heads)
     // Philox state: the caller's values, or (under graph capture) read on the device at replay
     // time from the generator's captured state (at::cuda::philox::unpack, flash_fwd_kernel.h:45)
@@ -206,9 +218,15 @@ fwd_prefill_kernel(const KParams p, const int n_mblocks) {
     float *oacc_g = nullptr;
     if constexpr (SPLIT) {
         const int split = blockIdx.y;
-        const int per = (((p.seqlen_k + BN - 1) / BN) + p.num_splits - 1) / p.num_splits;  // from the capacity
-        n_min = max(n_min, split * per);
-        n_max = min(n_max, (split + 1) * per);
+        if constexpr (KV8) {   // the keys this block sees, in equal parts
+            const int per = (max(n_max - n_min, 0) + p.num_splits - 1) / p.num_splits;
+            n_min += split * per;
+            n_max = min(n_max, n_min + per);
+        } else {
+            const int per = (((p.seqlen_k + BN - 1) / BN) + p.num_splits - 1) / p.num_splits;  // from the capacity
+            n_min = max(n_min, split * per);
+            n_max = min(n_max, (split + 1) * per);
+        }
         const int64_t acc_row0 = (((int64_t)split * p.b + bidb) * h_all + head0) * p.seqlen_q;
         lse_g = p.lseaccum + acc_row0;
         oacc_g = p.oaccum + acc_row0 * p.d;
@@ -261,6 +279,61 @@ fwd_prefill_kernel(const KParams p, const int n_mblocks) {
         kg += bi.k_off(p.k_bs, p.k_rs, bidb_cache);
         vg += bi.k_off(p.v_bs, p.v_rs, bidb_cache);
     }
+
+    // KV8: 16-byte pieces of the tile's codes per thread, and the scales of the wave's rows
+    constexpr int NP = KV8 ? CH / 2 : 1, PPR = DP / 16;
+    static_assert(!KV8 || (CH % 2 == 0 && 64 / PPR <= 16), "pieces of a wave lie in one group of 16 rows");
+    i32x4 kc8[NP], vc8[NP];
+    unsigned ks8[NP], vs8[NP];
+    int pg8[NP];
+    // keys that some row of the block sees: V of the others must not count, whatever stands there
+    const int vis_lo = p.is_local ? max(0, pos_lo_b + sk - sq - p.wl) : 0;
+    const int vis_hi = (p.is_causal || p.is_local) ? min(sk, pos_hi_b + sk - sq + p.wr) : sk;
+    auto load_pages8 = [&](int n) __attribute__((always_inline)) {
+        if constexpr (KV8) {
+#pragma unroll
+            for (int i = 0; i < NP; i++) {
+                const int g16 = n * BN + (((wave * 64 + i * NT) / PPR) & ~15);   // the wave's group of rows
+                pg8[i] = kv8_page(args, bidb, min(g16, (sk - 1) & ~15));
+            }
+        }
+    };
+    auto load_tile8 = [&](int n) __attribute__((always_inline)) {
+        if constexpr (KV8) {
+#pragma unroll
+            for (int i = 0; i < NP; i++) {
+                const int tr = (tid + i * NT) / PPR, col = (tid + i * NT) % PPR * 16;
+                const int g16 = min(n * BN + (((wave * 64 + i * NT) / PPR) & ~15), (sk - 1) & ~15);
+                const int page = __builtin_amdgcn_readfirstlane(pg8[i]);
+                const int row = kv8_row_in_page(args, g16), blk = kv8_div(row >> 4, args.blk_mul, args.blk_sh);
+                const int64_t pg = max(page, 0);
+                ks8[i] = page < 0 ? 255u : args.ks[pg * args.ks_bs + blk * args.ks_rs + hk * args.ks_hs];
+                vs8[i] = page < 0 ? 255u : args.vs[pg * args.vs_bs + blk * args.vs_rs + hk * args.vs_hs];
+                const unsigned char *kp = (const unsigned char *)p.k + hk * p.k_hs + pg * p.k_bs + (int64_t)(row + (tr & 15)) * p.k_rs + col;
+                const unsigned char *vp = (const unsigned char *)p.v + hk * p.v_hs + pg * p.v_bs + (int64_t)(row + (tr & 15)) * p.v_rs + col;
+                const bool ok = col < p.d, seen = n * BN + tr >= vis_lo && n * BN + tr < vis_hi;
+                kc8[i] = ok ? *(const i32x4 *)kp : i32x4{0, 0, 0, 0};
+                vc8[i] = ok && seen ? *(const i32x4 *)vp : i32x4{0, 0, 0, 0};
+            }
+        }
+    };
+    auto store_tile8 = [&](auto BUFC) __attribute__((always_inline)) {
+        constexpr int BUF = decltype(BUFC)::value;
+        if constexpr (KV8) {
+#pragma unroll
+            for (int i = 0; i < NP; i++) {
+                const int tr = (tid + i * NT) / PPR, ch = (tid + i * NT) % PPR * 2;
+                const float ks = e8m0_to_f32(ks8[i]), vs = e8m0_to_f32(vs8[i]);
+                char *kd = smem + BUF * Cfg::TILE_BYTES, *vd = smem + (2 + BUF) * Cfg::TILE_BYTES;
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    const int off = lds_off<DP>(tr, ch + e);
+                    *(i32x4 *)(kd + off) = kv8_to16<BF16>(i32x2{kc8[i][2 * e], kc8[i][2 * e + 1]}, ks);
+                    *(i32x4 *)(vd + off) = kv8_to16<BF16>(i32x2{vc8[i][2 * e], vc8[i][2 * e + 1]}, vs);
+                }
+            }
+        }
+    };
 
     i32x4 kreg[CH], vreg[CH];
     // FAST path state: descriptors and the per-lane byte offset of chunk 0 (out of range for the
@@ -554,6 +627,11 @@ fwd_prefill_kernel(const KParams p, const int n_mblocks) {
         FWD_BLK_STAMP(5);
         __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): this wave's part of the first tile is in LDS
         FWD_BLK_STAMP(6);
+    } else if constexpr (KV8) {
+        load_pages8(n_max - 1);
+        load_tile8(n_max - 1);
+        if (n_max - 2 >= n_min) load_pages8(n_max - 2);
+        store_tile8(std::integral_constant<int, 0>{});
     } else {
         load_pages(n_max - 1);
         load_tile(n_max - 1);
@@ -579,6 +657,9 @@ fwd_prefill_kernel(const KParams p, const int n_mblocks) {
             } else if constexpr (PDIRECT) {
                 load_tile_pdirect(n - 1, std::integral_constant<int, BUF ^ 1>{});
                 if (n - 2 >= n_min) load_pages(n - 2);
+            } else if constexpr (KV8) {
+                load_tile8(n - 1);
+                if (n - 2 >= n_min) load_pages8(n - 2);
             } else {
                 load_tile(n - 1);
                 if (n - 2 >= n_min) load_pages(n - 2);
@@ -798,6 +879,7 @@ fwd_prefill_kernel(const KParams p, const int n_mblocks) {
         }  // !skip
 
         if constexpr (TO_LDS) __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0) before the barrier
+        else if constexpr (KV8) { if (has_next) store_tile8(std::integral_constant<int, BUF ^ 1>{}); }
         else if (has_next) store_tile(std::integral_constant<int, BUF ^ 1>{});
         STAMP(4);
         __syncthreads();
@@ -872,9 +954,13 @@ fwd_prefill_kernel(const KParams p, const int n_mblocks) {
     FWD_BLK_STAMP(3);
 }
 
+inline const KParams &host_params(const KParams &p) { return p; }
+inline const KParams &host_params(const KV8Params &a) { return a.p; }
+
 template <int DP, bool BF16, int NW, int LD, bool DROP = false, bool SPLIT = false, bool PACK = false, int DV = DP>
-static hipError_t launch_prefill_impl(const KParams &p, hipStream_t stream) {
+static hipError_t launch_prefill_impl(const std::conditional_t<LD == 5, KV8Params, KParams> &args, hipStream_t stream) {
     using Cfg = PrefillCfg<DP, BF16, NW>;
+    const KParams &p = host_params(args);
     const int n_mblocks = (p.seqlen_q * (PACK ? p.pack_gqa : 1) + Cfg::BM - 1) / Cfg::BM;
     const long long blocks = (long long)n_mblocks * p.b * p.h;   // (PACK: p.h is the KV head count)
     if (blocks <= 0) return hipSuccess;
@@ -882,7 +968,7 @@ static hipError_t launch_prefill_impl(const KParams &p, hipStream_t stream) {
     static std::atomic<uint64_t> lds_set{0};
     if (hipError_t e = set_dyn_lds_once((const void *)kern, Cfg::LDS_BYTES, lds_set); e != hipSuccess) return e;
     hipLaunchKernelGGL(kern, dim3((unsigned)blocks, SPLIT ? (unsigned)p.num_splits : 1u), dim3(Cfg::NT),
-                       Cfg::LDS_BYTES, stream, p, n_mblocks);
+                       Cfg::LDS_BYTES, stream, args, n_mblocks);
     return hipGetLastError();
 }
 
@@ -957,6 +1043,24 @@ hipError_t run_fwd_prefill_pack(const KParams &p_in, hipStream_t stream) {
     if (p.d <= 64) return bf ? launch_pack_s<64, true>(p, stream) : launch_pack_s<64, false>(p, stream);
     if (p.d <= 128) return bf ? launch_pack_s<128, true>(p, stream) : launch_pack_s<128, false>(p, stream);
     return bf ? launch_pack_s<256, true>(p, stream) : launch_pack_s<256, false>(p, stream);
+}
+#elif defined(VFA_KV8_TU)
+// Longer queries over an 8-bit cache, a translation unit of its own (fwd_prefill_kv8.hip): the query heads of
+// a KV head packed into the rows (one head per KV head is a group of one).
+template <int DP, bool BF16>
+static hipError_t launch_kv8_prefill(const KV8Params &a, hipStream_t stream) {
+    return a.p.num_splits > 1 ? launch_prefill_impl<DP, BF16, 4, 5, false, true, true>(a, stream)
+                              : launch_prefill_impl<DP, BF16, 4, 5, false, false, true>(a, stream);
+}
+hipError_t run_fwd_kv8_prefill(const KV8Params &a_in, hipStream_t stream) {
+    KV8Params a = a_in;
+    a.p.pack_gqa = a_in.p.h_ratio;   // the grid walks the KV heads
+    a.p.h = a_in.p.h_k;
+    a.p.h_ratio = 1;
+    const bool bf = a.p.is_bf16;
+    if (a.p.d <= 64) return bf ? launch_kv8_prefill<64, true>(a, stream) : launch_kv8_prefill<64, false>(a, stream);
+    if (a.p.d <= 128) return bf ? launch_kv8_prefill<128, true>(a, stream) : launch_kv8_prefill<128, false>(a, stream);
+    return bf ? launch_kv8_prefill<256, true>(a, stream) : launch_kv8_prefill<256, false>(a, stream);
 }
 #elif defined(VFA_FWD64_TU)
 // The d <= 64 instantiations, a translation unit of their own (fwd_prefill_d64.hip) because they are
