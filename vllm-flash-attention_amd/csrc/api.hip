@@ -558,6 +558,8 @@ static int kv8_fill(const vfa_kv8_params *p, vfa::KV8Params &k) {
     VFA_CHECK(aligned16(a.k) && aligned16(a.v) && a.k_batch_stride % 16 == 0 && a.k_row_stride % 16 == 0 && a.k_head_stride % 16 == 0 &&
                   a.v_batch_stride % 16 == 0 && a.v_row_stride % 16 == 0 && a.v_head_stride % 16 == 0,
               "8-bit KV cache: codes must be 16-byte aligned, strides multiples of 16 bytes");
+    for (int64_t r : {a.k_row_stride, a.v_row_stride, p->k_scale_row_stride, p->v_scale_row_stride})
+        VFA_CHECK(r >= 0 && r < (int64_t)1 << 31, "8-bit KV cache: row strides must be under 2 GiB");
     fill_common(&a, k.p, a.seqlen_q, a.seqlen_k);
     k.p.k_cumulative = 0;
     k.ks = (unsigned char *)p->k_scale; k.vs = (unsigned char *)p->v_scale;

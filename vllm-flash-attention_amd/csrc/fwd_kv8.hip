@@ -53,17 +53,22 @@ __device__ __forceinline__ float quad_sum(float x) {
 // 16-byte chunk of row `row` of the V image: the 16 rows that 32 lanes of a transposed read touch lie in
 // different banks
 template <int DP>
-__device__ __forceinline__ int kv8_swz(int row) {
+__host__ __device__ constexpr int kv8_swz(int row) {
     if constexpr (DP == 64) return ((row >> 2) & 1) | ((row >> 4) & 1) << 1;
     else if constexpr (DP == 128) return ((row >> 1) & 3) | ((row >> 4) & 1) << 2;
     else return (row & 7) | ((row >> 4) & 1) << 3;
 }
 
-// Columns from p.d to DP are zero in Q, and their K and V codes are not loaded (zeros).
-template <int DP, bool BF16, int NR>
-__global__ void __launch_bounds__(A_NT, (NR == 1 && DP == 64) ? 4 : 2)
+// Columns from p.d to DP are zero in Q; a lane whose columns lie there reads column 0 of its key instead (a
+// finite code times zero, or a NaN that the key has anyway), its O is never stored.
+//
+// The loop is free of branches on the usual path, loads run NBUF steps ahead of their use (past the last
+// step they repeat it), and the page ids another step ahead of the loads.
+template <int DP, bool BF16, int NR, bool PAGED>
+__global__ void __launch_bounds__(A_NT, 2)
 fwd_kv8_kernel(const KV8Params a, const int n_mblocks) {
     using Cfg = Kv8Cfg<DP, NR>;
+    constexpr int NBUF = DP <= 128 ? 2 : 1;
     constexpr int NJ = DP / 64;              // 64-column groups of K: one 16-byte load per lane and key tile
     constexpr int NDB = DP / 16;             // 16-column blocks of O
     constexpr int CPR = DP / 16;             // 16-byte chunks of a V row
@@ -158,33 +163,56 @@ fwd_kv8_kernel(const KV8Params a, const int n_mblocks) {
     const unsigned char *kbase = (const unsigned char *)p.k + (int64_t)hk * p.k_hs;
     const unsigned char *vbase = (const unsigned char *)p.v + (int64_t)hk * p.v_hs;
     const unsigned char *ksb = a.ks + (int64_t)hk * a.ks_hs, *vsb = a.vs + (int64_t)hk * a.vs_hs;
+    const int k_rs = (int)p.k_rs, v_rs = (int)p.v_rs, ks_rs = (int)a.ks_rs, vs_rs = (int)a.vs_rs;
 
-    i32x4 kreg[2][NJ], vreg[NV];
-    unsigned ksc[2], vsc[2];
-    // Loads of the step n.  A tile of 16 keys lies in one page and one block of the scales (both are multiples
-    // of 16 rows); one that starts past the sequence's end takes the sequence's last tile (its keys are masked).
-    auto load_step = [&](int n) __attribute__((always_inline)) {
+    // lane offsets inside a tile of 16 keys: K 16 columns of key c, V chunk lane + 64 i
+    int64_t koff[NJ], voff[NV / 2];
+#pragma unroll
+    for (int j = 0; j < NJ; j++) koff[j] = (int64_t)c * k_rs + (64 * j + 16 * g < p.d ? 64 * j + 16 * g : 0);
+#pragma unroll
+    for (int i = 0; i < NV / 2; i++) {
+        const int ci = lane + 64 * i, vc = ci % CPR * 16;
+        voff[i] = (int64_t)(ci / CPR) * v_rs + (vc < p.d ? vc : 0);
+    }
+
+    struct Set {                 // one step's loads
+        i32x4 k[2][NJ], v[NV];
+        unsigned ks[2], vs[2];
+    };
+    Set set[NBUF];
+    const int last_tile = (sk - 1) & ~15;
+    int pid[2];
+    // Page ids of a step's two tiles.  A tile of 16 keys lies in one page and in one block of the scales (both
+    // are multiples of 16 rows); one that starts past the sequence's end takes its last tile (masked keys).
+    const int *table = PAGED ? p.block_table + (int64_t)bidb * p.bt_bs : nullptr;
+    if constexpr (!PAGED) pid[0] = pid[1] = p.cache_batch_idx ? p.cache_batch_idx[bidb] : bidb;
+    auto load_pages = [&](int n) __attribute__((always_inline)) {
+        if constexpr (PAGED) {
+#pragma unroll
+            for (int t = 0; t < 2; t++)
+                pid[t] = table[kv8_div(min(n * A_STEP + 16 * t, last_tile) >> 4, a.page_mul, a.page_sh)];
+        }
+    };
+    auto load_step = [&](int n, Set &w) __attribute__((always_inline)) {
+        const unsigned char *vt[2];
 #pragma unroll
         for (int t = 0; t < 2; t++) {
-            const int key = min(n * A_STEP + 16 * t, (sk - 1) & ~15);
-            const int page = __builtin_amdgcn_readfirstlane(kv8_page(a, bidb, key));
-            const int row = kv8_row_in_page(a, key);
-            const int64_t pg = max(page, 0);
+            const int key = min(n * A_STEP + 16 * t, last_tile);
+            const int page = __builtin_amdgcn_readfirstlane(pid[t]);
+            const bool bad = (unsigned)page >= (unsigned)a.num_pages;   // outside the pool: NaN, from the scale
+            const int64_t pg = bad ? 0 : page;
+            const int row = PAGED ? key - kv8_div(key >> 4, a.page_mul, a.page_sh) * a.page_rows : key;
             const int blk = kv8_div(row >> 4, a.blk_mul, a.blk_sh);
-            // (a page outside the pool: NaN, from the scale)
-            ksc[t] = page < 0 ? 255u : ksb[pg * a.ks_bs + blk * a.ks_rs];
-            vsc[t] = page < 0 ? 255u : vsb[pg * a.vs_bs + blk * a.vs_rs];
-            const unsigned char *kp = kbase + pg * p.k_bs + (int64_t)(row + c) * p.k_rs + 16 * g;
-            const unsigned char *vp = vbase + pg * p.v_bs + (int64_t)row * p.v_rs;
+            const unsigned char *kt = kbase + pg * p.k_bs + (int64_t)row * k_rs;
 #pragma unroll
-            for (int j = 0; j < NJ; j++)
-                kreg[t][j] = 64 * j + 16 * g < p.d ? *(const i32x4 *)(kp + 64 * j) : i32x4{0, 0, 0, 0};
-#pragma unroll
-            for (int i = 0; i < NV / 2; i++) {
-                const int ci = lane + 64 * i, vr = ci / CPR, vc = ci % CPR * 16;
-                vreg[t * (NV / 2) + i] = vc < p.d ? *(const i32x4 *)(vp + (int64_t)vr * p.v_rs + vc) : i32x4{0, 0, 0, 0};
-            }
+            for (int j = 0; j < NJ; j++) w.k[t][j] = *(const i32x4 *)(kt + koff[j]);
+            const unsigned kb = ksb[pg * a.ks_bs + (int64_t)blk * ks_rs], vb = vsb[pg * a.vs_bs + (int64_t)blk * vs_rs];
+            w.ks[t] = bad ? 255u : kb;
+            w.vs[t] = bad ? 255u : vb;
+            vt[t] = vbase + pg * p.v_bs + (int64_t)row * v_rs;
         }
+#pragma unroll
+        for (int i = 0; i < NV; i++) w.v[i] = *(const i32x4 *)(vt[i / (NV / 2)] + voff[i % (NV / 2)]);
     };
 
     f32x4 o[NR][NDB];
@@ -202,19 +230,18 @@ fwd_kv8_kernel(const KV8Params a, const int n_mblocks) {
     const int tj = c >> 1, trow = (tj < 4 ? 4 * g + tj : 12 + 4 * g + tj);
     const char *tr_base = vimg + trow * DP + (c & 1) * 8;
     const int tr_swz = kv8_swz<DP>(trow) << 4;
-
-    const int first = n0 + part;
-    if (first < n1) load_step(first);
-    for (int n = first; n < n1; n += parts) {
-        const int k0 = n * A_STEP;
-        const bool tail = k0 < vis_lo || k0 + A_STEP > vis_hi;   // keys that no row sees: V must not count, whatever stands there
+    int vwr[NV / 2];             // where a lane's V chunks go (the second tile: 16 rows on, chunks turned by a constant)
 #pragma unroll
-        for (int i = 0; i < NV; i++) {
-            const int ci = lane + 64 * (i % (NV / 2)), vr = ci / CPR + 16 * (i / (NV / 2)), ch = ci % CPR;
-            if (tail && (k0 + vr < vis_lo || k0 + vr >= vis_hi)) vreg[i] = i32x4{0, 0, 0, 0};
-            *(i32x4 *)(vimg + vr * DP + ((ch ^ kv8_swz<DP>(vr)) << 4)) = vreg[i];
-        }
-        const float ks[2] = {e8m0_to_f32(ksc[0]), e8m0_to_f32(ksc[1])}, vs[2] = {e8m0_to_f32(vsc[0]), e8m0_to_f32(vsc[1])};
+    for (int i = 0; i < NV / 2; i++) {
+        const int ci = lane + 64 * i;
+        vwr[i] = (ci / CPR) * DP + ((ci % CPR ^ kv8_swz<DP>(ci / CPR)) << 4);
+    }
+    constexpr int SWZ16 = kv8_swz<DP>(16) << 4;
+    const bool has_alibi = p.alibi_slopes != nullptr;
+
+    auto step = [&](const int n, Set &w, const int next) __attribute__((always_inline)) {
+        const int k0 = n * A_STEP;
+        const float ks[2] = {e8m0_to_f32(w.ks[0]), e8m0_to_f32(w.ks[1])}, vs[2] = {e8m0_to_f32(w.vs[0]), e8m0_to_f32(w.vs[1])};
         f32x4 s[NR][2];
 #pragma unroll
         for (int t = 0; t < 2; t++) {
@@ -222,8 +249,8 @@ fwd_kv8_kernel(const KV8Params a, const int n_mblocks) {
             for (int r = 0; r < NR; r++) s[r][t] = f32x4{0, 0, 0, 0};
 #pragma unroll
             for (int j = 0; j < NJ; j++) {
-                const i32x4 k_lo = kv8_to16<BF16>(i32x2{kreg[t][j][0], kreg[t][j][1]}, ks[t]);
-                const i32x4 k_hi = kv8_to16<BF16>(i32x2{kreg[t][j][2], kreg[t][j][3]}, ks[t]);
+                const i32x4 k_lo = kv8_to16<BF16>(i32x2{w.k[t][j][0], w.k[t][j][1]}, ks[t]);
+                const i32x4 k_hi = kv8_to16<BF16>(i32x2{w.k[t][j][2], w.k[t][j][3]}, ks[t]);
 #pragma unroll
                 for (int r = 0; r < NR; r++) {
                     s[r][t] = mma16<BF16>(k_lo, qf[r][2 * j], s[r][t]);
@@ -231,28 +258,52 @@ fwd_kv8_kernel(const KV8Params a, const int n_mblocks) {
                 }
             }
         }
-        if (n + parts < n1) load_step(n + parts);
+        if (k0 < vis_lo || k0 + A_STEP > vis_hi) {    // V of keys that no row sees must not count, whatever stands there
+#pragma unroll
+            for (int i = 0; i < NV; i++) {
+                const int key = k0 + (lane + 64 * (i % (NV / 2))) / CPR + 16 * (i / (NV / 2));
+                if (key < vis_lo || key >= vis_hi) w.v[i] = i32x4{0, 0, 0, 0};
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < NV; i++) {
+            const int at = i < NV / 2 ? vwr[i] : (vwr[i - NV / 2] ^ SWZ16) + 16 * DP;
+            *(i32x4 *)(vimg + at) = w.v[i];
+        }
+        load_step(min(next, n1 - 1), w);
+        load_pages(min(next + parts, n1 - 1));
 
-        bool need = p.alibi_slopes || k0 + A_STEP > sk;
+        bool need = k0 + A_STEP > sk;
         if (edge_r) need = need || (k0 + A_STEP > pos_lo + 1 + sk - sq + p.wr);
         if (p.is_local) need = need || (k0 < pos_hi + sk - sq - p.wl);
-        i32x4 pf[NR];
+        if (has_alibi) {
 #pragma unroll
-        for (int r = 0; r < NR; r++) {
-            if (need) {
-                const int lo = p.is_local ? max(0, pos[r] + sk - sq - p.wl) : 0;
-                const int hi = edge_r ? min(sk, pos[r] + 1 + sk - sq + p.wr) : sk;
+            for (int r = 0; r < NR; r++) {
+                const float at = p.is_causal ? 0.f : (float)(pos[r] + sk - sq);
 #pragma unroll
                 for (int t = 0; t < 2; t++)
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
-                        const int key = k0 + 16 * t + 4 * g + i;
-                        float x = s[r][t][i];
-                        if (p.alibi_slopes)
-                            x = p.is_causal ? x + slope[r] * (float)key : x - slope[r] * fabsf((float)(pos[r] + sk - sq - key));
-                        s[r][t][i] = (key >= lo && key < hi) ? x : -INFINITY;
+                        const float key = (float)(k0 + 16 * t + 4 * g + i);
+                        s[r][t][i] += slope[r] * (p.is_causal ? key : -fabsf(at - key));
                     }
             }
+        }
+        if (need) {
+#pragma unroll
+            for (int r = 0; r < NR; r++) {
+                const int lo = (p.is_local ? max(0, pos[r] + sk - sq - p.wl) : 0) - k0 - 4 * g;
+                const int hi = (edge_r ? min(sk, pos[r] + 1 + sk - sq + p.wr) : sk) - k0 - 4 * g;
+#pragma unroll
+                for (int t = 0; t < 2; t++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++)
+                        s[r][t][i] = (16 * t + i >= lo && 16 * t + i < hi) ? s[r][t][i] : -INFINITY;
+            }
+        }
+        i32x4 pf[NR];
+#pragma unroll
+        for (int r = 0; r < NR; r++) {
             float mx = fmaxf(fmaxf(fmaxf(s[r][0][0], s[r][0][1]), fmaxf(s[r][0][2], s[r][0][3])),
                              fmaxf(fmaxf(s[r][1][0], s[r][1][1]), fmaxf(s[r][1][2], s[r][1][3])));
             mx = quad_max(mx);
@@ -291,6 +342,24 @@ fwd_kv8_kernel(const KV8Params a, const int n_mblocks) {
             vf[0] = lo[0]; vf[1] = lo[1]; vf[2] = hi[0]; vf[3] = hi[1];
 #pragma unroll
             for (int r = 0; r < NR; r++) o[r][db] = mma16<BF16>(vf, pf[r], o[r][db]);
+        }
+    };
+
+    const int first = n0 + part;
+    if (first < n1) {
+        load_pages(first);
+#pragma unroll
+        for (int i = 0; i < NBUF; i++) {
+            load_step(min(first + i * parts, n1 - 1), set[i]);
+            load_pages(min(first + (i + 1) * parts, n1 - 1));
+        }
+        for (int n = first;;) {
+            step(n, set[0], n + NBUF * parts);
+            if ((n += parts) >= n1) break;
+            if constexpr (NBUF == 2) {
+                step(n, set[1], n + NBUF * parts);
+                if ((n += parts) >= n1) break;
+            }
         }
     }
 
@@ -347,14 +416,14 @@ fwd_kv8_kernel(const KV8Params a, const int n_mblocks) {
     }
 }
 
-template <int DP, bool BF16, int NR>
+template <int DP, bool BF16, int NR, bool PAGED>
 static hipError_t launch_kv8(const KV8Params &a, hipStream_t stream) {
     const KParams &p = a.p;
     const int n_mblocks = (p.seqlen_q * p.h_ratio + 16 * NR - 1) / (16 * NR);
     const long long blocks = (long long)n_mblocks * p.b * (p.h_k / a.heads_per_wg) * p.num_splits;
     if (blocks <= 0) return hipSuccess;
     if (blocks > 0x7fffffffLL) return hipErrorInvalidValue;
-    auto kern = fwd_kv8_kernel<DP, BF16, NR>;
+    auto kern = fwd_kv8_kernel<DP, BF16, NR, PAGED>;
     constexpr int lds = Kv8Cfg<DP, NR>::LDS_BYTES;
     static std::atomic<uint64_t> lds_set{0};
     if (hipError_t e = set_dyn_lds_once((const void *)kern, lds, lds_set); e != hipSuccess) return e;
@@ -362,15 +431,15 @@ static hipError_t launch_kv8(const KV8Params &a, hipStream_t stream) {
     return hipGetLastError();
 }
 
+template <int DP, bool BF16, int NR>
+static hipError_t launch_kv8_layout(const KV8Params &a, hipStream_t stream) {
+    return a.p.block_table ? launch_kv8<DP, BF16, NR, true>(a, stream) : launch_kv8<DP, BF16, NR, false>(a, stream);
+}
 template <int DP, bool BF16>
 static hipError_t launch_kv8_rows(const KV8Params &a, hipStream_t stream) {
-    const int rows = a.p.seqlen_q * a.p.h_ratio;
-    if constexpr (DP == 256) {
-        return launch_kv8<DP, BF16, 1>(a, stream);   // (the accumulators of 32 rows do not fit beside the loads)
-    } else {
-        if (rows <= 16) return launch_kv8<DP, BF16, 1>(a, stream);
-        return launch_kv8<DP, BF16, 2>(a, stream);
-    }
+    if constexpr (DP <= 128)     // (above, the accumulators of 32 rows do not fit beside the loads)
+        if (a.p.seqlen_q * a.p.h_ratio > 16) return launch_kv8_layout<DP, BF16, 2>(a, stream);
+    return launch_kv8_layout<DP, BF16, 1>(a, stream);
 }
 
 // Adjacent KV heads of a workgroup: a key's codes of one head are d bytes, and reads of 512 contiguous bytes
