@@ -250,6 +250,9 @@ typedef struct vfa_kv8_params {
     const int32_t *cu_seqlens_out;
     int64_t rows_out;
     int seqlen_out;
+    /* Attention: scratch of at least vfa_kv8_workspace() bytes, 256-byte aligned (NULL if that is 0). */
+    void *workspace;
+    size_t workspace_bytes;
 } vfa_kv8_params;
 
 /* Write new tokens at positions cu_seqlens_k[i] .. of every sequence.  A block's scale is the least power of
@@ -265,14 +268,15 @@ int vfa_kv8_quantize(const vfa_kv8_params *p);
 int vfa_kv8_dequantize(const vfa_kv8_params *p);
 
 /* Attention of q (dense (b, seqlen_q, h, d), or ragged with cu_seqlens_q) over the cache: a.q, a.out,
- * a.softmax_lse, masks, ALiBi, a.num_splits with its scratch as for vfa_mha_fwd_kvcache.  With a.knew the new
- * tokens (dense) are written first and attended. */
+ * a.softmax_lse, masks and ALiBi as for vfa_mha_fwd_kvcache.  With a.knew the new tokens (dense) are written
+ * first and attended.  a.num_splits: 0 = chosen here, n = at most n parts of a sequence's keys.  Partial results
+ * -- and for long queries the cache in 16 bits -- go to `workspace` (a.oaccum and a.softmax_lseaccum are not
+ * used); nothing in it has to be set. */
 int vfa_kv8_mha_fwd(const vfa_kv8_params *p);
 
-/* The num_splits that vfa_kv8_mha_fwd should be given: enough (batch, KV head group, 16- or 32-row block) work
- * items to fill num_cus compute units, at least 256 keys each. */
-int vfa_kv8_num_splits(int batch, int num_heads, int num_heads_k, int head_size, int max_seqlen_k, int max_seqlen_q,
-                       int num_cus);
+/* Bytes of workspace that vfa_kv8_mha_fwd needs for these arguments (of the pointers only whether they are
+ * NULL counts). */
+size_t vfa_kv8_workspace(const vfa_kv8_params *p);
 
 /* RMS norm of every head of q (b, s, h, d) and k (b, s, h_k, d), times a weight (d), then the position rotation of its first
  * rotary_dim columns (pairs (2i, 2i + 1) if interleaved, else (i, i + rotary_dim / 2)):

@@ -32,7 +32,9 @@ hipError_t run_kv8_quantize(const KV8Params &a, hipStream_t stream);            
 hipError_t run_kv8_dequantize(const KV8Params &a, hipStream_t stream);
 hipError_t run_fwd_kv8(const KV8Params &a, hipStream_t stream);                  // fwd_kv8.hip
 int kv8_heads_per_wg(int d, int h_k);
-bool kv8_takes_prefill(int d, int h_ratio, int seqlen_q);
+int kv8_decode_rows(int d, int rows);
+int kv8_decode_wgs_per_cu(int d, int rows);
+hipError_t run_fwd_kv8_prefill(const KV8Params &a, hipStream_t stream);          // fwd_prefill_kv8.hip
 hipError_t run_qk_norm_rotary(const QKNormParams &p, bool bwd, hipStream_t stream);   // qk_norm_rotary.hip
 void qk_norm_bwd_blocks(QKNormParams &p, int cus);
 }  // namespace vfa
@@ -559,7 +561,7 @@ static int kv8_fill(const vfa_kv8_params *p, vfa::KV8Params &k) {
                   a.v_batch_stride % 16 == 0 && a.v_row_stride % 16 == 0 && a.v_head_stride % 16 == 0,
               "8-bit KV cache: codes must be 16-byte aligned, strides multiples of 16 bytes");
     for (int64_t r : {a.k_row_stride, a.v_row_stride, p->k_scale_row_stride, p->v_scale_row_stride})
-        VFA_CHECK(r >= 0 && r < (int64_t)1 << 31, "8-bit KV cache: row strides must be under 2 GiB");
+        VFA_CHECK(r >= 0 && r < (int64_t)1 << 27, "8-bit KV cache: row strides must be under 128 MiB");
     fill_common(&a, k.p, a.seqlen_q, a.seqlen_k);
     k.p.k_cumulative = 0;
     k.ks = (unsigned char *)p->k_scale; k.vs = (unsigned char *)p->v_scale;
@@ -620,31 +622,111 @@ extern "C" int vfa_kv8_dequantize(const vfa_kv8_params *p) {
     return VFA_OK;
 }
 
-extern "C" int vfa_kv8_num_splits(int batch, int num_heads, int num_heads_k, int head_size, int max_seqlen_k, int max_seqlen_q,
-                                  int num_cus_) {
-    if (num_heads_k <= 0 || num_heads % num_heads_k != 0 || head_size <= 0 || batch <= 0) return 1;
-    const int ratio = num_heads / num_heads_k;
-    if (vfa::kv8_takes_prefill(head_size, ratio, max_seqlen_q)) {
-        // 128-row blocks, two workgroups per CU; split only what would fill less than a quarter of them (the
-        // rule of the 16-bit path's packed rows), at least four 64-key tiles each
-        const long long blocks = (long long)batch * num_heads_k * (((long long)max_seqlen_q * ratio + 127) / 128);
-        const long long chunks = ((long long)max_seqlen_k + 255) / 256;
-        if (blocks * 4 > 2LL * num_cus_ || chunks < 2) return 1;
-        return (int)std::min({chunks, 2LL * num_cus_ / blocks, 128LL});
+// Most (query position, head) rows of a KV head that the decode kernel takes, and the rows from which reading the
+// cache back and the 16-bit kernels are ahead of the prefill kernel over the codes.
+constexpr int VFA_KV8_DECODE_ROWS = 64, VFA_KV8_READ_BACK_ROWS = 1024, VFA_KV8_READ_BACK_ROWS_WIDE = 192;
+
+// How a call is carried out: sequences of few (query position, head) rows by the decode kernel, the others by the
+// prefill kernel -- over the codes, or over the cache read back into 16 bits first.
+struct Kv8Plan {
+    bool decode, prefill, read_back;
+    int dec_sq, dec_rows;        // most query positions and rows of a sequence of the decode kernel's
+    int dec_splits, pre_splits;
+    int goal, grid;              // decode: parts of all sequences to aim at per head group and row block, the most there can be
+    size_t o, lse, n_split;      // decode: offsets into the workspace
+    size_t pre_o, pre_lse;       // prefill
+    size_t k16, v16, lens;       // read back
+    size_t bytes;
+};
+
+static int kv8_plan(const vfa_kv8_params *p, Kv8Plan &w) {
+    const vfa_params &a = p->a;
+    std::memset(&w, 0, sizeof(w));
+    const int ratio = a.h / a.h_k, cus = num_cus();
+    const long long rows = (long long)a.seqlen_q * ratio;
+    w.dec_rows = VFA_KV8_DECODE_ROWS;
+    w.prefill = rows > w.dec_rows;
+    // a dense batch is all one kind; of a ragged one with long members only the lengths on the device know
+    w.decode = !w.prefill || (a.cu_seqlens_q && ratio <= w.dec_rows);
+    w.dec_sq = w.prefill ? std::max(1, w.dec_rows / ratio) : a.seqlen_q;
+    if (!w.decode) w.dec_rows = 0;
+    size_t at = 0;
+    auto take = [&](size_t bytes) { const size_t o = at; at += (bytes + 255) / 256 * 256; return o; };
+    if (w.decode) {
+        const int hpw = vfa::kv8_heads_per_wg(a.d, a.h_k), parts = 8 / hpw;
+        const int per = vfa::kv8_decode_rows(a.d, w.dec_sq * ratio);
+        const int mblocks = (w.dec_sq * ratio + per - 1) / per;
+        const long long items = (long long)a.b * (a.h_k / hpw) * mblocks;
+        // Parts of all sequences together: one workgroup each fills the device once.  A sequence may take up to four
+        // times the average (their lengths can differ), as many as its keys allow.
+        const int groups = (int)std::max(1LL, items / a.b);
+        const long long most = std::max(1LL, (long long)a.seqlen_k / (32LL * 3 * parts));
+        w.goal = std::max(1, cus * vfa::kv8_decode_wgs_per_cu(a.d, w.dec_sq * ratio) / groups);
+        const long long s = a.num_splits > 0 ? a.num_splits : w.goal * 2 <= a.b ? 1 : a.b == 1 ? w.goal : 4LL * ((w.goal + a.b - 1) / a.b);
+        w.dec_splits = (int)std::max(1LL, std::min({s, most, 128LL}));
+        // (a count given: the grid holds that many parts of every sequence)
+        w.grid = (int)std::min<long long>(0x7fffffff, a.num_splits > 0 ? (long long)a.b * w.dec_splits : std::max(w.goal, a.b));
+        if (a.num_splits > 0) w.goal = w.grid;
+        if (w.dec_splits > 1) {
+            const size_t n = (size_t)w.dec_splits * a.b * a.h * w.dec_sq;
+            w.o = take(n * a.d * sizeof(float));
+            w.lse = take(n * sizeof(float));
+            w.n_split = take((size_t)a.b * mblocks * sizeof(int));
+        }
     }
-    const int hpw = vfa::kv8_heads_per_wg(head_size, num_heads_k), parts = 8 / hpw;
-    const long long items = (long long)batch * (num_heads_k / hpw) * (((long long)max_seqlen_q * ratio + 31) / 32);
-    // two workgroups per CU; a wave keeps at least 4 of its steps of 32 keys
-    const long long most = std::max(1LL, (long long)max_seqlen_k / (32LL * 4 * parts));
-    const long long want = (2LL * num_cus_ + items - 1) / std::max(1LL, items);
-    return (int)std::max(1LL, std::min({want, most, 128LL}));
+    if (w.prefill) {
+        const size_t codes = (size_t)a.b * a.seqlen_k * a.h_k * a.d;
+        w.read_back = rows >= (a.d <= 128 ? VFA_KV8_READ_BACK_ROWS : VFA_KV8_READ_BACK_ROWS_WIDE) && codes * 4 <= (size_t)2 << 30;
+        w.pre_splits = 1;
+        if (w.read_back) {
+            w.k16 = take(codes * 2);
+            w.v16 = take(codes * 2);
+            w.lens = take((size_t)a.b * sizeof(int));
+            if (!a.cu_seqlens_q)
+                w.pre_splits = a.num_splits > 0 ? a.num_splits : vfa_decode_num_splits(a.b, a.h, a.h_k, a.d, a.seqlen_k, a.seqlen_q, cus);
+        } else if (!a.cu_seqlens_q) {
+            // 128-row blocks, two workgroups per CU; split only what would fill less than half of them (a part's
+            // fp32 results cost HBM traffic in proportion to its rows), at least four 64-key tiles each
+            const long long blocks = (long long)a.b * a.h_k * ((rows + 127) / 128);
+            const long long chunks = ((long long)a.seqlen_k + 255) / 256;
+            long long s = a.num_splits > 0 ? a.num_splits : blocks * 2 > 2LL * cus ? 1 : 2LL * cus / blocks;
+            w.pre_splits = (int)std::max(1LL, std::min({s, chunks, 128LL}));
+        }
+        if (w.pre_splits > 1) {
+            const size_t n = (size_t)w.pre_splits * a.b * a.h * a.seqlen_q;
+            w.pre_o = take(n * a.d * sizeof(float));
+            w.pre_lse = take(n * sizeof(float));
+        }
+    }
+    w.bytes = at;
+    return VFA_OK;
+}
+
+static int kv8_fwd_checks(const vfa_kv8_params *p, vfa::KV8Params &k) {
+    std::memset(&k, 0, sizeof(k));
+    int rc = kv8_fill(p, k);
+    if (rc) return rc;
+    const vfa_params &a = p->a;
+    VFA_CHECK(a.h > 0 && a.h % a.h_k == 0, "Number of heads in key/value must divide number of heads in query");
+    VFA_CHECK(a.seqlen_q >= 0 && a.num_splits >= 0, "negative size");
+    VFA_CHECK(a.num_splits <= 128, "num_splits > 128 not supported");
+    VFA_CHECK((long long)a.seqlen_q * a.h <= 1 << 30, "seqlen_q out of range");
+    return VFA_OK;
+}
+
+extern "C" size_t vfa_kv8_workspace(const vfa_kv8_params *p) {
+    g_err.clear();
+    vfa::KV8Params k;
+    if (kv8_fwd_checks(p, k)) return 0;
+    Kv8Plan w;
+    kv8_plan(p, w);
+    return w.bytes;
 }
 
 extern "C" int vfa_kv8_mha_fwd(const vfa_kv8_params *p) {
     g_err.clear();
     vfa::KV8Params k;
-    std::memset(&k, 0, sizeof(k));
-    int rc = kv8_fill(p, k);
+    int rc = kv8_fwd_checks(p, k);
     if (rc) return rc;
     const vfa_params &a = p->a;
     if ((rc = common_checks(&a))) return rc;
@@ -655,24 +737,66 @@ extern "C" int vfa_kv8_mha_fwd(const vfa_kv8_params *p) {
                   a.o_batch_stride % 8 == 0 && a.o_row_stride % 8 == 0 && a.o_head_stride % 8 == 0,
               "q and out must be 16-byte aligned, strides multiples of 8 elements");
     if ((rc = check_arch())) return rc;
-    if (a.seqlen_q <= 0) return VFA_OK;
+    Kv8Plan w;
+    kv8_plan(p, w);
+    VFA_CHECK(w.bytes == 0 || (p->workspace && p->workspace_bytes >= w.bytes && ((uintptr_t)p->workspace & 255) == 0),
+              "8-bit KV cache: workspace missing, too small (vfa_kv8_workspace) or not 256-byte aligned");
     hipStream_t stream = (hipStream_t)a.stream;
     hipError_t e;
     if (a.knew) {
         e = vfa::run_kv8_quantize(k, stream);
         if (e != hipSuccess) return hip_fail(e, "kv8 quantize launch");
     }
-    if (a.num_splits > 1) {
-        VFA_CHECK(a.num_splits <= 128, "num_splits > 128 not supported");
-        VFA_CHECK(a.oaccum && a.softmax_lseaccum, "split-KV needs oaccum / softmax_lseaccum scratch");
-        k.p.num_splits = a.num_splits;
-        k.p.oaccum = a.oaccum;
-        k.p.lseaccum = a.softmax_lseaccum;
+    if (a.seqlen_q == 0) return VFA_OK;
+    char *ws = (char *)p->workspace;
+    k.min_rows = w.dec_rows;
+    if (w.prefill && w.read_back) {
+        vfa::KV8Params r = k;
+        r.k_out = ws + w.k16; r.v_out = ws + w.v16;
+        r.lens_out = (int *)(ws + w.lens);
+        r.ko_hs = r.vo_hs = a.d; r.ko_rs = r.vo_rs = (int64_t)a.h_k * a.d; r.ko_bs = r.vo_bs = r.ko_rs * a.seqlen_k;
+        r.rows_out = (int64_t)a.b * a.seqlen_k; r.seqlen_out = a.seqlen_k;
+        e = vfa::run_kv8_dequantize(r, stream);
+        if (e != hipSuccess) return hip_fail(e, "kv8 dequantize launch");
+        vfa_params q = a;
+        q.k = r.k_out; q.v = r.v_out;
+        q.k_batch_stride = q.v_batch_stride = r.ko_bs; q.k_row_stride = q.v_row_stride = r.ko_rs; q.k_head_stride = q.v_head_stride = a.d;
+        q.cu_seqlens_k = r.lens_out; q.is_seqlens_k_cumulative = 0;
+        q.block_table = nullptr; q.cache_batch_idx = nullptr; q.knew = q.vnew = nullptr;
+        q.total_q = 0;   // (what is left are the long sequences: not packed for the sake of the short ones)
+        q.num_splits = w.pre_splits;
+        q.oaccum = w.pre_splits > 1 ? (float *)(ws + w.pre_o) : nullptr;
+        q.softmax_lseaccum = w.pre_splits > 1 ? (float *)(ws + w.pre_lse) : nullptr;
+        KParams k16;
+        fill_common(&q, k16, q.seqlen_q, q.seqlen_k);
+        k16.k_cumulative = 0;
+        if ((rc = launch_fwd(&q, k16, false))) return rc;
+    } else if (w.prefill) {
+        vfa::KV8Params f = k;
+        if (w.pre_splits > 1) {
+            f.p.num_splits = w.pre_splits;
+            f.p.oaccum = (float *)(ws + w.pre_o);
+            f.p.lseaccum = (float *)(ws + w.pre_lse);
+        }
+        e = vfa::run_fwd_kv8_prefill(f, stream);
+        if (e == hipSuccess && w.pre_splits > 1) e = vfa::run_fwd_combine(f.p, stream);
+        if (e != hipSuccess) return hip_fail(e, "kv8 prefill launch");
     }
-    k.heads_per_wg = vfa::kv8_heads_per_wg(a.d, a.h_k);
-    e = vfa::run_fwd_kv8(k, stream);
-    if (e == hipSuccess && a.num_splits > 1) e = vfa::run_fwd_combine(k.p, stream);
-    if (e != hipSuccess) return hip_fail(e, "kv8 attention launch");
+    if (w.decode) {   // (after the 16-bit kernels, which write zeros for the sequences that are not theirs)
+        k.heads_per_wg = vfa::kv8_heads_per_wg(a.d, a.h_k);
+        k.max_rows = w.prefill ? w.dec_rows : 0;
+        k.acc_sq = w.dec_sq;
+        k.p.num_splits = w.dec_splits;
+        if (w.dec_splits > 1) {
+            k.p.oaccum = (float *)(ws + w.o);
+            k.p.lseaccum = (float *)(ws + w.lse);
+            k.n_split = (int *)(ws + w.n_split);
+            k.split_goal = w.goal;
+            k.split_grid = w.grid;
+        }
+        e = vfa::run_fwd_kv8(k, stream);
+        if (e != hipSuccess) return hip_fail(e, "kv8 attention launch");
+    }
     return VFA_OK;
 }
 

@@ -18,11 +18,13 @@
 //     keys in the order {4g .. 4g+3, 16+4g .. 16+4g+3} for lane group g: ds_read_b64_tr_b8 reads any 8 rows,
 //     so V goes through a wave-private LDS image as codes and comes back transposed, to be converted there.
 #include "vfa_kv8.h"
+#include <algorithm>
 
 namespace vfa {
 
 constexpr int A_NW = 8, A_NT = A_NW * 64;
 constexpr int A_STEP = 32;                   // keys of a step
+constexpr int A_MIN_STEPS = 3;               // least steps of a wave in a part of the keys
 
 template <int DP, int NR>
 struct Kv8Cfg {
@@ -64,8 +66,14 @@ __host__ __device__ constexpr int kv8_swz(int row) {
 //
 // The loop is free of branches on the usual path, loads run NBUF steps ahead of their use (past the last
 // step they repeat it), and the page ids another step ahead of the loads.
-template <int DP, bool BF16, int NR, bool PAGED>
-__global__ void __launch_bounds__(A_NT, 2)
+// NT: the codes are loaded past the caches.  For streams that the 256 MiB last-level cache cannot hold anyway
+// (b128 kv8192 h32/8 d128: 5.85 -> 6.23 TB/s); shorter ones find part of it there (b1 kv65536: 37 against 50 us).
+//
+// The keys of a sequence are cut into parts for separate workgroups when there are too few (sequence, head group,
+// row block) items for the chip.  How many is decided here, from the lengths of all sequences: parts of equal
+// length, so that a batch of long and short sequences fills the chip evenly.
+template <int DP, bool BF16, int NR, bool PAGED, bool NT>
+__global__ void __launch_bounds__(A_NT, (DP == 64 && NR == 1) ? 4 : 2)
 fwd_kv8_kernel(const KV8Params a, const int n_mblocks) {
     using Cfg = Kv8Cfg<DP, NR>;
     constexpr int NBUF = DP <= 128 ? 2 : 1;
@@ -82,36 +90,105 @@ fwd_kv8_kernel(const KV8Params a, const int n_mblocks) {
     const int hpw = a.heads_per_wg, parts = A_NW / hpw;
     const int whead = wave & (hpw - 1), part = wave / hpw;
 
-    // blocks of one (batch, head group) -- its splits and row blocks -- run on one XCD at about the same time
+    // row blocks of the same keys on one XCD, whose L2 they share
     int L = blockIdx.x;
-    if (p.num_splits > 1 || n_mblocks > 1) {
-        const int per_xcd = gridDim.x / 8;
-        if (L < per_xcd * 8) L = (L % 8) * per_xcd + L / 8;
+    if (n_mblocks > 1) {
+        const int group = 8 * n_mblocks;
+        if (L < (int)gridDim.x / group * group) {
+            const int k = L / 8;
+            L = k / n_mblocks * group + L % 8 * n_mblocks + k % n_mblocks;
+        }
     }
     const int n_hblocks = p.h_k / hpw;
     const int m_block = L % n_mblocks; L /= n_mblocks;
     const int hblock = L % n_hblocks; L /= n_hblocks;
-    const int split = L % p.num_splits; L /= p.num_splits;
-    const int bidb = L;
     const int hk = hblock * hpw + whead;
     const int ratio = p.h_ratio;
-    const bool is_split = p.num_splits > 1;
+    const int q0 = m_block * 16 * NR;
+
+    // L -> (sequence, part of its keys)
+    int bidb = L, split = 0, nsplit = 1;
+    if (p.num_splits > 1) {
+        // steps of sequence i as this row block sees them, about; -1: not this launch's
+        const int span = p.is_local ? (min(p.wl, a.cap) + min(p.wr, a.cap) + 16 * NR) / A_STEP + 2 : 1 << 30;
+        auto steps_of = [&](int i) -> int {
+            if (i >= p.b) return -1;
+            const int len = min(kv8_cached(a, i) + (p.knew ? p.seqlen_knew : 0), a.cap);
+            const int qi = (p.cu_seqlens_q ? p.cu_seqlens_q[i + 1] - p.cu_seqlens_q[i] : p.seqlen_q) * ratio;
+            return qi > q0 && !(a.max_rows > 0 && qi > a.max_rows) ? min((len + A_STEP - 1) / A_STEP, span) : -1;
+        };
+        auto parts_of = [](int st, int part_steps) -> int { return st < 0 ? 0 : max(1, (st + part_steps - 1) / part_steps); };
+        auto wave_sum = [](int x) {
+#pragma unroll
+            for (int off = 32; off > 0; off >>= 1) x += __shfl_xor(x, off);
+            return x;
+        };
+        // Every wave works this out for itself, a lane a sequence (64 at a time): no barrier.  Steps of a part: the
+        // total over the goal, less about half a part that every sequence leaves over; if the parts then are more
+        // than the goal after all (a second round of workgroups), less a whole one each.  Not so few that a
+        // sequence needs more parts than there is scratch for.
+        const int st0 = steps_of(lane);
+        int sum = max(st0, 0), top = sum, some = st0 >= 0;
+        for (int i = lane + 64; i < p.b; i += 64) {
+            const int st = steps_of(i);
+            sum += max(st, 0);
+            top = max(top, st);
+            some += st >= 0;
+        }
+        sum = wave_sum(sum);
+        some = wave_sum(some);
+#pragma unroll
+        for (int off = 32; off > 0; off >>= 1) top = max(top, __shfl_xor(top, off));
+        const int least = max((top + p.num_splits - 1) / p.num_splits, A_MIN_STEPS * parts);
+        int part_steps = max((sum - 1) / max(a.split_goal - some / 2, 1) + 1, least);
+        if (some > 1) {
+            int n = parts_of(st0, part_steps);
+            for (int i = lane + 64; i < p.b; i += 64) n += parts_of(steps_of(i), part_steps);
+            if (wave_sum(n) > a.split_goal)
+                part_steps = a.split_goal > some ? max((sum - 1) / (a.split_goal - some) + 1, least) : max(top, 1);
+        }
+        // the sequence in whose run of parts L falls
+        int before = 0;
+        bidb = -1;
+        for (int i = lane; i - lane < p.b && bidb < 0; i += 64) {
+            const int mine = parts_of(i == lane ? st0 : steps_of(i), part_steps);
+            int upto = mine;
+#pragma unroll
+            for (int off = 1; off < 64; off <<= 1) {
+                const int y = __shfl_up(upto, off);
+                if (lane >= off) upto += y;
+            }
+            const uint64_t hit = __ballot(before + upto > L);
+            if (hit) {
+                const int at = __builtin_ctzll(hit);
+                bidb = i - lane + at;
+                nsplit = __builtin_amdgcn_readlane(mine, at);
+                split = L - before - (__builtin_amdgcn_readlane(upto, at) - nsplit);
+            }
+            before += __builtin_amdgcn_readlane(upto, 63);
+        }
+        if (bidb < 0) return;                          // fewer parts than workgroups
+        if (tid == 0 && split == 0 && hblock == 0) a.n_split[bidb * n_mblocks + m_block] = nsplit;
+    }
+    bidb = __builtin_amdgcn_readfirstlane(bidb);
+    split = __builtin_amdgcn_readfirstlane(split);
+    nsplit = __builtin_amdgcn_readfirstlane(nsplit);
+    const bool is_split = nsplit > 1;
 
     const BlockInfo bi(p, bidb);
     const int sq = bi.sq;
     const int sk = min(kv8_cached(a, bidb) + (p.knew ? p.seqlen_knew : 0), a.cap);
     const int rows = sq * ratio;
-    const int q0 = m_block * 16 * NR;
-    if (q0 >= rows) return;
+    if (q0 >= rows || (a.max_rows > 0 && rows > a.max_rows)) return;
     const int pos_lo = q0 / ratio, pos_hi = min(rows - 1, q0 + 16 * NR - 1) / ratio;
 
-    // keys that some row of the block sees, then this split's share of their steps
+    // keys that some row of the block sees, and this part of them
     const bool edge_r = p.is_causal || p.is_local;
     const int vis_lo = p.is_local ? max(0, pos_lo + sk - sq - p.wl) : 0;
     const int vis_hi = edge_r ? min(sk, pos_hi + 1 + sk - sq + p.wr) : sk;
     int n0 = vis_lo / A_STEP, n1 = vis_hi > vis_lo ? (vis_hi + A_STEP - 1) / A_STEP : n0;
     if (is_split) {
-        const int per = (n1 - n0 + p.num_splits - 1) / p.num_splits;
+        const int per = (n1 - n0 + nsplit - 1) / nsplit;
         n0 += split * per;
         n1 = min(n1, n0 + per);
     }
@@ -121,7 +198,7 @@ fwd_kv8_kernel(const KV8Params a, const int n_mblocks) {
     // row i of KV head `head`: query position i / ratio, query head head * ratio + i % ratio
     auto stat_at = [&](int head, int i) -> int64_t {
         const int64_t bh = (int64_t)bidb * p.h + head * ratio + i % ratio;
-        return ((is_split ? (int64_t)split * p.b * p.h : 0) + bh) * p.seqlen_q + i / ratio;
+        return is_split ? ((int64_t)split * p.b * p.h + bh) * a.acc_sq + i / ratio : bh * p.seqlen_q + i / ratio;
     };
     float *lse = is_split ? p.lseaccum : p.lse;
 
@@ -160,59 +237,73 @@ fwd_kv8_kernel(const KV8Params a, const int n_mblocks) {
         }
     }
 
-    const unsigned char *kbase = (const unsigned char *)p.k + (int64_t)hk * p.k_hs;
-    const unsigned char *vbase = (const unsigned char *)p.v + (int64_t)hk * p.v_hs;
-    const unsigned char *ksb = a.ks + (int64_t)hk * a.ks_hs, *vsb = a.vs + (int64_t)hk * a.vs_hs;
-    const int k_rs = (int)p.k_rs, v_rs = (int)p.v_rs, ks_rs = (int)a.ks_rs, vs_rs = (int)a.vs_rs;
-
+    const int k_rs = (int)p.k_rs, v_rs = (int)p.v_rs;
     // lane offsets inside a tile of 16 keys: K 16 columns of key c, V chunk lane + 64 i
-    int64_t koff[NJ], voff[NV / 2];
+    unsigned koff[NJ], voff[NV / 2];
 #pragma unroll
-    for (int j = 0; j < NJ; j++) koff[j] = (int64_t)c * k_rs + (64 * j + 16 * g < p.d ? 64 * j + 16 * g : 0);
+    for (int j = 0; j < NJ; j++) koff[j] = (unsigned)(c * k_rs + (64 * j + 16 * g < p.d ? 64 * j + 16 * g : 0));
 #pragma unroll
     for (int i = 0; i < NV / 2; i++) {
         const int ci = lane + 64 * i, vc = ci % CPR * 16;
-        voff[i] = (int64_t)(ci / CPR) * v_rs + (vc < p.d ? vc : 0);
+        voff[i] = (unsigned)(ci / CPR * v_rs + (vc < p.d ? vc : 0));
     }
+
+    // A step needs eight addresses: of K, V and their scales, for its two tiles.  Lane i of every eight works out
+    // address i (tile i & 1 of K, V, K scale, V scale); the rows' are then read into scalar registers and the
+    // scales fetched by the lanes that hold theirs.  (As scalar arithmetic this was a third of the step's
+    // instructions, and few-wave launches are bound by those.)
+    const int sel = (lane >> 1) & 3, tl = lane & 1;
+    const unsigned char *lbase = sel == 0 ? (const unsigned char *)p.k + (int64_t)hk * p.k_hs
+                               : sel == 1 ? (const unsigned char *)p.v + (int64_t)hk * p.v_hs
+                               : sel == 2 ? a.ks + (int64_t)hk * a.ks_hs : a.vs + (int64_t)hk * a.vs_hs;
+    const int64_t lps = sel == 0 ? p.k_bs : sel == 1 ? p.v_bs : sel == 2 ? a.ks_bs : a.vs_bs;
+    const unsigned lrs = (unsigned)(sel == 0 ? p.k_rs : sel == 1 ? p.v_rs : sel == 2 ? a.ks_rs : a.vs_rs);
 
     struct Set {                 // one step's loads
         i32x4 k[2][NJ], v[NV];
-        unsigned ks[2], vs[2];
+        unsigned sc, bad;        // lanes 4..7 (mod 8): K scales of the two tiles, V scales; 255 for a page outside the pool
     };
     Set set[NBUF];
     const int last_tile = (sk - 1) & ~15;
-    int pid[2];
-    // Page ids of a step's two tiles.  A tile of 16 keys lies in one page and in one block of the scales (both
+    // Page id of the lane's tile.  A tile of 16 keys lies in one page and in one block of the scales (both
     // are multiples of 16 rows); one that starts past the sequence's end takes its last tile (masked keys).
     const int *table = PAGED ? p.block_table + (int64_t)bidb * p.bt_bs : nullptr;
-    if constexpr (!PAGED) pid[0] = pid[1] = p.cache_batch_idx ? p.cache_batch_idx[bidb] : bidb;
+    int pid = PAGED ? 0 : p.cache_batch_idx ? p.cache_batch_idx[bidb] : bidb;
     auto load_pages = [&](int n) __attribute__((always_inline)) {
-        if constexpr (PAGED) {
-#pragma unroll
-            for (int t = 0; t < 2; t++)
-                pid[t] = table[kv8_div(min(n * A_STEP + 16 * t, last_tile) >> 4, a.page_mul, a.page_sh)];
-        }
+        if constexpr (PAGED) pid = table[kv8_div(min(n * A_STEP + 16 * tl, last_tile) >> 4, a.page_mul, a.page_sh)];
     };
-    auto load_step = [&](int n, Set &w) __attribute__((always_inline)) {
-        const unsigned char *vt[2];
+    // (the ids of the step after `n`, in `after`, are requested in front of n's rows: loads return in order, so
+    // what waits for those ids later does not wait for the rows)
+    auto load_step = [&](int n, Set &w, int after) __attribute__((always_inline)) {
+        const int key = min(n * A_STEP + 16 * tl, last_tile);
+        const bool bad = (unsigned)pid >= (unsigned)a.num_pages;   // outside the pool: NaN, from the scale
+        const unsigned pg = bad ? 0u : (unsigned)pid;
+        const int row = PAGED ? key - kv8_div(key >> 4, a.page_mul, a.page_sh) * a.page_rows : key;
+        const unsigned idx = (unsigned)(sel < 2 ? row : kv8_div(row >> 4, a.blk_mul, a.blk_sh));
+        const unsigned char *at = lbase + (int64_t)pg * lps + (uint64_t)idx * lrs;
+        load_pages(after);
+        w.sc = *at;
+        w.bad = bad ? 255u : 0u;
+        const unsigned alo = (unsigned)(uintptr_t)at, ahi = (unsigned)((uintptr_t)at >> 32);
+        auto rows_at = [&](int i) __attribute__((always_inline)) {   // address i of the eight, as a buffer's base
+            const uint64_t base = (uint64_t)(unsigned)__builtin_amdgcn_readlane((int)alo, i) |
+                                  (uint64_t)(unsigned)__builtin_amdgcn_readlane((int)ahi, i) << 32;
+            return __builtin_amdgcn_make_buffer_rsrc((void *)base, 0, 0xffffffffu, 0x00020000);
+        };
 #pragma unroll
         for (int t = 0; t < 2; t++) {
-            const int key = min(n * A_STEP + 16 * t, last_tile);
-            const int page = __builtin_amdgcn_readfirstlane(pid[t]);
-            const bool bad = (unsigned)page >= (unsigned)a.num_pages;   // outside the pool: NaN, from the scale
-            const int64_t pg = bad ? 0 : page;
-            const int row = PAGED ? key - kv8_div(key >> 4, a.page_mul, a.page_sh) * a.page_rows : key;
-            const int blk = kv8_div(row >> 4, a.blk_mul, a.blk_sh);
-            const unsigned char *kt = kbase + pg * p.k_bs + (int64_t)row * k_rs;
+            const auto kr = rows_at(t);
 #pragma unroll
-            for (int j = 0; j < NJ; j++) w.k[t][j] = *(const i32x4 *)(kt + koff[j]);
-            const unsigned kb = ksb[pg * a.ks_bs + (int64_t)blk * ks_rs], vb = vsb[pg * a.vs_bs + (int64_t)blk * vs_rs];
-            w.ks[t] = bad ? 255u : kb;
-            w.vs[t] = bad ? 255u : vb;
-            vt[t] = vbase + pg * p.v_bs + (int64_t)row * v_rs;
+            for (int j = 0; j < NJ; j++) w.k[t][j] = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(kr, koff[j], 0, NT ? 2 : 0));
         }
 #pragma unroll
-        for (int i = 0; i < NV; i++) w.v[i] = *(const i32x4 *)(vt[i / (NV / 2)] + voff[i % (NV / 2)]);
+        for (int t = 0; t < 2; t++) {
+            const auto vr = rows_at(2 + t);
+#pragma unroll
+            for (int i = 0; i < NV / 2; i++)
+                w.v[t * (NV / 2) + i] = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(vr, voff[i], 0, NT ? 2 : 0));
+        }
+        __builtin_amdgcn_sched_barrier(0);   // (steps' loads stay in order: the waits count them)
     };
 
     f32x4 o[NR][NDB];
@@ -241,7 +332,11 @@ fwd_kv8_kernel(const KV8Params a, const int n_mblocks) {
 
     auto step = [&](const int n, Set &w, const int next) __attribute__((always_inline)) {
         const int k0 = n * A_STEP;
-        const float ks[2] = {e8m0_to_f32(w.ks[0]), e8m0_to_f32(w.ks[1])}, vs[2] = {e8m0_to_f32(w.vs[0]), e8m0_to_f32(w.vs[1])};
+        float sc[4];
+        const int scl = (int)(w.sc | w.bad);
+#pragma unroll
+        for (int i = 0; i < 4; i++) sc[i] = e8m0_to_f32((unsigned)__builtin_amdgcn_readlane(scl, 4 + i));
+        const float *ks = sc, *vs = sc + 2;
         f32x4 s[NR][2];
 #pragma unroll
         for (int t = 0; t < 2; t++) {
@@ -270,8 +365,7 @@ fwd_kv8_kernel(const KV8Params a, const int n_mblocks) {
             const int at = i < NV / 2 ? vwr[i] : (vwr[i - NV / 2] ^ SWZ16) + 16 * DP;
             *(i32x4 *)(vimg + at) = w.v[i];
         }
-        load_step(min(next, n1 - 1), w);
-        load_pages(min(next + parts, n1 - 1));
+        load_step(min(next, n1 - 1), w, min(next + parts, n1 - 1));
 
         bool need = k0 + A_STEP > sk;
         if (edge_r) need = need || (k0 + A_STEP > pos_lo + 1 + sk - sq + p.wr);
@@ -349,17 +443,18 @@ fwd_kv8_kernel(const KV8Params a, const int n_mblocks) {
     if (first < n1) {
         load_pages(first);
 #pragma unroll
-        for (int i = 0; i < NBUF; i++) {
-            load_step(min(first + i * parts, n1 - 1), set[i]);
-            load_pages(min(first + (i + 1) * parts, n1 - 1));
-        }
-        for (int n = first;;) {
-            step(n, set[0], n + NBUF * parts);
-            if ((n += parts) >= n1) break;
-            if constexpr (NBUF == 2) {
-                step(n, set[1], n + NBUF * parts);
-                if ((n += parts) >= n1) break;
+        for (int i = 0; i < NBUF; i++) load_step(min(first + i * parts, n1 - 1), set[i], min(first + (i + 1) * parts, n1 - 1));
+        // (one way out of the loop: with another in the middle the compiler's wait counts take the path
+        // around it for one that leads back, and every step waits for the loads of the next)
+        int n = first;
+        if constexpr (NBUF == 2) {
+            for (; n + parts < n1; n += 2 * parts) {
+                step(n, set[0], n + 2 * parts);
+                step(n + parts, set[1], n + 3 * parts);
             }
+            if (n < n1) step(n, set[0], n1);
+        } else {
+            for (; n < n1; n += parts) step(n, set[0], n + parts);
         }
     }
 
@@ -416,47 +511,129 @@ fwd_kv8_kernel(const KV8Params a, const int n_mblocks) {
     }
 }
 
-template <int DP, bool BF16, int NR, bool PAGED>
+// Merge of the parts of a row: LSE-weighted sum, in part order.  One workgroup per (sequence, head, query
+// position): 256 threads are (16-byte output chunk) x (lane over the parts); everything is requested up front.
+template <bool BF16>
+__global__ void __launch_bounds__(256)
+kv8_combine_kernel(const KV8Params a, const int n_mblocks, const int rows_per_block) {
+    const KParams &p = a.p;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int pos = blockIdx.x % a.acc_sq, bh = blockIdx.x / a.acc_sq, bidb = bh / p.h, head = bh % p.h;
+    const BlockInfo bi(p, bidb);
+    if (pos >= bi.sq || (a.max_rows > 0 && bi.sq * p.h_ratio > a.max_rows)) return;
+    const int ns = a.n_split[bidb * n_mblocks + (pos * p.h_ratio + head % p.h_ratio) / rows_per_block];
+    if (ns <= 1) return;                       // one part: written in place
+    __shared__ float s_w[128], s_red[2][2], s_part[256 * 8];
+    const int cpr = p.d / 8, nlane = 256 / cpr, ch = tid % cpr, sl = tid / cpr;
+    const int64_t rows = (int64_t)p.b * p.h * a.acc_sq, row = (int64_t)bh * a.acc_sq + pos;
+    const float my = tid < ns ? p.lseaccum[tid * rows + row] : -INFINITY;
+    constexpr int PRE = 4;
+    f32x4 r0[PRE], r1[PRE];
+#pragma unroll
+    for (int i = 0; i < PRE; i++) {
+        const float *src = p.oaccum + (min(sl + i * nlane, ns - 1) * rows + row) * p.d + ch * 8;   // (clamped: weight 0 below)
+        r0[i] = *(const f32x4 *)src;
+        r1[i] = *(const f32x4 *)(src + 4);
+    }
+    float m = my;
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor(m, off));
+    if (wave < 2 && lane == 0) s_red[0][wave] = m;           // (at most 128 parts: waves 0 and 1)
+    __syncthreads();
+    m = fmaxf(s_red[0][0], s_red[0][1]);
+    const float ref = m == -INFINITY ? 0.f : m;
+    float e = tid < ns ? expf(my - ref) : 0.f;
+    float sum = e;
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) sum += __shfl_xor(sum, off);
+    if (wave < 2 && lane == 0) s_red[1][wave] = sum;
+    __syncthreads();
+    sum = s_red[1][0] + s_red[1][1];
+    const bool none = sum == 0.f;                             // no part saw a key of this row
+    if (tid < 128) s_w[tid] = none ? 0.f : e / sum;
+    if (tid == 0) p.lse[(int64_t)bh * p.seqlen_q + pos] = none ? INFINITY : logf(sum) + ref;
+    __syncthreads();
+    f32x4 a0 = {0, 0, 0, 0}, a1 = {0, 0, 0, 0};
+    if (sl < nlane) {
+#pragma unroll
+        for (int i = 0; i < PRE; i++) {
+            const int sp = sl + i * nlane;
+            if (sp < ns) { a0 += r0[i] * s_w[sp]; a1 += r1[i] * s_w[sp]; }
+        }
+        for (int sp = sl + PRE * nlane; sp < ns; sp += nlane) {
+            const float *src = p.oaccum + (sp * rows + row) * p.d + ch * 8;
+            a0 += *(const f32x4 *)src * s_w[sp];
+            a1 += *(const f32x4 *)(src + 4) * s_w[sp];
+        }
+    }
+    *(f32x4 *)(s_part + tid * 8) = a0;
+    *(f32x4 *)(s_part + tid * 8 + 4) = a1;
+    __syncthreads();
+    if (tid < cpr) {
+        for (int l = 1; l < min(nlane, ns); l++) {
+            a0 += *(const f32x4 *)(s_part + (l * cpr + tid) * 8);
+            a1 += *(const f32x4 *)(s_part + (l * cpr + tid) * 8 + 4);
+        }
+        unsigned short *og = (unsigned short *)p.o + bi.q_off(p.o_bs, p.o_rs, bidb) + (int64_t)head * p.o_hs + (int64_t)pos * p.o_rs + tid * 8;
+        i32x4 w;
+        w[0] = pack2<BF16>(a0[0], a0[1]); w[1] = pack2<BF16>(a0[2], a0[3]);
+        w[2] = pack2<BF16>(a1[0], a1[1]); w[3] = pack2<BF16>(a1[2], a1[3]);
+        *(i32x4 *)og = w;
+    }
+}
+
+// Rows of a decode workgroup (above head dim 128 the accumulators of 32 rows do not fit beside the loads) and
+// row blocks of the launch.
+int kv8_decode_rows(int d, int rows) { return d <= 128 && rows > 16 ? 32 : 16; }
+
+// Resident workgroups of 8 waves per CU: two where the kernel needs at most 128 registers, else one.
+int kv8_decode_wgs_per_cu(int d, int rows) { return d <= 64 && rows <= 16 ? 2 : 1; }
+
+template <int DP, bool BF16, int NR, bool PAGED, bool NT>
 static hipError_t launch_kv8(const KV8Params &a, hipStream_t stream) {
     const KParams &p = a.p;
-    const int n_mblocks = (p.seqlen_q * p.h_ratio + 16 * NR - 1) / (16 * NR);
-    const long long blocks = (long long)n_mblocks * p.b * (p.h_k / a.heads_per_wg) * p.num_splits;
+    const int n_mblocks = (a.acc_sq * p.h_ratio + 16 * NR - 1) / (16 * NR);
+    const long long blocks = (long long)n_mblocks * (p.h_k / a.heads_per_wg) * (p.num_splits > 1 ? a.split_grid : p.b);
     if (blocks <= 0) return hipSuccess;
     if (blocks > 0x7fffffffLL) return hipErrorInvalidValue;
-    auto kern = fwd_kv8_kernel<DP, BF16, NR, PAGED>;
+    auto kern = fwd_kv8_kernel<DP, BF16, NR, PAGED, NT>;
     constexpr int lds = Kv8Cfg<DP, NR>::LDS_BYTES;
     static std::atomic<uint64_t> lds_set{0};
     if (hipError_t e = set_dyn_lds_once((const void *)kern, lds, lds_set); e != hipSuccess) return e;
     hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3(A_NT), lds, stream, a, n_mblocks);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess || p.num_splits <= 1) return e;
+    const long long rows = (long long)p.b * p.h * a.acc_sq;
+    hipLaunchKernelGGL(kv8_combine_kernel<BF16>, dim3((unsigned)rows), dim3(256), 0, stream, a, n_mblocks, 16 * NR);
     return hipGetLastError();
 }
 
 template <int DP, bool BF16, int NR>
 static hipError_t launch_kv8_layout(const KV8Params &a, hipStream_t stream) {
-    return a.p.block_table ? launch_kv8<DP, BF16, NR, true>(a, stream) : launch_kv8<DP, BF16, NR, false>(a, stream);
+    const bool paged = a.p.block_table != nullptr;
+    if constexpr (DP == 128) {
+        // codes that the calls of a program can name at all: what the sequences may hold, or the pool
+        const long long codes = std::min((long long)a.p.b * a.cap, (long long)a.num_pages * a.page_rows) * a.p.h_k * a.p.d * 2;
+        if (codes > 512LL << 20) return paged ? launch_kv8<DP, BF16, NR, true, true>(a, stream) : launch_kv8<DP, BF16, NR, false, true>(a, stream);
+    }
+    return paged ? launch_kv8<DP, BF16, NR, true, false>(a, stream) : launch_kv8<DP, BF16, NR, false, false>(a, stream);
 }
 template <int DP, bool BF16>
 static hipError_t launch_kv8_rows(const KV8Params &a, hipStream_t stream) {
-    if constexpr (DP <= 128)     // (above, the accumulators of 32 rows do not fit beside the loads)
-        if (a.p.seqlen_q * a.p.h_ratio > 16) return launch_kv8_layout<DP, BF16, 2>(a, stream);
+    if constexpr (DP <= 128)
+        if (kv8_decode_rows(a.p.d, a.acc_sq * a.p.h_ratio) == 32) return launch_kv8_layout<DP, BF16, 2>(a, stream);
     return launch_kv8_layout<DP, BF16, 1>(a, stream);
 }
 
 // Adjacent KV heads of a workgroup: a key's codes of one head are d bytes, and reads of 512 contiguous bytes
-// are what keeps HBM busy.
+// are what keeps HBM busy (b128 kv8192 h32/8 d128, heads 1 / 2 / 4: 465 / 391 / 374 us).
 int kv8_heads_per_wg(int d, int h_k) {
     int n = 1;
     while (n < 8 && n * d < 512 && h_k % (2 * n) == 0) n *= 2;
     return n;
 }
 
-hipError_t run_fwd_kv8_prefill(const KV8Params &a, hipStream_t stream);   // fwd_prefill_kv8.hip
-
-// Whether a call's rows take the prefill kernel's 128-row blocks: from there on the products bound it.
-bool kv8_takes_prefill(int d, int h_ratio, int seqlen_q) { return (long long)seqlen_q * h_ratio > 32; }
-
 hipError_t run_fwd_kv8(const KV8Params &a, hipStream_t stream) {
-    if (kv8_takes_prefill(a.p.d, a.p.h_ratio, a.p.seqlen_q)) return run_fwd_kv8_prefill(a, stream);
     const bool bf = a.p.is_bf16;
     if (a.p.d <= 64) return bf ? launch_kv8_rows<64, true>(a, stream) : launch_kv8_rows<64, false>(a, stream);
     if (a.p.d <= 128) return bf ? launch_kv8_rows<128, true>(a, stream) : launch_kv8_rows<128, false>(a, stream);

@@ -181,6 +181,7 @@ fwd_prefill_kernel(const std::conditional_t<LD == 5, KV8Params, KParams> args, c
     if constexpr (KV8) sk_ = min(kv8_cached(args, bidb) + (p.knew ? p.seqlen_knew : 0), args.cap);
     const int sq = bi.sq, sk = sk_;
     const int sq_rows = sq * ratio;    // rows of this (batch, head): query positions (x grouped heads)
+    if constexpr (KV8) if (sq_rows <= args.min_rows) return;   // the decode kernel's
     // Philox state: the caller's values, or (under graph capture) read on the device at replay
     // time from the generator's captured state (at::cuda::philox::unpack, flash_fwd_kernel.h:45)
     unsigned long long ph_seed = p.philox_seed, ph_offset = p.philox_offset;
@@ -284,8 +285,16 @@ fwd_prefill_kernel(const std::conditional_t<LD == 5, KV8Params, KParams> args, c
     constexpr int NP = KV8 ? CH / 2 : 1, PPR = DP / 16;
     static_assert(!KV8 || (CH % 2 == 0 && 64 / PPR <= 16), "pieces of a wave lie in one group of 16 rows");
     i32x4 kc8[NP], vc8[NP];
-    unsigned ks8[NP], vs8[NP];
+    unsigned ks8[NP], vs8[NP], bad8[NP];
     int pg8[NP];
+    const unsigned char *k_base = (const unsigned char *)p.k + (int64_t)hk * p.k_hs, *v_base = (const unsigned char *)p.v + (int64_t)hk * p.v_hs;
+    const unsigned char *ks_base = nullptr, *vs_base = nullptr;
+    if constexpr (KV8) { ks_base = args.ks + (int64_t)hk * args.ks_hs; vs_base = args.vs + (int64_t)hk * args.vs_hs; }
+    // (a thread's row in its group of 16 and its columns are the same in every piece; columns past the head dim
+    // read column 0: they meet zero columns of Q, or columns of O that are not stored)
+    static_assert(!KV8 || NT / PPR % 16 == 0, "");
+    const int col8 = tid % PPR * 16 < p.d ? tid % PPR * 16 : 0;
+    const unsigned koff8 = (unsigned)(((tid / PPR) & 15) * (int)p.k_rs + col8), voff8 = (unsigned)(((tid / PPR) & 15) * (int)p.v_rs + col8);
     // keys that some row of the block sees: V of the others must not count, whatever stands there
     const int vis_lo = p.is_local ? max(0, pos_lo_b + sk - sq - p.wl) : 0;
     const int vis_hi = (p.is_causal || p.is_local) ? min(sk, pos_hi_b + sk - sq + p.wr) : sk;
@@ -293,8 +302,9 @@ fwd_prefill_kernel(const std::conditional_t<LD == 5, KV8Params, KParams> args, c
         if constexpr (KV8) {
 #pragma unroll
             for (int i = 0; i < NP; i++) {
-                const int g16 = n * BN + (((wave * 64 + i * NT) / PPR) & ~15);   // the wave's group of rows
-                pg8[i] = kv8_page(args, bidb, min(g16, (sk - 1) & ~15));
+                const int g16 = min(n * BN + (((wave * 64 + i * NT) / PPR) & ~15), (sk - 1) & ~15);   // the wave's group of rows
+                if (bt) pg8[i] = bt[kv8_div(g16 >> 4, args.page_mul, args.page_sh)];
+                else pg8[i] = bidb_cache;
             }
         }
     };
@@ -302,28 +312,33 @@ fwd_prefill_kernel(const std::conditional_t<LD == 5, KV8Params, KParams> args, c
         if constexpr (KV8) {
 #pragma unroll
             for (int i = 0; i < NP; i++) {
-                const int tr = (tid + i * NT) / PPR, col = (tid + i * NT) % PPR * 16;
                 const int g16 = min(n * BN + (((wave * 64 + i * NT) / PPR) & ~15), (sk - 1) & ~15);
                 const int page = __builtin_amdgcn_readfirstlane(pg8[i]);
-                const int row = kv8_row_in_page(args, g16), blk = kv8_div(row >> 4, args.blk_mul, args.blk_sh);
-                const int64_t pg = max(page, 0);
-                ks8[i] = page < 0 ? 255u : args.ks[pg * args.ks_bs + blk * args.ks_rs + hk * args.ks_hs];
-                vs8[i] = page < 0 ? 255u : args.vs[pg * args.vs_bs + blk * args.vs_rs + hk * args.vs_hs];
-                const unsigned char *kp = (const unsigned char *)p.k + hk * p.k_hs + pg * p.k_bs + (int64_t)(row + (tr & 15)) * p.k_rs + col;
-                const unsigned char *vp = (const unsigned char *)p.v + hk * p.v_hs + pg * p.v_bs + (int64_t)(row + (tr & 15)) * p.v_rs + col;
-                const bool ok = col < p.d, seen = n * BN + tr >= vis_lo && n * BN + tr < vis_hi;
-                kc8[i] = ok ? *(const i32x4 *)kp : i32x4{0, 0, 0, 0};
-                vc8[i] = ok && seen ? *(const i32x4 *)vp : i32x4{0, 0, 0, 0};
+                const bool bad = (unsigned)page >= (unsigned)args.num_pages;   // outside the pool: NaN, from the scale
+                const int row = bt ? g16 - kv8_div(g16 >> 4, args.page_mul, args.page_sh) * args.page_rows : g16;
+                const int64_t pg = bad ? 0 : page, blk = kv8_div(row >> 4, args.blk_mul, args.blk_sh);
+                bad8[i] = bad ? 255u : 0u;
+                ks8[i] = ks_base[pg * args.ks_bs + blk * args.ks_rs];
+                vs8[i] = vs_base[pg * args.vs_bs + blk * args.vs_rs];
+                kc8[i] = *(const i32x4 *)(k_base + pg * p.k_bs + (int64_t)row * p.k_rs + koff8);
+                vc8[i] = *(const i32x4 *)(v_base + pg * p.v_bs + (int64_t)row * p.v_rs + voff8);
             }
         }
     };
-    auto store_tile8 = [&](auto BUFC) __attribute__((always_inline)) {
+    auto store_tile8 = [&](int n, auto BUFC) __attribute__((always_inline)) {
         constexpr int BUF = decltype(BUFC)::value;
         if constexpr (KV8) {
+            if (n * BN < vis_lo || (n + 1) * BN > vis_hi) {
+#pragma unroll
+                for (int i = 0; i < NP; i++) {
+                    const int key = n * BN + (tid + i * NT) / PPR;
+                    if (key < vis_lo || key >= vis_hi) vc8[i] = i32x4{0, 0, 0, 0};
+                }
+            }
 #pragma unroll
             for (int i = 0; i < NP; i++) {
                 const int tr = (tid + i * NT) / PPR, ch = (tid + i * NT) % PPR * 2;
-                const float ks = e8m0_to_f32(ks8[i]), vs = e8m0_to_f32(vs8[i]);
+                const float ks = e8m0_to_f32(ks8[i] | bad8[i]), vs = e8m0_to_f32(vs8[i] | bad8[i]);
                 char *kd = smem + BUF * Cfg::TILE_BYTES, *vd = smem + (2 + BUF) * Cfg::TILE_BYTES;
 #pragma unroll
                 for (int e = 0; e < 2; e++) {
@@ -631,7 +646,7 @@ fwd_prefill_kernel(const std::conditional_t<LD == 5, KV8Params, KParams> args, c
         load_pages8(n_max - 1);
         load_tile8(n_max - 1);
         if (n_max - 2 >= n_min) load_pages8(n_max - 2);
-        store_tile8(std::integral_constant<int, 0>{});
+        store_tile8(n_max - 1, std::integral_constant<int, 0>{});
     } else {
         load_pages(n_max - 1);
         load_tile(n_max - 1);
@@ -879,7 +894,7 @@ fwd_prefill_kernel(const std::conditional_t<LD == 5, KV8Params, KParams> args, c
         }  // !skip
 
         if constexpr (TO_LDS) __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0) before the barrier
-        else if constexpr (KV8) { if (has_next) store_tile8(std::integral_constant<int, BUF ^ 1>{}); }
+        else if constexpr (KV8) { if (has_next) store_tile8(n - 1, std::integral_constant<int, BUF ^ 1>{}); }
         else if (has_next) store_tile(std::integral_constant<int, BUF ^ 1>{});
         STAMP(4);
         __syncthreads();

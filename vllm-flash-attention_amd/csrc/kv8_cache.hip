@@ -187,6 +187,16 @@ kv8_dequantize_kernel(const KV8Params a, const int tpw, const int cph) {
     const KParams &p = a.p;
     const int tid = threadIdx.x;
     const int64_t first = (int64_t)blockIdx.x * tpw;
+    // Read back for the 16-bit attention kernels: sequences that are the decode kernel's have length 0 there, and
+    // rows behind a sequence are not read, so not written.
+    auto length = [&](int i) -> int {
+        const int n = min(kv8_cached(a, i) + (p.knew ? p.seqlen_knew : 0), a.cap);
+        if (!a.lens_out) return n;
+        const int sq = p.cu_seqlens_q ? p.cu_seqlens_q[i + 1] - p.cu_seqlens_q[i] : p.seqlen_q;
+        return sq * p.h_ratio <= a.min_rows ? 0 : n;
+    };
+    if (a.lens_out && blockIdx.x == 0)
+        for (int i = tid; i < p.b; i += D_NT) a.lens_out[i] = length(i);
     if (tid < tpw && first + tid < a.rows_out) {
         const int64_t t = first + tid;
         int seq;
@@ -207,8 +217,8 @@ kv8_dequantize_kernel(const KV8Params a, const int tpw, const int cph) {
             tok = t - (int64_t)seq * a.seqlen_out;
             r.out_k = seq * a.ko_bs + tok * a.ko_rs; r.out_v = seq * a.vo_bs + tok * a.vo_rs;
         }
-        r.k = -1; r.v = r.ks = r.vs = 0;
-        if (tok >= 0 && tok < kv8_cached(a, seq)) {
+        r.k = a.lens_out ? -3 : -1; r.v = r.ks = r.vs = 0;
+        if (tok >= 0 && tok < length(seq)) {
             const int page = kv8_page(a, seq, (int)tok);
             if (page >= 0) {
                 const int row = kv8_row_in_page(a, (int)tok), blk = kv8_div(row >> 4, a.blk_mul, a.blk_sh);
@@ -227,6 +237,7 @@ kv8_dequantize_kernel(const KV8Params a, const int tpw, const int cph) {
         const int t = i / per, c = i - t * per;
         const int head = c / cph, col = (c - head * cph) * 16;
         const RowOf &r = s_row[t];
+        if (r.k == -3) continue;
         i32x4 k = {0, 0, 0, 0}, v = k;
         float ks = 1.f, vs = 1.f;
         if (r.k >= 0) {

@@ -1071,9 +1071,14 @@ std::vector<Tensor> fwd_kv8(const Tensor &q_, const Tensor &kc, const Tensor &vc
     P.a.window_size_right = (int)std::clamp<int64_t>(window_size_right, -1, 1 << 30);
     if (alibi_slopes.has_value()) expect_with(alibi_slopes.value(), "alibi_slopes", kc);
     set_alibi(P.a, alibi_slopes, b, h);
-    SplitScratch scratch;
-    if (num_splits < 1) num_splits = vfa_kv8_num_splits((int)b, (int)h, (int)hk, (int)d, P.a.seqlen_k, (int)sq, cu_count());
-    plan_splits(P.a, scratch, (int)std::min<int64_t>(num_splits, 1 << 20), b, h, d, P.a.seqlen_k, sq, opts);
+    TORCH_CHECK(num_splits <= 128, "num_splits > 128 not supported");
+    P.a.num_splits = (int)std::max<int64_t>(num_splits, 0);
+    Tensor work;
+    P.workspace_bytes = vfa_kv8_workspace(&P);
+    if (P.workspace_bytes > 0) {
+        work = torch::empty({(int64_t)P.workspace_bytes}, opts.dtype(at::kByte));
+        P.workspace = work.data_ptr();
+    }
     P.a.stream = current_stream();
     run(vfa_kv8_mha_fwd(&P));
     if (out_.has_value() && out.data_ptr() != out_.value().data_ptr()) {

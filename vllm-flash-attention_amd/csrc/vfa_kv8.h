@@ -24,7 +24,14 @@ struct KV8Params {
     int num_pages;               // pages; batch rows of a contiguous cache
     int cap;                     // most tokens a sequence can have
     int heads_per_wg;            // attention: adjacent KV heads per workgroup (1, 2, 4, 8)
-    unsigned page_mul, blk_mul;  // n / (page_rows / 16) = n * page_mul >> page_sh for n < 2^27 (and so for blk)
+    int max_rows;                // decode kernel: sequences with more (query, head) rows than this are another kernel's; 0: none are
+    int min_rows;                // prefill kernel, reading back for it: the sequences with at most so many rows are the decode kernel's
+    int split_goal;              // decode kernel: parts of the keys to aim at per head group and row block, over all sequences
+    int split_grid;              // and the most there can be
+    int acc_sq;                  // query positions of a sequence in the partial results
+    int *n_split;                // (b, row blocks): parts that a sequence's keys were cut into
+    int *lens_out;               // reading back: the lengths, or null
+    unsigned page_mul, blk_mul;  // exact division by page_rows / 16 and blk / 16 (kv8_div)
     int page_sh, blk_sh;
     // writing: new tokens are p.knew / p.vnew, dense (b, seqlen_knew) or ragged
     const int *cu_new;
@@ -36,16 +43,15 @@ struct KV8Params {
     int seqlen_out;
 };
 
-// multiplier and shift of the exact division of n < 2^27 by d: M = floor(2^k / d) + 1 with k = 27 + ceil(log2 d)
-// has an error under 2^-27 relative, less than a unit of the quotient's fraction
+// Exact division of n < 2^27 by d < 2^27 in one high product: M = ceil(2^(31 + s) / d), s = floor(log2 d), is off by
+// less than d 2^-(31 + s) of its value's unit, so n M / 2^(31 + s) is over n / d by less than 2^-3 / d.
 inline void kv8_div_magic(int d, unsigned &mul, int &shift) {
-    int l = 0;
-    while ((1 << l) < d) l++;
-    shift = 27 + l;
-    mul = (unsigned)((1ull << shift) / (unsigned)d + 1);
+    shift = 0;
+    while ((2 << shift) <= d) shift++;
+    mul = (unsigned)(((1ull << (31 + shift)) + d - 1) / (unsigned)d);
 }
 __device__ __forceinline__ int kv8_div(int n, unsigned mul, int shift) {
-    return (int)(((unsigned long long)(unsigned)n * mul) >> shift);
+    return (int)(__umulhi((unsigned)n << 1, mul) >> shift);
 }
 
 // tokens in the cache of sequence bidb before the call
