@@ -281,8 +281,8 @@ size_t vfa_kv8_workspace(const vfa_kv8_params *p);
 /* RMS norm of every head of q (b, s, h, d) and k (b, s, h_k, d), times a weight (d), then the position rotation of its first
  * rotary_dim columns (pairs (2i, 2i + 1) if interleaved, else (i, i + rotary_dim / 2)):
  *   y = R(position) (x / sqrt(mean(x^2) + eps) * w).
- * Ragged batches are b = 1.  Strides in elements, multiples of 8; base pointers 16-byte aligned; last dim
- * contiguous.  positions (b, s) int32, NULL = the index in s; a negative position marks padding (output and
+ * Ragged batches are b = 1.  Strides in elements, multiples of 8; base pointers (weights' and tables' too)
+ * 16-byte aligned; last dim contiguous.  positions (b, s) int32, NULL = the index in s; a negative position marks padding (output and
  * gradients zero); one past the tables gives NaN.  The backward reads q / k again, needs nothing else from
  * the forward, and gives the same bits on every run. */
 typedef struct vfa_qk_norm_rotary_params {

@@ -36,7 +36,7 @@ int kv8_decode_rows(int d, int rows);
 int kv8_decode_wgs_per_cu(int d, int rows);
 hipError_t run_fwd_kv8_prefill(const KV8Params &a, hipStream_t stream);          // fwd_prefill_kv8.hip
 hipError_t run_qk_norm_rotary(const QKNormParams &p, bool bwd, hipStream_t stream);   // qk_norm_rotary.hip
-void qk_norm_bwd_blocks(QKNormParams &p, int cus);
+void qk_norm_blocks(QKNormParams &p, int cus, bool bwd);
 }  // namespace vfa
 
 using vfa::KParams;
@@ -644,8 +644,9 @@ static int kv8_plan(const vfa_kv8_params *p, Kv8Plan &w) {
     std::memset(&w, 0, sizeof(w));
     const int ratio = a.h / a.h_k, cus = num_cus();
     const long long rows = (long long)a.seqlen_q * ratio;
-    w.dec_rows = VFA_KV8_DECODE_ROWS;
-    w.prefill = rows > w.dec_rows;
+    w.prefill = rows > VFA_KV8_DECODE_ROWS;
+    // beside longer ones only sequences of one 16-row block (of one query position, if that is more rows)
+    w.dec_rows = !w.prefill ? VFA_KV8_DECODE_ROWS : ratio <= 16 ? 16 : ratio <= 32 ? 32 : VFA_KV8_DECODE_ROWS;
     // a dense batch is all one kind; of a ragged one with long members only the lengths on the device know
     w.decode = !w.prefill || (a.cu_seqlens_q && ratio <= w.dec_rows);
     w.dec_sq = w.prefill ? std::max(1, w.dec_rows / ratio) : a.seqlen_q;
@@ -831,6 +832,8 @@ static int qk_norm_fill(const vfa_qk_norm_rotary_params *p, vfa::QKNormParams &k
                            p->ko_row_stride, p->ko_head_stride, p->dk_out, p->dko_batch_stride, p->dko_row_stride, p->dko_head_stride,
                            p->dk_weight);
     VFA_CHECK(ok_q && ok_k, "tensors must be 16-byte aligned, strides multiples of 8 elements");
+    VFA_CHECK(aligned16(p->q_weight) && aligned16(p->k_weight) && aligned16(p->rotary_cos) && aligned16(p->rotary_sin),
+              "weights and tables must be 16-byte aligned");
     if (!bwd) VFA_CHECK(!tokens || (p->q_out && p->k_out), "null output pointer");
     else VFA_CHECK(!tokens || (p->dq_out && p->dk_out), "null gradient pointer");
     k.b = p->b; k.s = p->s; k.d = p->d;
@@ -848,6 +851,7 @@ extern "C" int vfa_qk_norm_rotary_fwd(const vfa_qk_norm_rotary_params *p) {
     int rc = qk_norm_fill(p, k, false);
     if (rc) return rc;
     if ((rc = check_arch())) return rc;
+    vfa::qk_norm_blocks(k, num_cus(), false);
     hipError_t e = vfa::run_qk_norm_rotary(k, false, (hipStream_t)p->stream);
     if (e != hipSuccess) return hip_fail(e, "qk_norm_rotary launch");
     return VFA_OK;
@@ -859,7 +863,7 @@ extern "C" size_t vfa_qk_norm_rotary_bwd_workspace(const vfa_qk_norm_rotary_para
     std::memset(&k, 0, sizeof(k));
     k.t[0].h = p->h; k.t[1].h = p->h_k;
     k.b = p->b; k.s = p->s; k.d = p->d;
-    vfa::qk_norm_bwd_blocks(k, num_cus());
+    vfa::qk_norm_blocks(k, num_cus(), true);
     return (size_t)(k.blocks_q + k.blocks_k) * (size_t)p->d;
 }
 
@@ -871,7 +875,7 @@ extern "C" int vfa_qk_norm_rotary_bwd(const vfa_qk_norm_rotary_params *p) {
     VFA_CHECK(!(p->dq_weight || p->dk_weight) || p->workspace, "qk_norm_rotary: the weights' gradients need the workspace");
     if ((rc = check_arch())) return rc;
     k.dw_part = p->workspace;
-    vfa::qk_norm_bwd_blocks(k, num_cus());
+    vfa::qk_norm_blocks(k, num_cus(), true);
     hipError_t e = vfa::run_qk_norm_rotary(k, true, (hipStream_t)p->stream);
     if (e != hipSuccess) return hip_fail(e, "qk_norm_rotary backward launch");
     return VFA_OK;

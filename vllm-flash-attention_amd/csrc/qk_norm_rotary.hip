@@ -32,10 +32,25 @@ __device__ __forceinline__ i32x4 pack8(const float f[8]) {
     for (int i = 0; i < 4; i++) w[i] = pack2<BF16>(f[2 * i], f[2 * i + 1]);
     return w;
 }
-// element i of a table or weight held in fp32 or in the tensors' type
-template <bool BF16>
-__device__ __forceinline__ float ld_f(const void *p, int64_t i, int f32) {
-    return f32 ? ((const float *)p)[i] : to_f32<BF16>(((const unsigned short *)p)[i]);
+// N (4 or 8) consecutive elements of a table or weight held in fp32 or in the tensors' type, from element i
+// on (a multiple of N)
+template <bool BF16, int N>
+__device__ __forceinline__ void ld_f(const void *p, int64_t i, int f32, float out[N]) {
+    if (f32) {
+#pragma unroll
+        for (int j = 0; j < N / 4; j++) {
+            const f32x4 v = *(const f32x4 *)((const float *)p + i + 4 * j);
+#pragma unroll
+            for (int t = 0; t < 4; t++) out[4 * j + t] = v[t];
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < N / 4; j++) {
+            const i32x2 v = *(const i32x2 *)((const unsigned short *)p + i + 4 * j);
+#pragma unroll
+            for (int t = 0; t < 4; t++) out[4 * j + t] = to_f32<BF16>((unsigned short)((unsigned)v[t >> 1] >> (16 * (t & 1))));
+        }
+    }
 }
 template <int LPR>
 __device__ __forceinline__ float row_sum(float x) {
@@ -63,21 +78,17 @@ __device__ __forceinline__ void load_turn(const QKNormParams &p, int pos, int ch
     }
     const int64_t row = (int64_t)pos * half;
     if (p.interleaved) {
-        if (pos < p.table_rows)
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                t.c[i] = ld_f<BF16>(p.cos, row + col / 2 + i, p.table_f32);
-                t.s[i] = ld_f<BF16>(p.sin, row + col / 2 + i, p.table_f32);
-            }
+        if (pos < p.table_rows) {
+            ld_f<BF16, 4>(p.cos, row + col / 2, p.table_f32, t.c);
+            ld_f<BF16, 4>(p.sin, row + col / 2, p.table_f32, t.s);
+        }
     } else {
         const bool left = col < half;
         t.partner = left ? lane + half / 8 : lane - half / 8;
-        if (pos < p.table_rows)
-#pragma unroll
-            for (int i = 0; i < 8; i++) {
-                t.c[i] = ld_f<BF16>(p.cos, row + (left ? col : col - half) + i, p.table_f32);
-                t.s[i] = ld_f<BF16>(p.sin, row + (left ? col : col - half) + i, p.table_f32);
-            }
+        if (pos < p.table_rows) {
+            ld_f<BF16, 8>(p.cos, row + (left ? col : col - half), p.table_f32, t.c);
+            ld_f<BF16, 8>(p.sin, row + (left ? col : col - half), p.table_f32, t.s);
+        }
         if (left)
 #pragma unroll
             for (int i = 0; i < 8; i++) t.s[i] = -t.s[i];   // y = n c + partner s
@@ -122,58 +133,52 @@ __device__ __forceinline__ Item find_item(const QKNormParams &p, int64_t item, i
     return it;
 }
 
+// The first blocks_q workgroups walk q's items, the others k's.
 template <bool BF16, int LPR, int U>
 __global__ void __launch_bounds__(N_NT)
-qk_norm_fwd_kernel(const QKNormParams p, const int64_t items_q, const int64_t items, const int parts_q, const int parts_k) {
+qk_norm_fwd_kernel(const QKNormParams p, const int64_t items_q, const int64_t items_k, const int parts_q, const int parts_k) {
     constexpr int RPW = 64 / LPR;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    int64_t item = (int64_t)blockIdx.x * N_NW + wave;
-    if (item >= items) return;
-    const bool is_k = item >= items_q;
-    const QKNormTensor &t = p.t[is_k];
-    const Item it = find_item(p, is_k ? item - items_q : item, is_k ? parts_k : parts_q, RPW * U);
+    const bool is_k = (int)blockIdx.x >= p.blocks_q;
+    const QKNormTensor t = is_k ? p.t[1] : p.t[0];   // (selected field by field: an index would put both in scratch)
+    const int blk = is_k ? blockIdx.x - p.blocks_q : blockIdx.x, n_blk = is_k ? p.blocks_k : p.blocks_q;
+    const int64_t items = is_k ? items_k : items_q;
+    const int parts = is_k ? parts_k : parts_q;
     const int sub = lane / LPR, ch = lane % LPR, col = ch * 8;
-    const bool col_ok = col < p.d;
-
-    const unsigned short *xp = (const unsigned short *)t.x + it.bi * t.x_bs + it.si * t.x_rs + (col_ok ? col : 0);
-    unsigned short *yp = (unsigned short *)t.y + it.bi * t.y_bs + it.si * t.y_rs + col;
-    i32x4 x[U];
+    const bool col_ok = col < p.d, inside = col < p.rd, pairs = inside && !p.interleaved;
+    float w[8], wo[8];
+    const int pcol = (col < p.rd / 2 ? col + p.rd / 2 : col - p.rd / 2);   // the partner's columns
 #pragma unroll
-    for (int u = 0; u < U; u++) {
-        const int head = it.head0 + u * RPW + sub;
-        x[u] = (col_ok && head < t.h) ? *(const i32x4 *)(xp + head * t.x_hs) : i32x4{0, 0, 0, 0};
-    }
-    if (it.pos < 0) {                          // padding: zeros, whatever stands there
+    for (int i = 0; i < 8; i++) w[i] = wo[i] = 0.f;
+    if (col_ok) ld_f<BF16, 8>(t.w, col, p.w_f32, w);
+    if (pairs) ld_f<BF16, 8>(t.w, pcol, p.w_f32, wo);
+    for (int64_t item = (int64_t)blk * N_NW + wave; item < items; item += (int64_t)n_blk * N_NW) {
+        const Item it = find_item(p, item, parts, RPW * U);
+        const unsigned short *xp = (const unsigned short *)t.x + it.bi * t.x_bs + it.si * t.x_rs + (col_ok ? col : 0);
+        unsigned short *yp = (unsigned short *)t.y + it.bi * t.y_bs + it.si * t.y_rs + col;
+        i32x4 x[U];
 #pragma unroll
         for (int u = 0; u < U; u++) {
             const int head = it.head0 + u * RPW + sub;
-            if (col_ok && head < t.h) *(i32x4 *)(yp + head * t.y_hs) = i32x4{0, 0, 0, 0};
+            x[u] = (col_ok && head < t.h) ? *(const i32x4 *)(xp + head * t.x_hs) : i32x4{0, 0, 0, 0};
         }
-        return;
-    }
-    Turn tr;
-    load_turn<BF16>(p, it.pos, ch, lane, tr);
-    const bool inside = col < p.rd, pairs = inside && !p.interleaved;
-    float w[8], wo[8];
-    const int pcol = (tr.partner % LPR) * 8;
+        const bool pad = it.pos < 0;               // zeros, whatever stands there
+        Turn tr;
+        load_turn<BF16>(p, pad ? 0 : it.pos, ch, lane, tr);
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-        w[i] = col_ok ? ld_f<BF16>(t.w, col + i, p.w_f32) : 0.f;
-        wo[i] = pairs ? ld_f<BF16>(t.w, pcol + i, p.w_f32) : 0.f;
-    }
+        for (int u = 0; u < U; u++) {
+            const int head = it.head0 + u * RPW + sub;
+            float f[8], o[8], ss = 0.f;
+            unpack8<BF16>(x[u], f);
 #pragma unroll
-    for (int u = 0; u < U; u++) {
-        const int head = it.head0 + u * RPW + sub;
-        float f[8], o[8], ss = 0.f;
-        unpack8<BF16>(x[u], f);
+            for (int i = 0; i < 8; i++) ss += f[i] * f[i];
+            const float r = 1.f / sqrtf(row_sum<LPR>(ss) / (float)p.d + p.eps);
+            unpack8<BF16>(from_lane(x[u], tr.partner), o);
 #pragma unroll
-        for (int i = 0; i < 8; i++) ss += f[i] * f[i];
-        const float r = 1.f / sqrtf(row_sum<LPR>(ss) / (float)p.d + p.eps);
-        unpack8<BF16>(from_lane(x[u], tr.partner), o);
-#pragma unroll
-        for (int i = 0; i < 8; i++) { f[i] *= r * w[i]; o[i] *= r * wo[i]; }
-        turn8(p, tr, inside, f, o, 1.f);
-        if (col_ok && head < t.h) *(i32x4 *)(yp + head * t.y_hs) = pack8<BF16>(f);
+            for (int i = 0; i < 8; i++) { f[i] *= r * w[i]; o[i] *= r * wo[i]; }
+            turn8(p, tr, inside, f, o, 1.f);
+            if (col_ok && head < t.h) *(i32x4 *)(yp + head * t.y_hs) = pad ? i32x4{0, 0, 0, 0} : pack8<BF16>(f);
+        }
     }
 }
 
@@ -186,7 +191,7 @@ qk_norm_bwd_kernel(const QKNormParams p, const int64_t items_q, const int64_t it
     constexpr int RPW = 64 / LPR;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const bool is_k = (int)blockIdx.x >= p.blocks_q;
-    const QKNormTensor &t = p.t[is_k];
+    const QKNormTensor t = is_k ? p.t[1] : p.t[0];
     const int blk = is_k ? blockIdx.x - p.blocks_q : blockIdx.x, n_blk = is_k ? p.blocks_k : p.blocks_q;
     const int64_t items = is_k ? items_k : items_q;
     const int parts = is_k ? parts_k : parts_q;
@@ -194,10 +199,8 @@ qk_norm_bwd_kernel(const QKNormParams p, const int64_t items_q, const int64_t it
     const bool col_ok = col < p.d, inside = col < p.rd;
     float w[8], acc[8];
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-        w[i] = col_ok ? ld_f<BF16>(t.w, col + i, p.w_f32) : 0.f;
-        acc[i] = 0.f;
-    }
+    for (int i = 0; i < 8; i++) w[i] = acc[i] = 0.f;
+    if (col_ok) ld_f<BF16, 8>(t.w, col, p.w_f32, w);
     for (int64_t item = (int64_t)blk * N_NW + wave; item < items; item += (int64_t)n_blk * N_NW) {
         const Item it = find_item(p, item, parts, RPW * U);
         const unsigned short *xp = (const unsigned short *)t.x + it.bi * t.x_bs + it.si * t.x_rs + (col_ok ? col : 0);
@@ -256,12 +259,23 @@ qk_norm_bwd_kernel(const QKNormParams p, const int64_t items_q, const int64_t it
 template <bool BF16>
 __global__ void __launch_bounds__(N_NT)
 qk_norm_dw_kernel(const QKNormParams p) {
-    const QKNormTensor &t = p.t[blockIdx.y];
+    const QKNormTensor t = blockIdx.y ? p.t[1] : p.t[0];
     if (!t.dw) return;
     const int c = blockIdx.x * 8 + (threadIdx.x & 7), part = threadIdx.x >> 3;
     const int first = blockIdx.y ? p.blocks_q : 0, n = blockIdx.y ? p.blocks_k : p.blocks_q;
     float sum = 0.f;
-    for (int i = part; i < n; i += N_NT / 8) sum += p.dw_part[(int64_t)(first + i) * p.d + c];
+    constexpr int AHEAD = 8;       // loads in flight: the loop is latency
+    const float *src = p.dw_part + (int64_t)first * p.d + c;
+    for (int i = part; i < n; i += AHEAD * (N_NT / 8)) {
+        float v[AHEAD];
+#pragma unroll
+        for (int j = 0; j < AHEAD; j++) {
+            const int at = i + j * (N_NT / 8);
+            v[j] = src[(int64_t)min(at, n - 1) * p.d];
+        }
+#pragma unroll
+        for (int j = 0; j < AHEAD; j++) sum += i + j * (N_NT / 8) < n ? v[j] : 0.f;
+    }
     __shared__ float s[N_NT];
     s[threadIdx.x] = sum;
     __syncthreads();
@@ -280,14 +294,17 @@ static int head_parts(const QKNormParams &p, int side) {
     return (p.t[side].h + rows - 1) / rows;
 }
 
-// Workgroups of the backward per side: enough that every CU has work, few enough that the partial sums of
-// dw stay small beside q and k.
-void qk_norm_bwd_blocks(QKNormParams &p, int cus) {
-    for (int side = 0; side < 2; side++) {
-        const long long items = (long long)p.b * p.s * head_parts(p, side);
-        const long long want = (items + N_NW - 1) / N_NW;
-        (side ? p.blocks_k : p.blocks_q) = (int)std::max(1LL, std::min(want, 4LL * cus));
-    }
+// Workgroups, shared out between the sides by their items: enough that every CU has work, few enough that the
+// weights are loaded (and, backward, the partial sums of dw written) seldom.
+void qk_norm_blocks(QKNormParams &p, int cus, bool bwd) {
+    const long long iq = (long long)p.b * p.s * head_parts(p, 0), ik = (long long)p.b * p.s * head_parts(p, 1);
+    const long long most = (bwd ? 6LL : 8LL) * cus, all = std::max(1LL, iq + ik);
+    auto share = [&](long long items) {
+        const long long want = (items + N_NW - 1) / N_NW, part = (most * items + all - 1) / all;
+        return (int)std::max(1LL, std::min(want, part));
+    };
+    p.blocks_q = share(iq);
+    p.blocks_k = share(ik);
 }
 
 template <bool BF16, int LPR>
@@ -295,10 +312,8 @@ static hipError_t launch(const QKNormParams &p, bool bwd, hipStream_t stream) {
     const int parts_q = head_parts(p, 0), parts_k = head_parts(p, 1);
     const int64_t items_q = (int64_t)p.b * p.s * parts_q, items_k = (int64_t)p.b * p.s * parts_k;
     if (!bwd) {
-        const int64_t blocks = (items_q + items_k + N_NW - 1) / N_NW;
-        if (blocks > 0x7fffffff) return hipErrorInvalidValue;
-        hipLaunchKernelGGL((qk_norm_fwd_kernel<BF16, LPR, N_U>), dim3((unsigned)blocks), dim3(N_NT), 0, stream, p, items_q,
-                           items_q + items_k, parts_q, parts_k);
+        hipLaunchKernelGGL((qk_norm_fwd_kernel<BF16, LPR, N_U>), dim3((unsigned)(p.blocks_q + p.blocks_k)), dim3(N_NT), 0, stream, p,
+                           items_q, items_k, parts_q, parts_k);
         return hipGetLastError();
     }
     hipLaunchKernelGGL((qk_norm_bwd_kernel<BF16, LPR, N_U>), dim3((unsigned)(p.blocks_q + p.blocks_k)), dim3(N_NT), 0, stream, p,

@@ -1140,8 +1140,14 @@ void set_qk_norm(vfa_qk_norm_rotary_params &P, QKNormHeld &held, const Tensor &q
     P.q = q.data_ptr(); P.k = k.data_ptr();
     P.q_batch_stride = stride_of(q, 0); P.q_row_stride = stride_of(q, 1); P.q_head_stride = stride_of(q, 2);
     P.k_batch_stride = stride_of(k, 0); P.k_row_stride = stride_of(k, 1); P.k_head_stride = stride_of(k, 2);
-    P.q_weight = wq.data_ptr(); P.k_weight = wk.data_ptr();
-    P.rotary_cos = cos.data_ptr(); P.rotary_sin = sin.data_ptr();
+    const void *aligned[4];
+    int n = 0;
+    for (const Tensor *t : {&wq, &wk, &cos, &sin}) {   // (contiguous; a view can still start off a 16-byte boundary)
+        held.t.push_back(((uintptr_t)t->data_ptr() & 15) == 0 ? *t : t->clone());
+        aligned[n++] = held.t.back().data_ptr();
+    }
+    P.q_weight = aligned[0]; P.k_weight = aligned[1];
+    P.rotary_cos = aligned[2]; P.rotary_sin = aligned[3];
     P.table_rows = (int)cos.size(0); P.rotary_dim = (int)rd; P.is_rotary_interleaved = interleaved;
     P.eps = (float)eps;
 }

@@ -43,5 +43,9 @@ def qk_norm_rotary_func(q, k, q_weight, k_weight, rotary_cos, rotary_sin, positi
         positions = positions.contiguous()
     if any(t.requires_grad for t in (rotary_cos, rotary_sin)):
         raise ValueError("rotary_cos and rotary_sin have no gradient: detach them")
-    out = QKNormRotaryFunc.apply(q, k, q_weight, k_weight, rotary_cos, rotary_sin, positions, eps, rotary_interleaved)
+    args = (q, k, q_weight, k_weight, rotary_cos, rotary_sin, positions, eps, rotary_interleaved)
+    if torch.is_grad_enabled() and any(t.requires_grad for t in args[:4]):
+        out = QKNormRotaryFunc.apply(*args)
+    else:   # (a serving step is a few microseconds; recording it for a backward that cannot come would double that)
+        out = tuple(flash_attn_cuda.qk_norm_rotary_fwd(*args))
     return tuple(x[0] for x in out) if ragged else out
