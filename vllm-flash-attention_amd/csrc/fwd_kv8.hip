@@ -52,6 +52,23 @@ __device__ __forceinline__ float quad_sum(float x) {
     auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
     return half_swap_sum(__uint_as_float(r[0]) + __uint_as_float(r[1]));
 }
+// Inclusive scan over the wave's lanes (sum or maximum) by lane shifts inside the vector unit; lane 63 ends up with
+// the total.
+template <bool MAX>
+__device__ __forceinline__ int wave_scan(int x) {
+    auto join = [](int a, int b) { return MAX ? max(a, b) : a + b; };
+    x = join(x, __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false));   // row_shr:1
+    x = join(x, __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false));
+    x = join(x, __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false));
+    x = join(x, __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false));
+    x = join(x, __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false));   // row_bcast:15
+    x = join(x, __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false));   // row_bcast:31
+    return x;
+}
+// (values of at least 0: what a shift brings in from outside is 0)
+__device__ __forceinline__ int wave_total(int x) { return __builtin_amdgcn_readlane(wave_scan<false>(x), 63); }
+__device__ __forceinline__ int wave_top(int x) { return __builtin_amdgcn_readlane(wave_scan<true>(x), 63); }
+
 // 16-byte chunk of row `row` of the V image: the 16 rows that 32 lanes of a transposed read touch lie in
 // different banks
 template <int DP>
@@ -118,11 +135,6 @@ fwd_kv8_kernel(const KV8Params a, const int n_mblocks) {
             return qi > q0 && !(a.max_rows > 0 && qi > a.max_rows) ? min((len + A_STEP - 1) / A_STEP, span) : -1;
         };
         auto parts_of = [](int st, int part_steps) -> int { return st < 0 ? 0 : max(1, (st + part_steps - 1) / part_steps); };
-        auto wave_sum = [](int x) {
-#pragma unroll
-            for (int off = 32; off > 0; off >>= 1) x += __shfl_xor(x, off);
-            return x;
-        };
         // Every wave works this out for itself, a lane a sequence (64 at a time): no barrier.  Steps of a part: the
         // total over the goal, less about half a part that every sequence leaves over; if the parts then are more
         // than the goal after all (a second round of workgroups), less a whole one each.  Not so few that a
@@ -135,16 +147,15 @@ fwd_kv8_kernel(const KV8Params a, const int n_mblocks) {
             top = max(top, st);
             some += st >= 0;
         }
-        sum = wave_sum(sum);
-        some = wave_sum(some);
-#pragma unroll
-        for (int off = 32; off > 0; off >>= 1) top = max(top, __shfl_xor(top, off));
+        sum = wave_total(sum);
+        some = wave_total(some);
+        top = wave_top(top);
         const int least = max((top + p.num_splits - 1) / p.num_splits, A_MIN_STEPS * parts);
         int part_steps = max((sum - 1) / max(a.split_goal - some / 2, 1) + 1, least);
         if (some > 1) {
             int n = parts_of(st0, part_steps);
             for (int i = lane + 64; i < p.b; i += 64) n += parts_of(steps_of(i), part_steps);
-            if (wave_sum(n) > a.split_goal)
+            if (wave_total(n) > a.split_goal)
                 part_steps = a.split_goal > some ? max((sum - 1) / (a.split_goal - some) + 1, least) : max(top, 1);
         }
         // the sequence in whose run of parts L falls
@@ -152,12 +163,7 @@ fwd_kv8_kernel(const KV8Params a, const int n_mblocks) {
         bidb = -1;
         for (int i = lane; i - lane < p.b && bidb < 0; i += 64) {
             const int mine = parts_of(i == lane ? st0 : steps_of(i), part_steps);
-            int upto = mine;
-#pragma unroll
-            for (int off = 1; off < 64; off <<= 1) {
-                const int y = __shfl_up(upto, off);
-                if (lane >= off) upto += y;
-            }
+            const int upto = wave_scan<false>(mine);
             const uint64_t hit = __ballot(before + upto > L);
             if (hit) {
                 const int at = __builtin_ctzll(hit);
@@ -519,22 +525,24 @@ kv8_combine_kernel(const KV8Params a, const int n_mblocks, const int rows_per_bl
     const KParams &p = a.p;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int pos = blockIdx.x % a.acc_sq, bh = blockIdx.x / a.acc_sq, bidb = bh / p.h, head = bh % p.h;
-    const BlockInfo bi(p, bidb);
-    if (pos >= bi.sq || (a.max_rows > 0 && bi.sq * p.h_ratio > a.max_rows)) return;
-    const int ns = a.n_split[bidb * n_mblocks + (pos * p.h_ratio + head % p.h_ratio) / rows_per_block];
-    if (ns <= 1) return;                       // one part: written in place
+    // (requested before the number of parts is known, up to what there is scratch for)
     __shared__ float s_w[128], s_red[2][2], s_part[256 * 8];
     const int cpr = p.d / 8, nlane = 256 / cpr, ch = tid % cpr, sl = tid / cpr;
     const int64_t rows = (int64_t)p.b * p.h * a.acc_sq, row = (int64_t)bh * a.acc_sq + pos;
-    const float my = tid < ns ? p.lseaccum[tid * rows + row] : -INFINITY;
+    float my = p.lseaccum[min(tid, p.num_splits - 1) * rows + row];
     constexpr int PRE = 4;
     f32x4 r0[PRE], r1[PRE];
 #pragma unroll
     for (int i = 0; i < PRE; i++) {
-        const float *src = p.oaccum + (min(sl + i * nlane, ns - 1) * rows + row) * p.d + ch * 8;   // (clamped: weight 0 below)
+        const float *src = p.oaccum + (min(sl + i * nlane, p.num_splits - 1) * rows + row) * p.d + ch * 8;
         r0[i] = *(const f32x4 *)src;
         r1[i] = *(const f32x4 *)(src + 4);
     }
+    const int ns = a.n_split[bidb * n_mblocks + (pos * p.h_ratio + head % p.h_ratio) / rows_per_block];
+    const BlockInfo bi(p, bidb);
+    if (pos >= bi.sq || (a.max_rows > 0 && bi.sq * p.h_ratio > a.max_rows)) return;
+    if (ns <= 1) return;                       // one part: written in place
+    my = tid < ns ? my : -INFINITY;
     float m = my;
 #pragma unroll
     for (int off = 32; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor(m, off));
