@@ -81,8 +81,8 @@ __host__ __device__ constexpr int kv8_swz(int row) {
 // Columns from p.d to DP are zero in Q; a lane whose columns lie there reads column 0 of its key instead (a
 // finite code times zero, or a NaN that the key has anyway), its O is never stored.
 //
-// The loop is free of branches on the usual path, loads run NBUF steps ahead of their use (past the last
-// step they repeat it), and the page ids another step ahead of the loads.
+// The loop is free of branches on the usual path, loads run NBUF steps ahead of their use, and the page ids
+// another step ahead of the loads.
 // NT: the codes are loaded past the caches.  For streams that the 256 MiB last-level cache cannot hold anyway
 // (b128 kv8192 h32/8 d128: 5.85 -> 6.23 TB/s); shorter ones find part of it there (b1 kv65536: 37 against 50 us).
 //
@@ -94,6 +94,7 @@ __global__ void __launch_bounds__(A_NT, (DP == 64 && NR == 1) ? 4 : 2)
 fwd_kv8_kernel(const KV8Params a, const int n_mblocks) {
     using Cfg = Kv8Cfg<DP, NR>;
     constexpr int NBUF = DP <= 128 ? 2 : 1;
+    touch_kv8_args();
     constexpr int NJ = DP / 64;              // 64-column groups of K: one 16-byte load per lane and key tile
     constexpr int NDB = DP / 16;             // 16-column blocks of O
     constexpr int CPR = DP / 16;             // 16-byte chunks of a V row
@@ -104,8 +105,8 @@ fwd_kv8_kernel(const KV8Params a, const int n_mblocks) {
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int c = lane & 15, g = lane >> 4;
-    const int hpw = a.heads_per_wg, parts = A_NW / hpw;
-    const int whead = wave & (hpw - 1), part = wave / hpw;
+    const int hpw = a.heads_per_wg, hpw_sh = __builtin_ctz(hpw), parts = A_NW >> hpw_sh;   // (powers of two)
+    const int whead = wave & (hpw - 1), part = wave >> hpw_sh;
 
     // row blocks of the same keys on one XCD, whose L2 they share
     int L = blockIdx.x;
@@ -116,7 +117,7 @@ fwd_kv8_kernel(const KV8Params a, const int n_mblocks) {
             L = k / n_mblocks * group + L % 8 * n_mblocks + k % n_mblocks;
         }
     }
-    const int n_hblocks = p.h_k / hpw;
+    const int n_hblocks = p.h_k >> hpw_sh;
     const int m_block = L % n_mblocks; L /= n_mblocks;
     const int hblock = L % n_hblocks; L /= n_hblocks;
     const int hk = hblock * hpw + whead;
@@ -281,6 +282,7 @@ fwd_kv8_kernel(const KV8Params a, const int n_mblocks) {
     // (the ids of the step after `n`, in `after`, are requested in front of n's rows: loads return in order, so
     // what waits for those ids later does not wait for the rows)
     auto load_step = [&](int n, Set &w, int after) __attribute__((always_inline)) {
+        const unsigned bytes = n < n1 ? 0xffffffffu : 0u;           // past the last step: zeros, and no access
         const int key = min(n * A_STEP + 16 * tl, last_tile);
         const bool bad = (unsigned)pid >= (unsigned)a.num_pages;   // outside the pool: NaN, from the scale
         const unsigned pg = bad ? 0u : (unsigned)pid;
@@ -294,7 +296,7 @@ fwd_kv8_kernel(const KV8Params a, const int n_mblocks) {
         auto rows_at = [&](int i) __attribute__((always_inline)) {   // address i of the eight, as a buffer's base
             const uint64_t base = (uint64_t)(unsigned)__builtin_amdgcn_readlane((int)alo, i) |
                                   (uint64_t)(unsigned)__builtin_amdgcn_readlane((int)ahi, i) << 32;
-            return __builtin_amdgcn_make_buffer_rsrc((void *)base, 0, 0xffffffffu, 0x00020000);
+            return __builtin_amdgcn_make_buffer_rsrc((void *)base, 0, bytes, 0x00020000);
         };
 #pragma unroll
         for (int t = 0; t < 2; t++) {
@@ -371,7 +373,7 @@ fwd_kv8_kernel(const KV8Params a, const int n_mblocks) {
             const int at = i < NV / 2 ? vwr[i] : (vwr[i - NV / 2] ^ SWZ16) + 16 * DP;
             *(i32x4 *)(vimg + at) = w.v[i];
         }
-        load_step(min(next, n1 - 1), w, min(next + parts, n1 - 1));
+        load_step(next, w, next + parts);
 
         bool need = k0 + A_STEP > sk;
         if (edge_r) need = need || (k0 + A_STEP > pos_lo + 1 + sk - sq + p.wr);
@@ -449,7 +451,7 @@ fwd_kv8_kernel(const KV8Params a, const int n_mblocks) {
     if (first < n1) {
         load_pages(first);
 #pragma unroll
-        for (int i = 0; i < NBUF; i++) load_step(min(first + i * parts, n1 - 1), set[i], min(first + (i + 1) * parts, n1 - 1));
+        for (int i = 0; i < NBUF; i++) load_step(first + i * parts, set[i], first + (i + 1) * parts);
         // (one way out of the loop: with another in the middle the compiler's wait counts take the path
         // around it for one that leads back, and every step waits for the loads of the next)
         int n = first;
@@ -458,7 +460,7 @@ fwd_kv8_kernel(const KV8Params a, const int n_mblocks) {
                 step(n, set[0], n + 2 * parts);
                 step(n + parts, set[1], n + 3 * parts);
             }
-            if (n < n1) step(n, set[0], n1);
+            if (n < n1) step(n, set[0], n + 2 * parts);
         } else {
             for (; n < n1; n += parts) step(n, set[0], n + parts);
         }
@@ -493,25 +495,27 @@ fwd_kv8_kernel(const KV8Params a, const int n_mblocks) {
         if (part == 0 && g == 0 && row < rows)
             lse[stat_at(hk, row)] = none ? (is_split ? -INFINITY : INFINITY) : m_all * p.scale + __logf(l_all);
         __syncthreads();
-        for (int i = tid; i < hpw * 16 * (DP / 8); i += A_NT) {
-            const int ch = i % (DP / 8), rr = i / (DP / 8) % 16, hs = i / (DP / 8) / 16;
+        const int live = min(16, rows - (q0 + 16 * r));           // rows of this 16 that exist
+        for (int i = tid; i < hpw * live * (DP / 8); i += A_NT) {
+            const int ch = i % (DP / 8), j = i / (DP / 8), hs = j & (hpw - 1), rr = j >> hpw_sh;
+            if (ch * 8 >= p.d) continue;
             const int orow = q0 + 16 * r + rr, head = hblock * hpw + hs;
-            if (orow >= rows || ch * 8 >= p.d) continue;
             f32x4 a0 = {0, 0, 0, 0}, a1 = {0, 0, 0, 0};
             for (int w = 0; w < parts; w++) {
                 const char *src = smem + ((w * hpw + hs) * 16 + rr) * Cfg::O_ROWB + ch * 32;
                 a0 += *(const f32x4 *)src;
                 a1 += *(const f32x4 *)(src + 16);
             }
+            const int opos = orow / ratio, ohead = head * ratio + orow - opos * ratio;
             if (is_split) {
-                float *dst = p.oaccum + stat_at(head, orow) * p.d + ch * 8;
+                float *dst = p.oaccum + ((((int64_t)split * p.b + bidb) * p.h + ohead) * a.acc_sq + opos) * p.d + ch * 8;
                 *(f32x4 *)dst = a0;
                 *(f32x4 *)(dst + 4) = a1;
             } else {
                 i32x4 w;
                 w[0] = pack2<BF16>(a0[0], a0[1]); w[1] = pack2<BF16>(a0[2], a0[3]);
                 w[2] = pack2<BF16>(a1[0], a1[1]); w[3] = pack2<BF16>(a1[2], a1[3]);
-                *(i32x4 *)(og + (int64_t)(orow / ratio) * p.o_rs + (int64_t)(head * ratio + orow % ratio) * p.o_hs + ch * 8) = w;
+                *(i32x4 *)(og + (int64_t)opos * p.o_rs + (int64_t)ohead * p.o_hs + ch * 8) = w;
             }
         }
     }

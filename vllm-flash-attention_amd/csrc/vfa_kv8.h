@@ -72,6 +72,22 @@ __device__ __forceinline__ int kv8_row_in_page(const KV8Params &a, int tok) {
     return a.p.block_table ? tok - kv8_div(tok >> 4, a.page_mul, a.page_sh) * a.page_rows : tok;
 }
 
+// Requests every cache line of the kernel's arguments (a KV8Params first) at once.  They lie in host memory: left to
+// their first uses, the lines of a large argument block arrive one after the other, a microsecond or two each.
+__device__ __forceinline__ void touch_kv8_args() {
+    static_assert(sizeof(KV8Params) > 14 * 64 && sizeof(KV8Params) <= 15 * 64, "a load per line");
+    int x[15];
+    asm volatile("s_load_dword %0, %15, 0x0\n\ts_load_dword %1, %15, 0x40\n\ts_load_dword %2, %15, 0x80\n\t"
+                 "s_load_dword %3, %15, 0xc0\n\ts_load_dword %4, %15, 0x100\n\ts_load_dword %5, %15, 0x140\n\t"
+                 "s_load_dword %6, %15, 0x180\n\ts_load_dword %7, %15, 0x1c0\n\ts_load_dword %8, %15, 0x200\n\t"
+                 "s_load_dword %9, %15, 0x240\n\ts_load_dword %10, %15, 0x280\n\ts_load_dword %11, %15, 0x2c0\n\t"
+                 "s_load_dword %12, %15, 0x300\n\ts_load_dword %13, %15, 0x340\n\ts_load_dword %14, %15, 0x380\n\t"
+                 "s_waitcnt lgkmcnt(0)"
+                 : "=&s"(x[0]), "=&s"(x[1]), "=&s"(x[2]), "=&s"(x[3]), "=&s"(x[4]), "=&s"(x[5]), "=&s"(x[6]), "=&s"(x[7]),
+                   "=&s"(x[8]), "=&s"(x[9]), "=&s"(x[10]), "=&s"(x[11]), "=&s"(x[12]), "=&s"(x[13]), "=&s"(x[14])
+                 : "s"(__builtin_amdgcn_kernarg_segment_ptr()));
+}
+
 __device__ __forceinline__ float e8m0_to_f32(unsigned byte) {
     return __uint_as_float(byte == 255u ? 0x7fc00000u : byte << 23);
 }
