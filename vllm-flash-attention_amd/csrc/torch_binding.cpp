@@ -18,6 +18,7 @@
 #include <optional>
 #include <vector>
 #include <torch/csrc/Dtype.h>
+#include <torch/csrc/autograd/custom_function.h>
 
 #include "vfa.h"
 
@@ -1208,6 +1209,42 @@ std::vector<Tensor> qk_norm_rotary_bwd(const Tensor &dqo_, const Tensor &dko_, c
     return {dq, dk, dwq, dwk};
 }
 
+// qk_norm_rotary as a node of the autograd graph.  In C++ rather than Python: forward and backward of a short
+// sequence are a few microseconds of kernels, and a Python node's backward costs the engine's thread several times
+// that (b1 s2731 h12/12 d96: 97 -> 78 us a forward and backward).
+struct QKNormRotary : torch::autograd::Function<QKNormRotary> {
+    static torch::autograd::variable_list forward(torch::autograd::AutogradContext *ctx, const Tensor &q, const Tensor &k, const Tensor &wq,
+                                                  const Tensor &wk, const Tensor &cos, const Tensor &sin, const OptTensor &positions,
+                                                  double eps, bool interleaved) {
+        ctx->save_for_backward({q, k, wq, wk, cos, sin, positions.has_value() ? positions.value() : Tensor()});
+        ctx->saved_data["eps"] = eps;
+        ctx->saved_data["interleaved"] = interleaved;
+        return qk_norm_rotary_fwd(q, k, wq, wk, cos, sin, positions, eps, interleaved);
+    }
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx, torch::autograd::variable_list grads) {
+        TORCH_CHECK(!at::GradMode::is_enabled(), "qk_norm_rotary_func: its gradients have no gradient (create_graph=True)");
+        const auto saved = ctx->get_saved_variables();
+        const Tensor &q = saved[0], &k = saved[1];
+        OptTensor positions;
+        if (saved[6].defined()) positions = saved[6];
+        // an output that nothing was asked of
+        const Tensor dq_out = grads[0].defined() ? grads[0] : torch::zeros_like(q), dk_out = grads[1].defined() ? grads[1] : torch::zeros_like(k);
+        auto out = qk_norm_rotary_bwd(dq_out, dk_out, q, k, saved[2], saved[3], saved[4], saved[5], positions,
+                                      ctx->saved_data["eps"].toDouble(), ctx->saved_data["interleaved"].toBool(), ctx->needs_input_grad(0),
+                                      ctx->needs_input_grad(1), ctx->needs_input_grad(2), ctx->needs_input_grad(3));
+        out.resize(9);
+        return out;
+    }
+};
+
+std::vector<Tensor> qk_norm_rotary(const Tensor &q, const Tensor &k, const Tensor &wq, const Tensor &wk, const Tensor &cos, const Tensor &sin,
+                                   const OptTensor &positions, double eps, bool interleaved) {
+    // a serving step is a few microseconds: it is not recorded for a backward that cannot come
+    if (at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || wq.requires_grad() || wk.requires_grad()))
+        return QKNormRotary::apply(q, k, wq, wk, cos, sin, positions, eps, interleaved);
+    return qk_norm_rotary_fwd(q, k, wq, wk, cos, sin, positions, eps, interleaved);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -1237,6 +1274,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
                               torch::python::detail::py_object_to_dtype(dtype));
     }, "Read an 8-bit KV cache in 16 bits");
     m.def("fwd_kv8", &fwd_kv8, "Forward pass, with an 8-bit KV cache");
-    m.def("qk_norm_rotary_fwd", &qk_norm_rotary_fwd, "RMS norm and rotation of query and key heads");
-    m.def("qk_norm_rotary_bwd", &qk_norm_rotary_bwd, "Backward of qk_norm_rotary_fwd");
+    m.def("qk_norm_rotary", &qk_norm_rotary, "RMS norm and rotation of query and key heads, differentiable");
 }

@@ -1,22 +1,7 @@
 """RMS norm of query and key heads with the position rotation in the same pass, forward and backward."""
-import torch
-from torch.autograd.function import once_differentiable
+import torch  # noqa: F401  (in front of the extension, which links against it)
 
 import vllm_flash_attn_2_cuda as flash_attn_cuda
-
-
-class QKNormRotaryFunc(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, q_weight, k_weight, rotary_cos, rotary_sin, positions, eps, interleaved):
-        ctx.save_for_backward(q, k, q_weight, k_weight, rotary_cos, rotary_sin, positions)
-        ctx.eps, ctx.interleaved = eps, interleaved
-        return tuple(flash_attn_cuda.qk_norm_rotary_fwd(q, k, q_weight, k_weight, rotary_cos, rotary_sin, positions, eps, interleaved))
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dq_out, dk_out):
-        grads = flash_attn_cuda.qk_norm_rotary_bwd(dq_out, dk_out, *ctx.saved_tensors, ctx.eps, ctx.interleaved, *ctx.needs_input_grad[:4])
-        return (*grads, None, None, None, None, None)
 
 
 def qk_norm_rotary_func(q, k, q_weight, k_weight, rotary_cos, rotary_sin, positions=None, eps=1e-6, rotary_interleaved=True):
@@ -41,11 +26,7 @@ def qk_norm_rotary_func(q, k, q_weight, k_weight, rotary_cos, rotary_sin, positi
         q, k, positions = q[None], k[None], positions[None]
     if positions is not None and positions.stride(-1) != 1:
         positions = positions.contiguous()
-    if any(t.requires_grad for t in (rotary_cos, rotary_sin)):
+    if rotary_cos.requires_grad or rotary_sin.requires_grad:
         raise ValueError("rotary_cos and rotary_sin have no gradient: detach them")
-    args = (q, k, q_weight, k_weight, rotary_cos, rotary_sin, positions, eps, rotary_interleaved)
-    if torch.is_grad_enabled() and any(t.requires_grad for t in args[:4]):
-        out = QKNormRotaryFunc.apply(*args)
-    else:   # (a serving step is a few microseconds; recording it for a backward that cannot come would double that)
-        out = tuple(flash_attn_cuda.qk_norm_rotary_fwd(*args))
-    return tuple(x[0] for x in out) if ragged else out
+    out = flash_attn_cuda.qk_norm_rotary(q, k, q_weight, k_weight, rotary_cos, rotary_sin, positions, eps, rotary_interleaved)
+    return tuple(x[0] for x in out) if ragged else tuple(out)
