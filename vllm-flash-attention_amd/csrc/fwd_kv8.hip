@@ -226,6 +226,18 @@ fwd_kv8_kernel(const KV8Params a, const int n_mblocks) {
         return;
     }
 
+    const int tl = lane & 1;                         // the tile of a step that this lane works out addresses for
+    const int last_tile = (sk - 1) & ~15;
+    // Page id of the lane's tile.  A tile of 16 keys lies in one page and in one block of the scales (both
+    // are multiples of 16 rows); one that starts past the sequence's end takes its last tile (masked keys).
+    const int *table = PAGED ? p.block_table + (int64_t)bidb * p.bt_bs : nullptr;
+    int pid = PAGED ? 0 : p.cache_batch_idx ? p.cache_batch_idx[bidb] : bidb;
+    auto load_pages = [&](int n) __attribute__((always_inline)) {
+        if constexpr (PAGED) pid = table[kv8_div(min(n * A_STEP + 16 * tl, last_tile) >> 4, a.page_mul, a.page_sh)];
+    };
+    const int first = n0 + part;
+    load_pages(min(first, n1 - 1));      // (in front of Q: the first rows wait for these)
+
     // Q operand: columns 64 j + 16 g + 8 s .. of k-step 2 j + s
     i32x4 qf[NR][2 * NJ];
     int pos[NR];
@@ -259,7 +271,7 @@ fwd_kv8_kernel(const KV8Params a, const int n_mblocks) {
     // address i (tile i & 1 of K, V, K scale, V scale); the rows' are then read into scalar registers and the
     // scales fetched by the lanes that hold theirs.  (As scalar arithmetic this was a third of the step's
     // instructions, and few-wave launches are bound by those.)
-    const int sel = (lane >> 1) & 3, tl = lane & 1;
+    const int sel = (lane >> 1) & 3;
     const unsigned char *lbase = sel == 0 ? (const unsigned char *)p.k + (int64_t)hk * p.k_hs
                                : sel == 1 ? (const unsigned char *)p.v + (int64_t)hk * p.v_hs
                                : sel == 2 ? a.ks + (int64_t)hk * a.ks_hs : a.vs + (int64_t)hk * a.vs_hs;
@@ -271,14 +283,6 @@ fwd_kv8_kernel(const KV8Params a, const int n_mblocks) {
         unsigned sc, bad;        // lanes 4..7 (mod 8): K scales of the two tiles, V scales; 255 for a page outside the pool
     };
     Set set[NBUF];
-    const int last_tile = (sk - 1) & ~15;
-    // Page id of the lane's tile.  A tile of 16 keys lies in one page and in one block of the scales (both
-    // are multiples of 16 rows); one that starts past the sequence's end takes its last tile (masked keys).
-    const int *table = PAGED ? p.block_table + (int64_t)bidb * p.bt_bs : nullptr;
-    int pid = PAGED ? 0 : p.cache_batch_idx ? p.cache_batch_idx[bidb] : bidb;
-    auto load_pages = [&](int n) __attribute__((always_inline)) {
-        if constexpr (PAGED) pid = table[kv8_div(min(n * A_STEP + 16 * tl, last_tile) >> 4, a.page_mul, a.page_sh)];
-    };
     // (the ids of the step after `n`, in `after`, are requested in front of n's rows: loads return in order, so
     // what waits for those ids later does not wait for the rows)
     auto load_step = [&](int n, Set &w, int after) __attribute__((always_inline)) {
@@ -447,9 +451,7 @@ fwd_kv8_kernel(const KV8Params a, const int n_mblocks) {
         }
     };
 
-    const int first = n0 + part;
     if (first < n1) {
-        load_pages(first);
 #pragma unroll
         for (int i = 0; i < NBUF; i++) load_step(first + i * parts, set[i], first + (i + 1) * parts);
         // (one way out of the loop: with another in the middle the compiler's wait counts take the path

@@ -963,6 +963,7 @@ std::pair<Tensor, Tensor> set_kv8_new(vfa_kv8_params &P, const Tensor &k_, const
 void kv8_quantize(const Tensor &k, const Tensor &v, const Tensor &kc, const Tensor &vc, const Tensor &ks, const Tensor &vs,
                   const Tensor &seqlens, const OptTensor &cache_batch_idx, const OptTensor &block_table, const OptTensor &cu_seqlens,
                   int64_t max_seqlen) {
+    at::NoGradGuard no_grad;   // a cache is not trained through
     vfa_kv8_params P{};
     set_kv8_cache(P, kc, vc, ks, vs, -1, seqlens, cache_batch_idx, block_table);
     at::hip::HIPGuardMasqueradingAsCUDA device_guard{(c10::DeviceIndex)kc.get_device()};
@@ -975,6 +976,7 @@ void kv8_quantize(const Tensor &k, const Tensor &v, const Tensor &kc, const Tens
 std::vector<Tensor> kv8_dequantize(const Tensor &kc, const Tensor &vc, const Tensor &ks, const Tensor &vs, const Tensor &seqlens,
                                    const OptTensor &cache_batch_idx, const OptTensor &block_table, const OptTensor &cu_seqlens,
                                    int64_t rows, at::ScalarType dtype) {
+    at::NoGradGuard no_grad;   // a cache is not trained through
     vfa_kv8_params P{};
     const int64_t b = set_kv8_cache(P, kc, vc, ks, vs, -1, seqlens, cache_batch_idx, block_table);
     TORCH_CHECK(dtype == at::kHalf || dtype == at::kBFloat16, "FlashAttention only support fp16 and bf16 data type");
@@ -1009,6 +1011,7 @@ std::vector<Tensor> fwd_kv8(const Tensor &q_, const Tensor &kc, const Tensor &vc
                             OptTensor &v_, OptTensor &seqlens, OptTensor &cache_batch_idx, OptTensor &block_table, OptTensor &alibi_slopes,
                             OptTensor &out_, OptTensor &cu_seqlens_q, int64_t max_seqlen_q, const double softmax_scale, bool is_causal,
                             int64_t window_size_left, int64_t window_size_right, int64_t num_splits) {
+    at::NoGradGuard no_grad;   // a cache is not trained through
     const int dt = dtype_code(q_);
     const bool ragged = cu_seqlens_q.has_value();
     TORCH_CHECK(q_.dim() == (ragged ? 3 : 4), ragged ? "q must be (total_q, nheads, headdim) with cu_seqlens_q"

@@ -30,7 +30,6 @@ def _index(x):
     return None if x is None else x.contiguous()
 
 
-@torch.no_grad()
 def quantize_kvcache(k, v, k_cache, v_cache, k_scale, v_scale, cache_seqlens: Union[int, torch.Tensor],
                      cache_batch_idx: Optional[torch.Tensor] = None, block_table: Optional[torch.Tensor] = None,
                      cu_seqlens: Optional[torch.Tensor] = None, max_seqlen: Optional[int] = None):
@@ -53,7 +52,6 @@ def quantize_kvcache(k, v, k_cache, v_cache, k_scale, v_scale, cache_seqlens: Un
                                  max_seqlen or 0)
 
 
-@torch.no_grad()
 def dequantize_kvcache(k_cache, v_cache, k_scale, v_scale, cache_seqlens: torch.Tensor, max_seqlen: Optional[int] = None,
                        cu_seqlens: Optional[torch.Tensor] = None, total_seqlen: Optional[int] = None,
                        cache_batch_idx: Optional[torch.Tensor] = None, block_table: Optional[torch.Tensor] = None,
@@ -69,7 +67,6 @@ def dequantize_kvcache(k_cache, v_cache, k_scale, v_scale, cache_seqlens: torch.
                                                 max_seqlen if cu_seqlens is None else total_seqlen, dtype))
 
 
-@torch.no_grad()
 def flash_attn_with_quantized_kvcache(q, k_cache, v_cache, k_scale, v_scale, k=None, v=None,
                                       cache_seqlens: Optional[Union[int, torch.Tensor]] = None,
                                       cache_batch_idx: Optional[torch.Tensor] = None,
