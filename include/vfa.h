@@ -318,6 +318,8 @@ size_t vfa_qk_norm_rotary_bwd_workspace(const vfa_qk_norm_rotary_params *p);   /
 /* sizeof(vfa_params) of the built library, for foreign-function bindings to check their mirror of
  * the struct against (no counterpart in the reference: its boundary is typed by pybind). */
 size_t vfa_params_sizeof(void);
+size_t vfa_kv8_params_sizeof(void);
+size_t vfa_qk_norm_rotary_params_sizeof(void);
 
 /* Message of the last failed call on this thread ("" if none). */
 const char *vfa_last_error(void);

@@ -665,6 +665,7 @@ static int kv8_plan(const vfa_kv8_params *p, Kv8Plan &w) {
         w.goal = std::max(1, cus * vfa::kv8_decode_wgs_per_cu(a.d, w.dec_sq * ratio) / groups);
         const long long s = a.num_splits > 0 ? a.num_splits : w.goal * 2 <= a.b ? 1 : a.b == 1 ? w.goal : 4LL * ((w.goal + a.b - 1) / a.b);
         w.dec_splits = (int)std::max(1LL, std::min({s, most, 128LL}));
+        if ((long long)a.b * (a.seqlen_k / 32 + 1) > 0x7fffffff) w.dec_splits = 1;   // (the device adds the steps up in 32 bits)
         // (a count given: the grid holds that many parts of every sequence)
         w.grid = (int)std::min<long long>(0x7fffffff, a.num_splits > 0 ? (long long)a.b * w.dec_splits : std::max(w.goal, a.b));
         if (a.num_splits > 0) w.goal = w.grid;
@@ -882,5 +883,7 @@ extern "C" int vfa_qk_norm_rotary_bwd(const vfa_qk_norm_rotary_params *p) {
 }
 
 extern "C" size_t vfa_params_sizeof(void) { return sizeof(vfa_params); }
+extern "C" size_t vfa_kv8_params_sizeof(void) { return sizeof(vfa_kv8_params); }
+extern "C" size_t vfa_qk_norm_rotary_params_sizeof(void) { return sizeof(vfa_qk_norm_rotary_params); }
 extern "C" const char *vfa_last_error(void) { return g_err.c_str(); }
 extern "C" const char *vfa_version(void) { return "vfa-mi355x 0.1.0 (api of vllm_flash_attn 2.5.8.post3)"; }

@@ -180,7 +180,7 @@ fwd_prefill_kernel(const std::conditional_t<LD == 5, KV8Params, KParams> args, c
     int sk_ = bi.sk;
     if constexpr (KV8) sk_ = min(kv8_cached(args, bidb) + (p.knew ? p.seqlen_knew : 0), args.cap);
     const int sq = bi.sq, sk = sk_;
-    const int sq_rows = sq * ratio;    // rows of this (batch, head): query positions (x grouped heads)
+    const int sq_rows = (KV8 ? min(sq, p.seqlen_q) : sq) * ratio;    // rows of this (batch, head): query positions (x grouped heads)
     if constexpr (KV8) if (sq_rows <= args.min_rows) return;   // the decode kernel's
     // Philox state: the caller's values, or (under graph capture) read on the device at replay
     // time from the generator's captured state (at::cuda::philox::unpack, flash_fwd_kernel.h:45)

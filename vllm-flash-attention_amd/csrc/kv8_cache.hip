@@ -88,8 +88,9 @@ kv8_quantize_kernel(const KV8Params a, const int n_blocks, const int n_hgroups) 
     if (a.cu_new) { src0 = a.cu_new[bidb]; n_new = a.cu_new[bidb + 1] - a.cu_new[bidb]; }
     else { src0 = 0; n_new = p.seqlen_knew; }
     const int end = (int)min((int64_t)start + max(n_new, 0), (int64_t)a.cap);
-    const int lo = kv8_div(start >> 4, a.blk_mul, a.blk_sh) * a.blk + j * a.blk;
-    if (lo >= end || end <= start) return;
+    const int64_t block0 = kv8_div(start >> 4, a.blk_mul, a.blk_sh) * a.blk + (int64_t)j * a.blk;
+    if (block0 >= end || end <= start) return;
+    const int lo = (int)block0;
     const int r0 = max(start, lo), r1 = min(end, lo + a.blk);
     const int page = kv8_page(a, bidb, lo);
     if (page < 0) return;                // the table names no page of the pool: nothing is written
@@ -136,7 +137,8 @@ kv8_quantize_kernel(const KV8Params a, const int n_blocks, const int n_hgroups) 
     if (holds) e = max(e, e_old);
     // past this exponent the largest code would stand for a value the 16-bit type does not have
     constexpr int E_TOP = BF16 ? 120 : 8;
-    const float inv = exp2_int(-e), lim = e >= E_TOP ? 240.f : 448.f;
+    // (a scale of 2^127 and one that is NaN are never written here, but can stand in a cache made elsewhere)
+    const float inv = e < 127 ? exp2_int(-e) : __uint_as_float(0x400000u), lim = e >= E_TOP ? 240.f : 448.f;
     if (holds && e > e_old) {
         const float f = e - e_old > 126 ? 0.f : exp2_int(e_old - e);
         for (int row = wave; row < start - lo; row += Q_NW) {

@@ -9,6 +9,7 @@
 #include <ATen/hip/HIPContext.h>
 #include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 
 #include <ATen/Parallel.h>
 
@@ -19,6 +20,7 @@
 #include <vector>
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/variable.h>
 
 #include "vfa.h"
 
@@ -1240,11 +1242,27 @@ struct QKNormRotary : torch::autograd::Function<QKNormRotary> {
     }
 };
 
+// A leaf keeps the stream of the first live graph that it is part of, and a backward pass hands its gradient over to
+// that stream.  The default stream cannot take part in a capture: the backward pass would end the process.
+void expect_capturable(const Tensor &x) {
+    if (!x.requires_grad() || !x.is_leaf() || !x.is_cuda()) return;
+    const auto leaf = torch::autograd::impl::try_get_grad_accumulator(x);
+    const auto stream = leaf ? leaf->stream() : c10::nullopt;
+    TORCH_CHECK(!stream || stream->id() != 0,
+                "qk_norm_rotary_func: a graph recorded on the default stream still holds an input; drop it before capturing a pass with gradients");
+}
+
 std::vector<Tensor> qk_norm_rotary(const Tensor &q, const Tensor &k, const Tensor &wq, const Tensor &wk, const Tensor &cos, const Tensor &sin,
                                    const OptTensor &positions, double eps, bool interleaved) {
     // a serving step is a few microseconds: it is not recorded for a backward that cannot come
-    if (at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || wq.requires_grad() || wk.requires_grad()))
+    if (at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || wq.requires_grad() || wk.requires_grad())) {
+        if (q.is_cuda()) {
+            at::hip::HIPGuardMasqueradingAsCUDA device_guard{(c10::DeviceIndex)q.get_device()};
+            if (c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None)
+                for (const Tensor *x : {&q, &k, &wq, &wk}) expect_capturable(*x);
+        }
         return QKNormRotary::apply(q, k, wq, wk, cos, sin, positions, eps, interleaved);
+    }
     return qk_norm_rotary_fwd(q, k, wq, wk, cos, sin, positions, eps, interleaved);
 }
 
