@@ -367,6 +367,39 @@ def test_large_and_uneven_batches(b, h, hk, d, cap, num_splits):
     _check(cache, lens, _q((b, 1, h, d), "bf16", 93), "bf16", num_splits=num_splits)
 
 
+@pytest.mark.parametrize("equal", [True, False])
+@pytest.mark.parametrize("b,sq,h,hk,d,cap,dtype,page", [
+    (150, 1, 4, 4, 128, 1600, "bf16", 32),           # one to two workgroups a sequence
+    (300, 1, 4, 4, 128, 1000, "fp16", 0),            # more sequences than workgroups
+    (140, 1, 20, 1, 128, 3000, "bf16", 32),          # 32 rows
+    (140, 2, 2, 2, 256, 1600, "fp16", 64),
+    (600, 1, 4, 4, 112, 700, "bf16", 16),
+])
+def test_runs_of_keys_across_sequences(b, sq, h, hk, d, cap, dtype, page, equal):
+    """Batches that parts of equal length leave much of the chip idle with: a workgroup then has pieces of several
+    sequences.  Some sequences are empty; the result does not depend on the batch that a sequence is in, beyond the
+    order of sums."""
+    g = torch.Generator().manual_seed(91)
+    lens = [cap] * b if equal else (cap * torch.rand(b, generator=g)).int().tolist()
+    lens[3] = lens[70] = 0
+    cache = Cache(b, cap, hk, d, 16, page, seed=92)
+    _check(cache, lens, _q((b, sq, h, d), dtype, 93), dtype)
+
+
+def test_runs_of_keys_with_windows_and_new_tokens():
+    b, cap = 150, 1600
+    lens = (cap * (0.5 + 0.5 * torch.rand(b, generator=torch.Generator().manual_seed(94)))).int().tolist()
+    cache = Cache(b, cap + 2, 4, 128, 16, 16, seed=95)
+    q = _q((b, 2, 8, 128), "bf16", 96)
+    _check(cache, lens, q, "bf16", causal=True, window=(900, 0))
+    _check(cache, lens, q, "bf16", causal=True, news=[_q((b, 2, 4, 128), "bf16", 97 + w) for w in range(2)])
+    gpu, table = cache.gpu(), cache.block_table()
+    args = dict(cache_seqlens=torch.tensor(lens, dtype=torch.int32).cuda(), block_table=table, causal=True)
+    first = _fa().flash_attn_with_quantized_kvcache(q.cuda(), *gpu, **args)
+    for _ in range(10):
+        assert torch.equal(first, _fa().flash_attn_with_quantized_kvcache(q.cuda(), *gpu, **args))
+
+
 def test_scales_at_the_ends_of_their_range():
     """Bytes 0 and 254 (2^-127, 2^127) and 255 (NaN): never written here, but what a cache from elsewhere can hold."""
     fa = _fa()

@@ -663,12 +663,12 @@ static int kv8_plan(const vfa_kv8_params *p, Kv8Plan &w) {
         const int groups = (int)std::max(1LL, items / a.b);
         const long long most = std::max(1LL, (long long)a.seqlen_k / (32LL * 3 * parts));
         w.goal = std::max(1, cus * vfa::kv8_decode_wgs_per_cu(a.d, w.dec_sq * ratio) / groups);
-        const long long s = a.num_splits > 0 ? a.num_splits : w.goal * 2 <= a.b ? 1 : a.b == 1 ? w.goal : 4LL * ((w.goal + a.b - 1) / a.b);
+        const long long s = a.num_splits > 1 ? a.num_splits + 1LL   // (cuts at its average length: one part more than cuts)
+                            : a.num_splits == 1 || w.goal * 4 <= a.b ? 1 : a.b == 1 ? w.goal : 4LL * ((w.goal + a.b - 1) / a.b);
         w.dec_splits = (int)std::max(1LL, std::min({s, most, 128LL}));
-        if ((long long)a.b * (a.seqlen_k / 32 + 1) > 0x7fffffff) w.dec_splits = 1;   // (the device adds the steps up in 32 bits)
-        // (a count given: the grid holds that many parts of every sequence)
-        w.grid = (int)std::min<long long>(0x7fffffff, a.num_splits > 0 ? (long long)a.b * w.dec_splits : std::max(w.goal, a.b));
-        if (a.num_splits > 0) w.goal = w.grid;
+        if (a.num_splits > 1) w.goal = (int)std::min<long long>(1 << 24, (long long)a.b * a.num_splits);
+        if (a.b * (16LL * (a.seqlen_k / 32 + 5)) > 1 << 30) w.dec_splits = 1;   // (the device adds the steps up in 32 bits)
+        w.grid = std::max(w.goal, a.b);
         if (w.dec_splits > 1) {
             const size_t n = (size_t)w.dec_splits * a.b * a.h * w.dec_sq;
             w.o = take(n * a.d * sizeof(float));

@@ -24,6 +24,7 @@ namespace vfa {
 
 constexpr int A_NW = 8, A_NT = A_NW * 64;
 constexpr int A_STEP = 32;                   // keys of a step
+constexpr long long VFA_KV8_LONG = 512LL << 20;   // bytes of codes of a launch that streams for long
 constexpr int A_MIN_STEPS = 3;               // least steps of a wave in a part of the keys
 
 template <int DP, int NR>
@@ -78,6 +79,17 @@ __host__ __device__ constexpr int kv8_swz(int row) {
     else return (row & 7) | ((row >> 4) & 1) << 3;
 }
 
+// Steps of 32 keys of sequence i that the rows from q0 on see, about; -1: it has no such rows, or is not this launch's.
+template <int NR>
+__device__ __forceinline__ int kv8_steps(const KV8Params &a, int i, int q0) {
+    const KParams &p = a.p;
+    if (i >= p.b) return -1;
+    const int span = p.is_local ? (min(p.wl, a.cap) + min(p.wr, a.cap) + 16 * NR) / A_STEP + 2 : 1 << 30;
+    const int len = min(kv8_cached(a, i) + (p.knew ? p.seqlen_knew : 0), a.cap);
+    const int rows = (p.cu_seqlens_q ? p.cu_seqlens_q[i + 1] - p.cu_seqlens_q[i] : p.seqlen_q) * p.h_ratio;
+    return rows > q0 && !(a.max_rows > 0 && rows > a.max_rows) ? min((len + A_STEP - 1) / A_STEP, span) : -1;
+}
+
 // Columns from p.d to DP are zero in Q; a lane whose columns lie there reads column 0 of its key instead (a
 // finite code times zero, or a NaN that the key has anyway), its O is never stored.
 //
@@ -86,12 +98,11 @@ __host__ __device__ constexpr int kv8_swz(int row) {
 // NT: the codes are loaded past the caches.  For streams that the 256 MiB last-level cache cannot hold anyway
 // (b128 kv8192 h32/8 d128: 5.85 -> 6.23 TB/s); shorter ones find part of it there (b1 kv65536: 37 against 50 us).
 //
-// The keys of a sequence are cut into parts for separate workgroups when there are too few (sequence, head group,
-// row block) items for the chip.  How many is decided here, from the lengths of all sequences: parts of equal
-// length, so that a batch of long and short sequences fills the chip evenly.
-template <int DP, bool BF16, int NR, bool PAGED, bool NT>
+// A launch of too few (sequence, head group, row block) items to fill the chip evenly is cut along the keys, by the
+// lengths of all sequences, which only the device knows.
+template <int DP, bool BF16, int NR, bool PAGED, bool NT, bool RUNS>
 __global__ void __launch_bounds__(A_NT, (DP == 64 && NR == 1) ? 4 : 2)
-fwd_kv8_kernel(const KV8Params a, const int n_mblocks) {
+fwd_kv8_kernel(const KV8Params args, const int n_mblocks) {
     using Cfg = Kv8Cfg<DP, NR>;
     constexpr int NBUF = DP == 64 || (DP == 128 && NR == 1) ? 2 : 1;   // (more do not leave the registers: d 128, 32 rows 166 -> 163 us)
     touch_kv8_args();
@@ -100,13 +111,6 @@ fwd_kv8_kernel(const KV8Params a, const int n_mblocks) {
     constexpr int CPR = DP / 16;             // 16-byte chunks of a V row
     constexpr int NV = A_STEP * CPR / 64;    // V loads per lane and step
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    const KParams &p = a.p;
-
-    const int tid = threadIdx.x, lane = tid & 63;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int c = lane & 15, g = lane >> 4;
-    const int hpw = a.heads_per_wg, hpw_sh = __builtin_ctz(hpw), parts = A_NW >> hpw_sh;   // (powers of two)
-    const int whead = wave & (hpw - 1), part = wave >> hpw_sh;
 
     // row blocks of the same keys on one XCD, whose L2 they share
     int L = blockIdx.x;
@@ -117,33 +121,47 @@ fwd_kv8_kernel(const KV8Params a, const int n_mblocks) {
             L = k / n_mblocks * group + L % 8 * n_mblocks + k % n_mblocks;
         }
     }
-    const int n_hblocks = p.h_k >> hpw_sh;
+    const int hpw = args.heads_per_wg, hpw_sh = __builtin_ctz(hpw), parts = A_NW >> hpw_sh;   // (powers of two)
+    const int n_hblocks = args.p.h_k >> hpw_sh;
     const int m_block = L % n_mblocks; L /= n_mblocks;
     const int hblock = L % n_hblocks; L /= n_hblocks;
-    const int hk = hblock * hpw + whead;
-    const int ratio = p.h_ratio;
     const int q0 = m_block * 16 * NR;
 
-    // L -> (sequence, part of its keys)
-    int bidb = L, split = 0, nsplit = 1;
-    if (p.num_splits > 1) {
-        // steps of sequence i as this row block sees them, about; -1: not this launch's
-        const int span = p.is_local ? (min(p.wl, a.cap) + min(p.wr, a.cap) + 16 * NR) / A_STEP + 2 : 1 << 30;
-        auto steps_of = [&](int i) -> int {
-            if (i >= p.b) return -1;
-            const int len = min(kv8_cached(a, i) + (p.knew ? p.seqlen_knew : 0), a.cap);
-            const int qi = (p.cu_seqlens_q ? p.cu_seqlens_q[i + 1] - p.cu_seqlens_q[i] : p.seqlen_q) * ratio;
-            return qi > q0 && !(a.max_rows > 0 && qi > a.max_rows) ? min((len + A_STEP - 1) / A_STEP, span) : -1;
-        };
+    // ---- L -> its sequence; or, where keys are cut into parts, what it has of them ----
+    // Every wave works this out for itself, a lane a sequence (64 at a time): no barrier.
+    // Usually a workgroup has one part, and a sequence's parts are of equal length.  Steps of a part: the total over the
+    // goal, less about half a part that every sequence leaves over; if the parts then are more than the goal after all
+    // (a second round of workgroups), less a whole one each.
+    // RUNS: where that leaves much of the chip idle (65 sequences to 128 workgroups: one each), a workgroup has an equal
+    // run of all sequences' steps instead, across their ends: their weights (steps, and what a piece of work costs beside
+    // them) stand in a row, cut at every multiple of `run`.  A cut within `edge` of a sequence's end moves there.  All in
+    // 1/16 steps.
+    constexpr int U = 16;
+    const bool cut = args.p.num_splits > 1;
+    const int few = A_MIN_STEPS * parts, edge = U * few / 2;
+    int bidb0 = L, split0 = 0, nsplit0 = 1;
+    bool runs = false;
+    int run = 1, chunk = 0, before = 0, at_w = 0, at_s = 0;
+    uint64_t hits = 0;                       // sequences of this chunk that the workgroup has a piece of
+    auto weight_of = [&](int st) -> int { return st < 0 ? 0 : U * (st + few / 2); };
+    // the cuts inside a sequence (weight w, at s in the row) are numbers first .. last; its parts are their workgroups'
+    // and the one's before
+    auto first_cut = [&](int s) -> int { return (s + edge + run - 1) / run; };
+    auto last_cut = [&](int s, int w) -> int { return w < 2 * edge ? first_cut(s) - 1 : (s + w - edge) / run; };
+    auto place = [&]() __attribute__((always_inline)) {
+        const int upto = wave_scan<false>(at_w);
+        at_s = before + upto - at_w;
+        before += __builtin_amdgcn_readlane(upto, 63);
+        const int lo = first_cut(at_s), hi = last_cut(at_s, at_w), whole = (at_s + at_w / 2) / run;
+        hits = __ballot(at_w > 0 && (hi < lo ? L == whole : L >= lo - 1 && L <= hi));
+    };
+    if (cut) {
+        const int lane = threadIdx.x & 63;
         auto parts_of = [](int st, int part_steps) -> int { return st < 0 ? 0 : max(1, (st + part_steps - 1) / part_steps); };
-        // Every wave works this out for itself, a lane a sequence (64 at a time): no barrier.  Steps of a part: the
-        // total over the goal, less about half a part that every sequence leaves over; if the parts then are more
-        // than the goal after all (a second round of workgroups), less a whole one each.  Not so few that a
-        // sequence needs more parts than there is scratch for.
-        const int st0 = steps_of(lane);
+        const int st0 = kv8_steps<NR>(args, lane, q0);
         int sum = max(st0, 0), top = sum, some = st0 >= 0;
-        for (int i = lane + 64; i < p.b; i += 64) {
-            const int st = steps_of(i);
+        for (int i = lane + 64; i < args.p.b; i += 64) {
+            const int st = kv8_steps<NR>(args, i, q0);
             sum += max(st, 0);
             top = max(top, st);
             some += st >= 0;
@@ -151,32 +169,87 @@ fwd_kv8_kernel(const KV8Params a, const int n_mblocks) {
         sum = wave_total(sum);
         some = wave_total(some);
         top = wave_top(top);
-        const int least = max((top + p.num_splits - 1) / p.num_splits, A_MIN_STEPS * parts);
-        int part_steps = max((sum - 1) / max(a.split_goal - some / 2, 1) + 1, least);
+        // (no more parts of one sequence than there is scratch for)
+        const int least = max((top + args.p.num_splits - 1) / args.p.num_splits, few);
+        int part_steps = max((sum - 1) / max(args.split_goal - some / 2, 1) + 1, least);
         if (some > 1) {
             int n = parts_of(st0, part_steps);
-            for (int i = lane + 64; i < p.b; i += 64) n += parts_of(steps_of(i), part_steps);
-            if (wave_total(n) > a.split_goal)
-                part_steps = a.split_goal > some ? max((sum - 1) / (a.split_goal - some) + 1, least) : max(top, 1);
+            for (int i = lane + 64; i < args.p.b; i += 64) n += parts_of(kv8_steps<NR>(args, i, q0), part_steps);
+            if (wave_total(n) > args.split_goal)
+                part_steps = args.split_goal > some ? max((sum - 1) / (args.split_goal - some) + 1, least) : max(top, 1);
         }
-        // the sequence in whose run of parts L falls
-        int before = 0;
-        bidb = -1;
-        for (int i = lane; i - lane < p.b && bidb < 0; i += 64) {
-            const int mine = parts_of(i == lane ? st0 : steps_of(i), part_steps);
-            const int upto = wave_scan<false>(mine);
-            const uint64_t hit = __ballot(before + upto > L);
-            if (hit) {
-                const int at = __builtin_ctzll(hit);
-                bidb = i - lane + at;
-                nsplit = __builtin_amdgcn_readlane(mine, at);
-                split = L - before - (__builtin_amdgcn_readlane(upto, at) - nsplit);
+        if constexpr (RUNS) {
+            const int sum_w = U * (sum + some * (few / 2));
+            run = max((int)((float)sum_w / (float)args.split_goal) + (sum_w >> 20) + 1, U * few);   // (no less than exact)
+            if (args.p.num_splits < args.split_goal) run = max(run, (weight_of(top) - 2 * edge) / (args.p.num_splits - 1) + 1);
+            // (a second piece of work costs about as much as `few` steps; more sequences than workgroups: rounds of them)
+            const int rounds = some <= args.split_goal ? 1 : (some + args.split_goal - 1) / args.split_goal;
+            runs = U * (rounds * min(part_steps, top) - few) > run;
+            if (runs) {
+                if ((int64_t)L * run >= sum_w) return;   // fewer runs than workgroups
+                at_w = weight_of(st0);
+                place();
             }
-            before += __builtin_amdgcn_readlane(upto, 63);
         }
-        if (bidb < 0) return;                          // fewer parts than workgroups
-        if (tid == 0 && split == 0 && hblock == 0) a.n_split[bidb * n_mblocks + m_block] = nsplit;
+        if (!runs) {
+            // the sequence in whose row of parts L falls
+            int first = 0;
+            bidb0 = -1;
+            for (int i = lane; i - lane < args.p.b && bidb0 < 0; i += 64) {
+                const int mine = parts_of(i == lane ? st0 : kv8_steps<NR>(args, i, q0), part_steps);
+                const int upto = wave_scan<false>(mine);
+                const uint64_t hit = __ballot(first + upto > L);
+                if (hit) {
+                    const int at = __builtin_ctzll(hit);
+                    bidb0 = i - lane + at;
+                    nsplit0 = __builtin_amdgcn_readlane(mine, at);
+                    split0 = L - first - (__builtin_amdgcn_readlane(upto, at) - nsplit0);
+                }
+                first += __builtin_amdgcn_readlane(upto, 63);
+            }
+            if (bidb0 < 0) return;                        // fewer parts than workgroups
+        }
     }
+
+  for (;;) {
+    int tid = threadIdx.x;
+    const KV8Params *args_at = &args;
+    if constexpr (RUNS) {
+        // (nothing but the plan stays in registers from one piece to the next: the arguments and the lane's place are
+        // new to the compiler here, or it would keep all that depends on them, and spill)
+        const auto *at = (const __attribute__((address_space(4))) KV8Params *)__builtin_amdgcn_kernarg_segment_ptr();
+        asm volatile("" : "+s"(at), "+v"(tid));
+        args_at = (const KV8Params *)at;
+    }
+    const KV8Params &a = *args_at;
+    const KParams &p = a.p;
+    const int lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int c = lane & 15, g = lane >> 4;
+    const int whead = wave & (hpw - 1), part = wave >> hpw_sh;
+    const int hk = hblock * hpw + whead;
+    const int ratio = p.h_ratio;
+
+    int bidb = bidb0, split = split0, nsplit = nsplit0;
+    int r_lo = split, r_hi = split + 1, weight = nsplit;      // the part's ends inside its sequence, of `weight`
+    if (runs) {
+        while (hits == 0) {
+            chunk += 64;
+            if (chunk >= p.b || before - edge > (L + 1) * run) return;
+            at_w = weight_of(kv8_steps<NR>(a, chunk + lane, q0));
+            place();
+        }
+        const int at = __builtin_ctzll(hits);
+        hits &= hits - 1;
+        bidb = chunk + at;
+        weight = __builtin_amdgcn_readlane(at_w, at);
+        const int s = __builtin_amdgcn_readlane(at_s, at), lo = first_cut(s), hi = last_cut(s, weight);
+        nsplit = hi < lo ? 1 : hi - lo + 2;
+        split = hi < lo ? 0 : L - lo + 1;
+        r_lo = split == 0 ? 0 : L * run - s;
+        r_hi = split == nsplit - 1 ? weight : (L + 1) * run - s;
+    }
+    if (cut && tid == 0 && split == 0 && hblock == 0) a.n_split[bidb * n_mblocks + m_block] = nsplit;
     bidb = __builtin_amdgcn_readfirstlane(bidb);
     split = __builtin_amdgcn_readfirstlane(split);
     nsplit = __builtin_amdgcn_readfirstlane(nsplit);
@@ -186,7 +259,10 @@ fwd_kv8_kernel(const KV8Params a, const int n_mblocks) {
     const int sq = bi.sq;
     const int sk = min(kv8_cached(a, bidb) + (p.knew ? p.seqlen_knew : 0), a.cap);
     const int rows = min(sq, p.seqlen_q) * ratio;    // (results have places for seqlen_q positions)
-    if (q0 >= rows || (a.max_rows > 0 && rows > a.max_rows)) return;
+    if (q0 >= rows || (a.max_rows > 0 && rows > a.max_rows)) {
+        if (runs) continue;
+        return;
+    }
     const int pos_lo = q0 / ratio, pos_hi = min(rows - 1, q0 + 16 * NR - 1) / ratio;
 
     // keys that some row of the block sees, and this part of them
@@ -195,9 +271,10 @@ fwd_kv8_kernel(const KV8Params a, const int n_mblocks) {
     const int vis_hi = edge_r ? min(sk, pos_hi + 1 + sk - sq + p.wr) : sk;
     int n0 = vis_lo / A_STEP, n1 = vis_hi > vis_lo ? (vis_hi + A_STEP - 1) / A_STEP : n0;
     if (is_split) {
-        const int per = (n1 - n0 + nsplit - 1) / nsplit;
-        n0 += split * per;
-        n1 = min(n1, n0 + per);
+        const float per = (float)(n1 - n0) / (float)weight;
+        const int n_all = n1 - n0, lo = min(n_all, (int)((float)r_lo * per));
+        if (split < nsplit - 1) n1 = n0 + min(n_all, (int)((float)r_hi * per));
+        n0 += lo;
     }
 
     const unsigned short *qg = (const unsigned short *)p.q + bi.q_off(p.q_bs, p.q_rs, bidb);
@@ -223,6 +300,7 @@ fwd_kv8_kernel(const KV8Params a, const int n_mblocks) {
             }
             if (ch == 0) lse[stat_at(head, row)] = is_split ? -INFINITY : INFINITY;
         }
+        if (runs) continue;
         return;
     }
 
@@ -521,6 +599,9 @@ fwd_kv8_kernel(const KV8Params a, const int n_mblocks) {
             }
         }
     }
+    if (!runs) return;
+    __syncthreads();                              // the next part's V images overwrite these rows
+  }
 }
 
 // Merge of the parts of a row: LSE-weighted sum, in part order.  One workgroup per (sequence, head, query
@@ -603,14 +684,14 @@ int kv8_decode_rows(int d, int rows) { return d <= 128 && rows > 16 ? 32 : 16; }
 // Resident workgroups of 8 waves per CU: two where the kernel needs at most 128 registers, else one.
 int kv8_decode_wgs_per_cu(int d, int rows) { return d <= 64 && rows <= 16 ? 2 : 1; }
 
-template <int DP, bool BF16, int NR, bool PAGED, bool NT>
+template <int DP, bool BF16, int NR, bool PAGED, bool NT, bool RUNS = false>
 static hipError_t launch_kv8(const KV8Params &a, hipStream_t stream) {
     const KParams &p = a.p;
     const int n_mblocks = (a.acc_sq * p.h_ratio + 16 * NR - 1) / (16 * NR);
     const long long blocks = (long long)n_mblocks * (p.h_k / a.heads_per_wg) * (p.num_splits > 1 ? a.split_grid : p.b);
     if (blocks <= 0) return hipSuccess;
     if (blocks > 0x7fffffffLL) return hipErrorInvalidValue;
-    auto kern = fwd_kv8_kernel<DP, BF16, NR, PAGED, NT>;
+    auto kern = fwd_kv8_kernel<DP, BF16, NR, PAGED, NT, RUNS>;
     constexpr int lds = Kv8Cfg<DP, NR>::LDS_BYTES;
     static std::atomic<uint64_t> lds_set{0};
     if (hipError_t e = set_dyn_lds_once((const void *)kern, lds, lds_set); e != hipSuccess) return e;
@@ -622,21 +703,31 @@ static hipError_t launch_kv8(const KV8Params &a, hipStream_t stream) {
     return hipGetLastError();
 }
 
-template <int DP, bool BF16, int NR>
-static hipError_t launch_kv8_layout(const KV8Params &a, hipStream_t stream) {
+template <int DP, bool BF16, int NR, bool NT>
+static hipError_t launch_kv8_layout(const KV8Params &a, long long codes, hipStream_t stream) {
     const bool paged = a.p.block_table != nullptr;
-    if constexpr (DP == 128) {
-        // codes that the calls of a program can name at all: what the sequences may hold, or the pool
-        const long long codes = std::min((long long)a.p.b * a.cap, (long long)a.num_pages * a.page_rows) * a.p.h_k * a.p.d * 2;
-        if (codes > 512LL << 20) return paged ? launch_kv8<DP, BF16, NR, true, true>(a, stream) : launch_kv8<DP, BF16, NR, false, true>(a, stream);
-    }
-    return paged ? launch_kv8<DP, BF16, NR, true, false>(a, stream) : launch_kv8<DP, BF16, NR, false, false>(a, stream);
+    // Runs of steps (see the kernel) cost 2 us more before the first key; worth it where parts of equal length can leave
+    // a good part of the chip idle: two parts a sequence at most, or up to eight of long ones.  b4096 h32/8 d128, 64-row
+    // pages: b129 311 -> 196 us, b65 154 -> 107; b48 kv16384 320 -> 274; b20 42.5 (44 with runs).
+    // (In the 128 registers of head dim 64 the loop over pieces spills.)
+    if constexpr (DP > 64 || NR > 1)
+        if (a.p.num_splits > 1 && (a.p.b * 2 > a.split_goal || (a.p.b * 8 > a.split_goal && codes > VFA_KV8_LONG)))
+            return paged ? launch_kv8<DP, BF16, NR, true, NT, true>(a, stream) : launch_kv8<DP, BF16, NR, false, NT, true>(a, stream);
+    return paged ? launch_kv8<DP, BF16, NR, true, NT>(a, stream) : launch_kv8<DP, BF16, NR, false, NT>(a, stream);
+}
+template <int DP, bool BF16, int NR>
+static hipError_t launch_kv8_stream(const KV8Params &a, hipStream_t stream) {
+    // codes that the calls of a program can name at all: what the sequences may hold, or the pool
+    const long long codes = std::min((long long)a.p.b * a.cap, (long long)a.num_pages * a.page_rows) * a.p.h_k * a.p.d * 2;
+    if constexpr (DP == 128)
+        if (codes > VFA_KV8_LONG) return launch_kv8_layout<DP, BF16, NR, true>(a, codes, stream);
+    return launch_kv8_layout<DP, BF16, NR, false>(a, codes, stream);
 }
 template <int DP, bool BF16>
 static hipError_t launch_kv8_rows(const KV8Params &a, hipStream_t stream) {
     if constexpr (DP <= 128)
-        if (kv8_decode_rows(a.p.d, a.acc_sq * a.p.h_ratio) == 32) return launch_kv8_layout<DP, BF16, 2>(a, stream);
-    return launch_kv8_layout<DP, BF16, 1>(a, stream);
+        if (kv8_decode_rows(a.p.d, a.acc_sq * a.p.h_ratio) == 32) return launch_kv8_stream<DP, BF16, 2>(a, stream);
+    return launch_kv8_stream<DP, BF16, 1>(a, stream);
 }
 
 // Adjacent KV heads of a workgroup: a key's codes of one head are d bytes, and reads of 512 contiguous bytes
