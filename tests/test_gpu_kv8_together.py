@@ -400,6 +400,61 @@ def test_runs_of_keys_with_windows_and_new_tokens():
         assert torch.equal(first, _fa().flash_attn_with_quantized_kvcache(q.cuda(), *gpu, **args))
 
 
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("b,sq,h,hk,d,blk,page,lens,window,num_splits", [
+    (2, 1, 2, 2, 64, 16, 16, [700, 33], -1, 0),
+    (3, 2, 16, 4, 64, 32, 64, [0, 31, 1777], -1, 3),          # 8 rows a head
+    (2, 3, 4, 2, 48, 16, 0, [300, 2], 100, 1),                # fewer keys than queries
+    (2, 1, 16, 16, 16, 16, 32, [500, 129], 64, 0),
+    (1, 1, 42, 6, 64, 48, 48, [5000], -1, 0),                 # 7 rows; 3 pairs
+    (2, 2, 10, 2, 64, 16, 16, [400, 60], -1, 0),              # 10 rows: not in pairs
+    (2, 1, 3, 3, 64, 16, 16, [400, 60], -1, 0),               # an odd number of heads
+])
+def test_narrow_heads_in_pairs(b, sq, h, hk, d, blk, page, lens, window, num_splits, dtype):
+    cache = Cache(b, max(lens) + 20, hk, d, blk, page, seed=110)
+    slopes = torch.rand(h, generator=torch.Generator().manual_seed(111)) * 0.2 if d == 48 else None
+    _check(cache, lens, _q((b, sq, h, d), dtype, 112), dtype, causal=True, window=(window, -1), num_splits=num_splits, slopes=slopes)
+
+
+def test_a_nan_of_one_head_stays_out_of_its_neighbour():
+    for num_splits in (1, 3):
+        cache = Cache(2, 300, 4, 64, 16, 16, seed=113)
+        clean = cache.gpu()
+        q = _q((2, 1, 8, 64), "bf16", 114).cuda()
+        args = dict(cache_seqlens=torch.tensor([300, 200], dtype=torch.int32).cuda(), block_table=cache.block_table(), num_splits=num_splits)
+        want = _fa().flash_attn_with_quantized_kvcache(q, *clean, **args)
+        for which, head in ((0, 1), (1, 2), (0, 2), (1, 3)):
+            bad = [t.clone() for t in clean]
+            pg, row = cache.place(0, 150)
+            bad[which].view(torch.uint8)[pg, row, head] = 127
+            got = _fa().flash_attn_with_quantized_kvcache(q, *bad, **args)
+            hit = torch.zeros(2, 1, 8, dtype=torch.bool)
+            hit[0, :, 2 * head:2 * head + 2] = True
+            assert torch.isnan(got[hit.cuda()]).all() and torch.equal(got[~hit.cuda()], want[~hit.cuda()])
+        scaled = [t.clone() for t in clean]                  # and a NaN scale
+        scaled[2].view(torch.uint8)[pg, 0, 1] = 255
+        got = _fa().flash_attn_with_quantized_kvcache(q, *scaled, **args)
+        assert torch.isnan(got[0, :, 2:4]).all() and torch.equal(got[0, :, 4:], want[0, :, 4:]) and torch.equal(got[:, :, :2], want[:, :, :2])
+
+
+@pytest.mark.parametrize("h,hk,d", [(4, 2, 64), (8, 2, 128), (4, 2, 256), (40, 2, 64)])
+def test_caches_with_heads_outside_and_padded_rows(h, hk, d):
+    """A pool stored as (pages, heads, rows, headdim + padding): the same result as the plain layout."""
+    cache = Cache(3, 400, hk, d, 16, 32, seed=115)
+    plain, table = cache.gpu(), cache.block_table()
+    q = _q((3, 1, h, d), "fp16", 116).cuda()
+    args = dict(cache_seqlens=torch.tensor([400, 0, 77], dtype=torch.int32).cuda(), block_table=table)
+    n = plain[0].shape[0]
+    other = []
+    for t in plain[:2]:
+        wide = torch.full((n, hk, 32, d + 16), 127, dtype=torch.uint8, device="cuda")
+        wide[..., :d] = t.view(torch.uint8).transpose(1, 2)
+        other.append(wide[..., :d].transpose(1, 2).view(torch.float8_e4m3fn))
+    for t in plain[2:]:
+        other.append(t.view(torch.uint8).transpose(1, 2).contiguous().transpose(1, 2).view(torch.float8_e8m0fnu))
+    assert torch.equal(_fa().flash_attn_with_quantized_kvcache(q, *other, **args), _fa().flash_attn_with_quantized_kvcache(q, *plain, **args))
+
+
 def test_scales_at_the_ends_of_their_range():
     """Bytes 0 and 254 (2^-127, 2^127) and 255 (NaN): never written here, but what a cache from elsewhere can hold."""
     fa = _fa()

@@ -31,9 +31,10 @@ hipError_t run_bwd_dropout(const KParams &p, hipStream_t stream, hipEvent_t *sta
 hipError_t run_kv8_quantize(const KV8Params &a, hipStream_t stream);             // kv8_cache.hip
 hipError_t run_kv8_dequantize(const KV8Params &a, hipStream_t stream);
 hipError_t run_fwd_kv8(const KV8Params &a, hipStream_t stream);                  // fwd_kv8.hip
-int kv8_heads_per_wg(int d, int h_k);
+int kv8_heads_per_wg(int d, int h_k, bool pairs);
+bool kv8_pairs(int d, int h_k, int rows, int64_t k_hs, int64_t v_hs);
 int kv8_decode_rows(int d, int rows);
-int kv8_decode_wgs_per_cu(int d, int rows);
+int kv8_decode_wgs_per_cu(int d, int rows, bool pairs);
 hipError_t run_fwd_kv8_prefill(const KV8Params &a, hipStream_t stream);          // fwd_prefill_kv8.hip
 hipError_t run_qk_norm_rotary(const QKNormParams &p, bool bwd, hipStream_t stream);   // qk_norm_rotary.hip
 void qk_norm_blocks(QKNormParams &p, int cus, bool bwd);
@@ -632,6 +633,8 @@ struct Kv8Plan {
     bool decode, prefill, read_back;
     int dec_sq, dec_rows;        // most query positions and rows of a sequence of the decode kernel's
     int dec_splits, pre_splits;
+    int hpw;                     // decode: KV heads, or pairs of them, of a workgroup
+    bool pairs;
     int goal, grid;              // decode: parts of all sequences to aim at per head group and row block, the most there can be
     size_t o, lse, n_split;      // decode: offsets into the workspace
     size_t pre_o, pre_lse;       // prefill
@@ -654,15 +657,17 @@ static int kv8_plan(const vfa_kv8_params *p, Kv8Plan &w) {
     size_t at = 0;
     auto take = [&](size_t bytes) { const size_t o = at; at += (bytes + 255) / 256 * 256; return o; };
     if (w.decode) {
-        const int hpw = vfa::kv8_heads_per_wg(a.d, a.h_k), parts = 8 / hpw;
+        w.pairs = vfa::kv8_pairs(a.d, a.h_k, w.dec_sq * ratio, a.k_head_stride, a.v_head_stride);
+        w.hpw = vfa::kv8_heads_per_wg(a.d, a.h_k, w.pairs);
+        const int parts = 8 / w.hpw;
         const int per = vfa::kv8_decode_rows(a.d, w.dec_sq * ratio);
         const int mblocks = (w.dec_sq * ratio + per - 1) / per;
-        const long long items = (long long)a.b * (a.h_k / hpw) * mblocks;
+        const long long items = (long long)a.b * ((w.pairs ? a.h_k / 2 : a.h_k) / w.hpw) * mblocks;
         // Parts of all sequences together: one workgroup each fills the device once.  A sequence may take up to four
         // times the average (their lengths can differ), as many as its keys allow.
         const int groups = (int)std::max(1LL, items / a.b);
         const long long most = std::max(1LL, (long long)a.seqlen_k / (32LL * 3 * parts));
-        w.goal = std::max(1, cus * vfa::kv8_decode_wgs_per_cu(a.d, w.dec_sq * ratio) / groups);
+        w.goal = std::max(1, cus * vfa::kv8_decode_wgs_per_cu(a.d, w.dec_sq * ratio, w.pairs) / groups);
         const long long s = a.num_splits > 1 ? a.num_splits + 1LL   // (cuts at its average length: one part more than cuts)
                             : a.num_splits == 1 || w.goal * 4 <= a.b ? 1 : a.b == 1 ? w.goal : 4LL * ((w.goal + a.b - 1) / a.b);
         w.dec_splits = (int)std::max(1LL, std::min({s, most, 128LL}));
@@ -785,7 +790,8 @@ extern "C" int vfa_kv8_mha_fwd(const vfa_kv8_params *p) {
         if (e != hipSuccess) return hip_fail(e, "kv8 prefill launch");
     }
     if (w.decode) {   // (after the 16-bit kernels, which write zeros for the sequences that are not theirs)
-        k.heads_per_wg = vfa::kv8_heads_per_wg(a.d, a.h_k);
+        k.heads_per_wg = w.hpw;
+        k.pairs = w.pairs;
         k.max_rows = w.prefill ? w.dec_rows : 0;
         k.acc_sq = w.dec_sq;
         k.p.num_splits = w.dec_splits;

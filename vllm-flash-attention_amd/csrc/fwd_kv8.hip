@@ -90,6 +90,11 @@ __device__ __forceinline__ int kv8_steps(const KV8Params &a, int i, int q0) {
     return rows > q0 && !(a.max_rows > 0 && rows > a.max_rows) ? min((len + A_STEP - 1) / A_STEP, span) : -1;
 }
 
+// PAIR: two adjacent heads of at most 64 columns and 8 rows share a wave.  They take the 16 columns of Q^T between
+// them and each a half of the 128 columns of K and V, whose rows then are whole 128-byte lines: as head dim 64 alone,
+// waves that request half a line each, the kernel reaches 4.6 TB/s.  A column's scores come from its own head's product
+// (the other one's is dropped, not added as zeros: a NaN of one head stays out of the other).
+//
 // Columns from p.d to DP are zero in Q; a lane whose columns lie there reads column 0 of its key instead (a
 // finite code times zero, or a NaN that the key has anyway), its O is never stored.
 //
@@ -100,7 +105,7 @@ __device__ __forceinline__ int kv8_steps(const KV8Params &a, int i, int q0) {
 //
 // A launch of too few (sequence, head group, row block) items to fill the chip evenly is cut along the keys, by the
 // lengths of all sequences, which only the device knows.
-template <int DP, bool BF16, int NR, bool PAGED, bool NT, bool RUNS>
+template <int DP, bool BF16, int NR, bool PAGED, bool NT, bool RUNS, bool PAIR>
 __global__ void __launch_bounds__(A_NT, (DP == 64 && NR == 1) ? 4 : 2)
 fwd_kv8_kernel(const KV8Params args, const int n_mblocks) {
     using Cfg = Kv8Cfg<DP, NR>;
@@ -108,6 +113,9 @@ fwd_kv8_kernel(const KV8Params args, const int n_mblocks) {
     touch_kv8_args();
     constexpr int NJ = DP / 64;              // 64-column groups of K: one 16-byte load per lane and key tile
     constexpr int NDB = DP / 16;             // 16-column blocks of O
+    constexpr int HD = PAIR ? DP / 2 : DP;   // columns of a head
+    constexpr int HR = PAIR ? 8 : 16 * NR;   // its rows in a workgroup
+    static_assert(!PAIR || (DP == 128 && NR == 1), "");
     constexpr int CPR = DP / 16;             // 16-byte chunks of a V row
     constexpr int NV = A_STEP * CPR / 64;    // V loads per lane and step
     extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -122,7 +130,7 @@ fwd_kv8_kernel(const KV8Params args, const int n_mblocks) {
         }
     }
     const int hpw = args.heads_per_wg, hpw_sh = __builtin_ctz(hpw), parts = A_NW >> hpw_sh;   // (powers of two)
-    const int n_hblocks = args.p.h_k >> hpw_sh;
+    const int n_hblocks = (PAIR ? args.p.h_k >> 1 : args.p.h_k) >> hpw_sh;
     const int m_block = L % n_mblocks; L /= n_mblocks;
     const int hblock = L % n_hblocks; L /= n_hblocks;
     const int q0 = m_block * 16 * NR;
@@ -227,7 +235,7 @@ fwd_kv8_kernel(const KV8Params args, const int n_mblocks) {
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int c = lane & 15, g = lane >> 4;
     const int whead = wave & (hpw - 1), part = wave >> hpw_sh;
-    const int hk = hblock * hpw + whead;
+    const int hk = (hblock * hpw + whead) * (PAIR ? 2 : 1);
     const int ratio = p.h_ratio;
 
     int bidb = bidb0, split = split0, nsplit = nsplit0;
@@ -287,8 +295,8 @@ fwd_kv8_kernel(const KV8Params args, const int n_mblocks) {
     float *lse = is_split ? p.lseaccum : p.lse;
 
     if (n1 <= n0) {
-        for (int i = tid; i < hpw * 16 * NR * (DP / 8); i += A_NT) {
-            const int ch = i % (DP / 8), rr = i / (DP / 8) % (16 * NR), head = hblock * hpw + i / (DP / 8) / (16 * NR);
+        for (int i = tid; i < hpw * 16 * NR * (HD / 8); i += A_NT) {
+            const int ch = i % (HD / 8), rr = i / (HD / 8) % HR, head = hblock * hpw * (PAIR ? 2 : 1) + i / (HD / 8) / HR;
             const int row = q0 + rr;
             if (row >= rows || ch * 8 >= p.d) continue;
             if (is_split) {
@@ -316,19 +324,20 @@ fwd_kv8_kernel(const KV8Params args, const int n_mblocks) {
     const int first = n0 + part;
     load_pages(min(first, n1 - 1));      // (in front of Q: the first rows wait for these)
 
-    // Q operand: columns 64 j + 16 g + 8 s .. of k-step 2 j + s
-    i32x4 qf[NR][2 * NJ];
+    // Q operand: columns 64 j + 16 g + 8 s .. of k-step 2 j + s (PAIR: of both heads' k-steps s)
+    constexpr int NQ = PAIR ? 2 : 2 * NJ;
+    i32x4 qf[NR][NQ];
     int pos[NR];
     float slope[NR];
 #pragma unroll
     for (int r = 0; r < NR; r++) {
-        const int row = min(q0 + 16 * r + c, rows - 1);
+        const int row = min(PAIR ? c & 7 : q0 + 16 * r + c, rows - 1);
         pos[r] = row / ratio;
-        const int head = hk * ratio + row % ratio;
+        const int head = (hk + (PAIR ? c >> 3 : 0)) * ratio + row % ratio;
         slope[r] = p.alibi_slopes ? p.alibi_slopes[(int64_t)bidb * p.alibi_bs + head] / p.scale : 0.f;
         const unsigned short *qr = qg + (int64_t)pos[r] * p.q_rs + (int64_t)head * p.q_hs;
 #pragma unroll
-        for (int s = 0; s < 2 * NJ; s++) {
+        for (int s = 0; s < NQ; s++) {
             const int col = 64 * (s >> 1) + 16 * g + 8 * (s & 1);
             qf[r][s] = col < p.d ? *(const i32x4 *)(qr + col) : i32x4{0, 0, 0, 0};
         }
@@ -338,11 +347,14 @@ fwd_kv8_kernel(const KV8Params args, const int n_mblocks) {
     // lane offsets inside a tile of 16 keys: K 16 columns of key c, V chunk lane + 64 i
     unsigned koff[NJ], voff[NV / 2];
 #pragma unroll
-    for (int j = 0; j < NJ; j++) koff[j] = (unsigned)(c * k_rs + (64 * j + 16 * g < p.d ? 64 * j + 16 * g : 0));
+    for (int j = 0; j < NJ; j++) {
+        const int col = (PAIR ? 0 : 64 * j) + 16 * g;
+        koff[j] = (unsigned)(c * k_rs + (PAIR ? j * (int)p.k_hs : 0) + (col < p.d ? col : 0));
+    }
 #pragma unroll
     for (int i = 0; i < NV / 2; i++) {
-        const int ci = lane + 64 * i, vc = ci % CPR * 16;
-        voff[i] = (unsigned)(ci / CPR * v_rs + (vc < p.d ? vc : 0));
+        const int ci = lane + 64 * i, vc = ci % CPR * 16 % HD;
+        voff[i] = (unsigned)(ci / CPR * v_rs + (PAIR ? ci % CPR * 16 / HD * (int)p.v_hs : 0) + (vc < p.d ? vc : 0));
     }
 
     // A step needs eight addresses: of K, V and their scales, for its two tiles.  Lane i of every eight works out
@@ -350,9 +362,10 @@ fwd_kv8_kernel(const KV8Params args, const int n_mblocks) {
     // scales fetched by the lanes that hold theirs.  (As scalar arithmetic this was a third of the step's
     // instructions, and few-wave launches are bound by those.)
     const int sel = (lane >> 1) & 3;
+    const int sc_head = hk + (PAIR ? (lane >> 3) & 1 : 0);   // (PAIR: the second eight fetch the second head's scales)
     const unsigned char *lbase = sel == 0 ? (const unsigned char *)p.k + (int64_t)hk * p.k_hs
                                : sel == 1 ? (const unsigned char *)p.v + (int64_t)hk * p.v_hs
-                               : sel == 2 ? a.ks + (int64_t)hk * a.ks_hs : a.vs + (int64_t)hk * a.vs_hs;
+                               : sel == 2 ? a.ks + (int64_t)sc_head * a.ks_hs : a.vs + (int64_t)sc_head * a.vs_hs;
     const int64_t lps = sel == 0 ? p.k_bs : sel == 1 ? p.v_bs : sel == 2 ? a.ks_bs : a.vs_bs;
     const unsigned lrs = (unsigned)(sel == 0 ? p.k_rs : sel == 1 ? p.v_rs : sel == 2 ? a.ks_rs : a.vs_rs);
 
@@ -422,11 +435,12 @@ fwd_kv8_kernel(const KV8Params args, const int n_mblocks) {
 
     auto step = [&](const int n, Set &w, const int next) __attribute__((always_inline)) {
         const int k0 = n * A_STEP;
-        float sc[4];
+        float sc[PAIR ? 2 : 1][4];
         const int scl = (int)(w.sc | w.bad);
 #pragma unroll
-        for (int i = 0; i < 4; i++) sc[i] = e8m0_to_f32((unsigned)__builtin_amdgcn_readlane(scl, 4 + i));
-        const float *ks = sc, *vs = sc + 2;
+        for (int i = 0; i < 4; i++)
+#pragma unroll
+            for (int e = 0; e < (PAIR ? 2 : 1); e++) sc[e][i] = e8m0_to_f32((unsigned)__builtin_amdgcn_readlane(scl, 4 + i + 8 * e));
         f32x4 s[NR][2];
 #pragma unroll
         for (int t = 0; t < 2; t++) {
@@ -434,12 +448,21 @@ fwd_kv8_kernel(const KV8Params args, const int n_mblocks) {
             for (int r = 0; r < NR; r++) s[r][t] = f32x4{0, 0, 0, 0};
 #pragma unroll
             for (int j = 0; j < NJ; j++) {
-                const i32x4 k_lo = kv8_to16<BF16>(i32x2{w.k[t][j][0], w.k[t][j][1]}, ks[t]);
-                const i32x4 k_hi = kv8_to16<BF16>(i32x2{w.k[t][j][2], w.k[t][j][3]}, ks[t]);
+                const float ks = sc[PAIR ? j : 0][t];
+                const i32x4 k_lo = kv8_to16<BF16>(i32x2{w.k[t][j][0], w.k[t][j][1]}, ks);
+                const i32x4 k_hi = kv8_to16<BF16>(i32x2{w.k[t][j][2], w.k[t][j][3]}, ks);
+                if constexpr (PAIR) {    // each head's keys against all 16 columns; a column takes its own head's
+                    f32x4 x = {0, 0, 0, 0};
+                    x = mma16<BF16>(k_lo, qf[0][0], x);
+                    x = mma16<BF16>(k_hi, qf[0][1], x);
 #pragma unroll
-                for (int r = 0; r < NR; r++) {
-                    s[r][t] = mma16<BF16>(k_lo, qf[r][2 * j], s[r][t]);
-                    s[r][t] = mma16<BF16>(k_hi, qf[r][2 * j + 1], s[r][t]);
+                    for (int i = 0; i < 4; i++) s[0][t][i] = j == 0 ? x[i] : c < 8 ? s[0][t][i] : x[i];
+                } else {
+#pragma unroll
+                    for (int r = 0; r < NR; r++) {
+                        s[r][t] = mma16<BF16>(k_lo, qf[r][2 * j], s[r][t]);
+                        s[r][t] = mma16<BF16>(k_hi, qf[r][2 * j + 1], s[r][t]);
+                    }
                 }
             }
         }
@@ -522,6 +545,7 @@ fwd_kv8_kernel(const KV8Params args, const int n_mblocks) {
             const i32x2 vt = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
                 (__attribute__((address_space(3))) i32x2 *)(tr_base + ((db << 4) ^ tr_swz)));
             i32x4 vf;
+            const float *vs = sc[PAIR ? db * 16 / HD : 0] + 2;
             const i32x4 lo = kv8_to16<BF16>(i32x2{vt[0], 0}, vs[0]), hi = kv8_to16<BF16>(i32x2{vt[1], 0}, vs[1]);
             vf[0] = lo[0]; vf[1] = lo[1]; vf[2] = hi[0]; vf[3] = hi[1];
 #pragma unroll
@@ -571,18 +595,18 @@ fwd_kv8_kernel(const KV8Params args, const int n_mblocks) {
         char *ob = smem + wave * 16 * Cfg::O_ROWB + c * Cfg::O_ROWB + g * 16;
 #pragma unroll
         for (int db = 0; db < NDB; db++) *(f32x4 *)(ob + db * 64) = o[r][db] * f;
-        const int row = q0 + 16 * r + c;
+        const int row = PAIR ? c & 7 : q0 + 16 * r + c;
         if (part == 0 && g == 0 && row < rows)
-            lse[stat_at(hk, row)] = none ? (is_split ? -INFINITY : INFINITY) : m_all * p.scale + __logf(l_all);
+            lse[stat_at(hk + (PAIR ? c >> 3 : 0), row)] = none ? (is_split ? -INFINITY : INFINITY) : m_all * p.scale + __logf(l_all);
         __syncthreads();
-        const int live = min(16, rows - (q0 + 16 * r));           // rows of this 16 that exist
-        for (int i = tid; i < hpw * live * (DP / 8); i += A_NT) {
-            const int ch = i % (DP / 8), j = i / (DP / 8), hs = j & (hpw - 1), rr = j >> hpw_sh;
-            if (ch * 8 >= p.d) continue;
-            const int orow = q0 + 16 * r + rr, head = hblock * hpw + hs;
+        const int live = PAIR ? 16 : min(16, rows - (q0 + 16 * r));           // rows of this 16 that exist
+        for (int i = tid; i < hpw * live * (HD / 8); i += A_NT) {
+            const int ch = i % (HD / 8), j = i / (HD / 8), hs = j & (hpw - 1), rr = j >> hpw_sh;
+            const int orow = PAIR ? rr & 7 : q0 + 16 * r + rr, head = PAIR ? 2 * (hblock * hpw + hs) + (rr >> 3) : hblock * hpw + hs;
+            if (ch * 8 >= p.d || (PAIR && orow >= rows)) continue;
             f32x4 a0 = {0, 0, 0, 0}, a1 = {0, 0, 0, 0};
             for (int w = 0; w < parts; w++) {
-                const char *src = smem + ((w * hpw + hs) * 16 + rr) * Cfg::O_ROWB + ch * 32;
+                const char *src = smem + ((w * hpw + hs) * 16 + rr) * Cfg::O_ROWB + (PAIR ? (rr >> 3) * HD * 4 : 0) + ch * 32;
                 a0 += *(const f32x4 *)src;
                 a1 += *(const f32x4 *)(src + 16);
             }
@@ -682,16 +706,16 @@ kv8_combine_kernel(const KV8Params a, const int n_mblocks, const int rows_per_bl
 int kv8_decode_rows(int d, int rows) { return d <= 128 && rows > 16 ? 32 : 16; }
 
 // Resident workgroups of 8 waves per CU: two where the kernel needs at most 128 registers, else one.
-int kv8_decode_wgs_per_cu(int d, int rows) { return d <= 64 && rows <= 16 ? 2 : 1; }
+int kv8_decode_wgs_per_cu(int d, int rows, bool pairs) { return d <= 64 && rows <= 16 && !pairs ? 2 : 1; }
 
-template <int DP, bool BF16, int NR, bool PAGED, bool NT, bool RUNS = false>
+template <int DP, bool BF16, int NR, bool PAGED, bool NT, bool PAIR, bool RUNS = false>
 static hipError_t launch_kv8(const KV8Params &a, hipStream_t stream) {
     const KParams &p = a.p;
     const int n_mblocks = (a.acc_sq * p.h_ratio + 16 * NR - 1) / (16 * NR);
-    const long long blocks = (long long)n_mblocks * (p.h_k / a.heads_per_wg) * (p.num_splits > 1 ? a.split_grid : p.b);
+    const long long blocks = (long long)n_mblocks * ((PAIR ? p.h_k / 2 : p.h_k) / a.heads_per_wg) * (p.num_splits > 1 ? a.split_grid : p.b);
     if (blocks <= 0) return hipSuccess;
     if (blocks > 0x7fffffffLL) return hipErrorInvalidValue;
-    auto kern = fwd_kv8_kernel<DP, BF16, NR, PAGED, NT, RUNS>;
+    auto kern = fwd_kv8_kernel<DP, BF16, NR, PAGED, NT, RUNS, PAIR>;
     constexpr int lds = Kv8Cfg<DP, NR>::LDS_BYTES;
     static std::atomic<uint64_t> lds_set{0};
     if (hipError_t e = set_dyn_lds_once((const void *)kern, lds, lds_set); e != hipSuccess) return e;
@@ -703,7 +727,7 @@ static hipError_t launch_kv8(const KV8Params &a, hipStream_t stream) {
     return hipGetLastError();
 }
 
-template <int DP, bool BF16, int NR, bool NT>
+template <int DP, bool BF16, int NR, bool NT, bool PAIR = false>
 static hipError_t launch_kv8_layout(const KV8Params &a, long long codes, hipStream_t stream) {
     const bool paged = a.p.block_table != nullptr;
     // Runs of steps (see the kernel) cost 2 us more before the first key; worth it where parts of equal length can leave
@@ -712,16 +736,16 @@ static hipError_t launch_kv8_layout(const KV8Params &a, long long codes, hipStre
     // (In the 128 registers of head dim 64 the loop over pieces spills.)
     if constexpr (DP > 64 || NR > 1)
         if (a.p.num_splits > 1 && (a.p.b * 2 > a.split_goal || (a.p.b * 8 > a.split_goal && codes > VFA_KV8_LONG)))
-            return paged ? launch_kv8<DP, BF16, NR, true, NT, true>(a, stream) : launch_kv8<DP, BF16, NR, false, NT, true>(a, stream);
-    return paged ? launch_kv8<DP, BF16, NR, true, NT>(a, stream) : launch_kv8<DP, BF16, NR, false, NT>(a, stream);
+            return paged ? launch_kv8<DP, BF16, NR, true, NT, PAIR, true>(a, stream) : launch_kv8<DP, BF16, NR, false, NT, PAIR, true>(a, stream);
+    return paged ? launch_kv8<DP, BF16, NR, true, NT, PAIR>(a, stream) : launch_kv8<DP, BF16, NR, false, NT, PAIR>(a, stream);
 }
-template <int DP, bool BF16, int NR>
+template <int DP, bool BF16, int NR, bool PAIR = false>
 static hipError_t launch_kv8_stream(const KV8Params &a, hipStream_t stream) {
     // codes that the calls of a program can name at all: what the sequences may hold, or the pool
     const long long codes = std::min((long long)a.p.b * a.cap, (long long)a.num_pages * a.page_rows) * a.p.h_k * a.p.d * 2;
     if constexpr (DP == 128)
-        if (codes > VFA_KV8_LONG) return launch_kv8_layout<DP, BF16, NR, true>(a, codes, stream);
-    return launch_kv8_layout<DP, BF16, NR, false>(a, codes, stream);
+        if (codes > VFA_KV8_LONG) return launch_kv8_layout<DP, BF16, NR, true, PAIR>(a, codes, stream);
+    return launch_kv8_layout<DP, BF16, NR, false, PAIR>(a, codes, stream);
 }
 template <int DP, bool BF16>
 static hipError_t launch_kv8_rows(const KV8Params &a, hipStream_t stream) {
@@ -730,9 +754,15 @@ static hipError_t launch_kv8_rows(const KV8Params &a, hipStream_t stream) {
     return launch_kv8_stream<DP, BF16, 1>(a, stream);
 }
 
+// Whether adjacent KV heads of `rows` (query, head) rows each go in pairs (their codes in one buffer's 32-bit offsets).
+bool kv8_pairs(int d, int h_k, int rows, int64_t k_hs, int64_t v_hs) {
+    return d <= 64 && h_k % 2 == 0 && rows <= 8 && std::min(k_hs, v_hs) >= 0 && std::max(k_hs, v_hs) <= 1 << 30;
+}
+
 // Adjacent KV heads of a workgroup: a key's codes of one head are d bytes, and reads of 512 contiguous bytes
 // are what keeps HBM busy (b128 kv8192 h32/8 d128, heads 1 / 2 / 4: 465 / 391 / 374 us).
-int kv8_heads_per_wg(int d, int h_k) {
+int kv8_heads_per_wg(int d, int h_k, bool pairs) {   // (in pairs: of those)
+    if (pairs) d *= 2, h_k /= 2;
     int n = 1;
     while (n < 8 && n * d < 512 && h_k % (2 * n) == 0) n *= 2;
     return n;
@@ -740,6 +770,8 @@ int kv8_heads_per_wg(int d, int h_k) {
 
 hipError_t run_fwd_kv8(const KV8Params &a, hipStream_t stream) {
     const bool bf = a.p.is_bf16;
+    if (a.pairs)
+        return bf ? launch_kv8_stream<128, true, 1, true>(a, stream) : launch_kv8_stream<128, false, 1, true>(a, stream);
     if (a.p.d <= 64) return bf ? launch_kv8_rows<64, true>(a, stream) : launch_kv8_rows<64, false>(a, stream);
     if (a.p.d <= 128) return bf ? launch_kv8_rows<128, true>(a, stream) : launch_kv8_rows<128, false>(a, stream);
     return bf ? launch_kv8_rows<256, true>(a, stream) : launch_kv8_rows<256, false>(a, stream);

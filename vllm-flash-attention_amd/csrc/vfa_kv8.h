@@ -23,7 +23,8 @@ struct KV8Params {
     int page_rows;               // rows of a page; of a contiguous cache: its capacity
     int num_pages;               // pages; batch rows of a contiguous cache
     int cap;                     // most tokens a sequence can have
-    int heads_per_wg;            // attention: adjacent KV heads per workgroup (1, 2, 4, 8)
+    int heads_per_wg;            // attention: adjacent KV heads, or pairs of them, per workgroup (1, 2, 4, 8)
+    int pairs;                   // decode kernel: KV heads in pairs
     int max_rows;                // decode kernel: sequences with more (query, head) rows than this are another kernel's; 0: none are
     int min_rows;                // prefill kernel, reading back for it: the sequences with at most so many rows are the decode kernel's
     int split_goal;              // decode kernel: parts of the keys to aim at per head group and row block, over all sequences
