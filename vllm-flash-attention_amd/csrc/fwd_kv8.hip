@@ -628,31 +628,118 @@ fwd_kv8_kernel(const KV8Params args, const int n_mblocks) {
   }
 }
 
-// Merge of the parts of a row: LSE-weighted sum, in part order.  One workgroup per (sequence, head, query
-// position): 256 threads are (16-byte output chunk) x (lane over the parts); everything is requested up front.
+// Merge of the parts of a row: LSE-weighted sum, in part order.  Its arguments in two cache lines: they lie in host
+// memory, and the kernel is little else than its latency.
+struct Kv8Merge {
+    const float *o, *lse;
+    float *out_lse;
+    unsigned short *out;
+    const int *n_split, *cu_q;
+    int64_t out_bs, out_rs, out_hs;
+    int b, h, d, acc_sq, num_splits, seqlen_q, max_rows, ratio, n_mblocks, rows_per_block;
+};
+
+struct Kv8MergeRow {
+    int bidb, head, pos, n;        // n: parts, 0 where there is nothing to merge (one part is written in place)
+    int64_t rows, at;              // rows of a part, the row in it
+    __device__ __forceinline__ Kv8MergeRow(const Kv8Merge &a, int row) {
+        pos = row % a.acc_sq;
+        const int bh = row / a.acc_sq;
+        bidb = bh / a.h;
+        head = bh - bidb * a.h;
+        rows = (int64_t)a.b * a.h * a.acc_sq;
+        at = row;
+        n = a.n_split[bidb * a.n_mblocks + (pos * a.ratio + head % a.ratio) / a.rows_per_block];
+        const int sq = a.cu_q ? a.cu_q[bidb + 1] - a.cu_q[bidb] : a.seqlen_q;
+        if (pos >= sq || (a.max_rows > 0 && sq * a.ratio > a.max_rows) || n <= 1) n = 0;
+    }
+    __device__ __forceinline__ unsigned short *out(const Kv8Merge &a) const {
+        return a.out + (a.cu_q ? (int64_t)a.cu_q[bidb] * a.out_rs : bidb * a.out_bs) + (int64_t)head * a.out_hs + (int64_t)pos * a.out_rs;
+    }
+    __device__ __forceinline__ float *lse(const Kv8Merge &a) const { return a.out_lse + ((int64_t)bidb * a.h + head) * a.seqlen_q + pos; }
+};
+template <bool BF16>
+__device__ __forceinline__ void kv8_store8(unsigned short *to, f32x4 a0, f32x4 a1) {
+    i32x4 w;
+    w[0] = pack2<BF16>(a0[0], a0[1]); w[1] = pack2<BF16>(a0[2], a0[3]);
+    w[2] = pack2<BF16>(a1[0], a1[1]); w[3] = pack2<BF16>(a1[2], a1[3]);
+    *(i32x4 *)to = w;
+}
+
+// Up to 16 parts: a wave a row.  Lanes are (16-byte output chunk) x (lane over the parts); everything is requested before
+// the number of parts is known.
+constexpr int A_FEW_PARTS = 16;
 template <bool BF16>
 __global__ void __launch_bounds__(256)
-kv8_combine_kernel(const KV8Params a, const int n_mblocks, const int rows_per_block) {
-    const KParams &p = a.p;
+kv8_combine_few_kernel(const Kv8Merge a) {
+    const int lane = threadIdx.x & 63, row = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
+    if (row >= a.b * a.h * a.acc_sq) return;
+    const Kv8MergeRow r(a, row);
+    const int cpr = a.d / 8, nlane = min(4, 64 / cpr), ch = lane % cpr, sl = lane / cpr;   // (lanes past nlane * cpr idle)
+    const int top = a.num_splits - 1;
+    const float my_lse = a.lse[min(lane, top) * r.rows + r.at];
+    constexpr int PRE = A_FEW_PARTS / 2;     // (at head dim 256 two lanes share the parts, else three or four)
+    f32x4 x0[PRE], x1[PRE];
+#pragma unroll
+    for (int i = 0; i < PRE; i++) {
+        if (i * nlane > top) break;
+        const float *src = a.o + (min(sl + i * nlane, top) * r.rows + r.at) * a.d + ch * 8;
+        x0[i] = *(const f32x4 *)src;
+        x1[i] = *(const f32x4 *)(src + 4);
+    }
+    if (r.n == 0) return;
+    const float my = lane < r.n ? my_lse : -INFINITY;
+    float m = my;
+#pragma unroll
+    for (int off = 8; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor(m, off));   // (16 lanes hold them all)
+    m = __shfl(m, 0);
+    const float ref = m == -INFINITY ? 0.f : m;
+    const float e = lane < r.n ? expf(my - ref) : 0.f;
+    float sum = e;
+#pragma unroll
+    for (int off = 8; off > 0; off >>= 1) sum += __shfl_xor(sum, off);
+    sum = __shfl(sum, 0);
+    const bool none = sum == 0.f;                             // no part saw a key of this row
+    const float w = none ? 0.f : e / sum;
+    if (lane == 0) *r.lse(a) = none ? INFINITY : logf(sum) + ref;
+    f32x4 a0 = {0, 0, 0, 0}, a1 = {0, 0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < PRE; i++) {
+        if (i * nlane >= r.n) break;
+        const int sp = sl + i * nlane;
+        const float f = __shfl(w, sp & 63);
+        if (sl < nlane && sp < r.n) { a0 += x0[i] * f; a1 += x1[i] * f; }
+    }
+    for (int k = 1; k < nlane; k++) {
+        const int from = (lane + k * cpr) & 63;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const float y0 = __shfl(a0[i], from), y1 = __shfl(a1[i], from);
+            if (sl == 0) { a0[i] += y0; a1[i] += y1; }
+        }
+    }
+    if (sl == 0) kv8_store8<BF16>(r.out(a) + ch * 8, a0, a1);
+}
+
+// More: a workgroup a row, 256 threads on the same plan.
+template <bool BF16>
+__global__ void __launch_bounds__(256)
+kv8_combine_kernel(const Kv8Merge a) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int pos = blockIdx.x % a.acc_sq, bh = blockIdx.x / a.acc_sq, bidb = bh / p.h, head = bh % p.h;
-    // (requested before the number of parts is known, up to what there is scratch for)
     __shared__ float s_w[128], s_red[2][2], s_part[256 * 8];
-    const int cpr = p.d / 8, nlane = 256 / cpr, ch = tid % cpr, sl = tid / cpr;
-    const int64_t rows = (int64_t)p.b * p.h * a.acc_sq, row = (int64_t)bh * a.acc_sq + pos;
-    float my = p.lseaccum[min(tid, p.num_splits - 1) * rows + row];
+    const int cpr = a.d / 8, nlane = 256 / cpr, ch = tid % cpr, sl = tid / cpr;
+    const Kv8MergeRow r(a, blockIdx.x);
+    float my = a.lse[min(tid, a.num_splits - 1) * r.rows + r.at];
     constexpr int PRE = 4;
     f32x4 r0[PRE], r1[PRE];
 #pragma unroll
     for (int i = 0; i < PRE; i++) {
-        const float *src = p.oaccum + (min(sl + i * nlane, p.num_splits - 1) * rows + row) * p.d + ch * 8;
+        const float *src = a.o + (min(sl + i * nlane, a.num_splits - 1) * r.rows + r.at) * a.d + ch * 8;
         r0[i] = *(const f32x4 *)src;
         r1[i] = *(const f32x4 *)(src + 4);
     }
-    const int ns = a.n_split[bidb * n_mblocks + (pos * p.h_ratio + head % p.h_ratio) / rows_per_block];
-    const BlockInfo bi(p, bidb);
-    if (pos >= bi.sq || (a.max_rows > 0 && bi.sq * p.h_ratio > a.max_rows)) return;
-    if (ns <= 1) return;                       // one part: written in place
+    const int ns = r.n;
+    if (ns == 0) return;
     my = tid < ns ? my : -INFINITY;
     float m = my;
 #pragma unroll
@@ -670,7 +757,7 @@ kv8_combine_kernel(const KV8Params a, const int n_mblocks, const int rows_per_bl
     sum = s_red[1][0] + s_red[1][1];
     const bool none = sum == 0.f;                             // no part saw a key of this row
     if (tid < 128) s_w[tid] = none ? 0.f : e / sum;
-    if (tid == 0) p.lse[(int64_t)bh * p.seqlen_q + pos] = none ? INFINITY : logf(sum) + ref;
+    if (tid == 0) *r.lse(a) = none ? INFINITY : logf(sum) + ref;
     __syncthreads();
     f32x4 a0 = {0, 0, 0, 0}, a1 = {0, 0, 0, 0};
     if (sl < nlane) {
@@ -680,7 +767,7 @@ kv8_combine_kernel(const KV8Params a, const int n_mblocks, const int rows_per_bl
             if (sp < ns) { a0 += r0[i] * s_w[sp]; a1 += r1[i] * s_w[sp]; }
         }
         for (int sp = sl + PRE * nlane; sp < ns; sp += nlane) {
-            const float *src = p.oaccum + (sp * rows + row) * p.d + ch * 8;
+            const float *src = a.o + (sp * r.rows + r.at) * a.d + ch * 8;
             a0 += *(const f32x4 *)src * s_w[sp];
             a1 += *(const f32x4 *)(src + 4) * s_w[sp];
         }
@@ -693,11 +780,7 @@ kv8_combine_kernel(const KV8Params a, const int n_mblocks, const int rows_per_bl
             a0 += *(const f32x4 *)(s_part + (l * cpr + tid) * 8);
             a1 += *(const f32x4 *)(s_part + (l * cpr + tid) * 8 + 4);
         }
-        unsigned short *og = (unsigned short *)p.o + bi.q_off(p.o_bs, p.o_rs, bidb) + (int64_t)head * p.o_hs + (int64_t)pos * p.o_rs + tid * 8;
-        i32x4 w;
-        w[0] = pack2<BF16>(a0[0], a0[1]); w[1] = pack2<BF16>(a0[2], a0[3]);
-        w[2] = pack2<BF16>(a1[0], a1[1]); w[3] = pack2<BF16>(a1[2], a1[3]);
-        *(i32x4 *)og = w;
+        kv8_store8<BF16>(r.out(a) + tid * 8, a0, a1);
     }
 }
 
@@ -723,7 +806,11 @@ static hipError_t launch_kv8(const KV8Params &a, hipStream_t stream) {
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || p.num_splits <= 1) return e;
     const long long rows = (long long)p.b * p.h * a.acc_sq;
-    hipLaunchKernelGGL(kv8_combine_kernel<BF16>, dim3((unsigned)rows), dim3(256), 0, stream, a, n_mblocks, 16 * NR);
+    if (rows > 0x7fffffffLL) return hipErrorInvalidValue;
+    const Kv8Merge m{p.oaccum, p.lseaccum, p.lse, (unsigned short *)p.o, a.n_split, p.cu_seqlens_q, p.o_bs, p.o_rs, p.o_hs,
+                     p.b, p.h, p.d, a.acc_sq, p.num_splits, p.seqlen_q, a.max_rows, p.h_ratio, n_mblocks, 16 * NR};
+    if (p.num_splits <= A_FEW_PARTS) hipLaunchKernelGGL(kv8_combine_few_kernel<BF16>, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, stream, m);
+    else hipLaunchKernelGGL(kv8_combine_kernel<BF16>, dim3((unsigned)rows), dim3(256), 0, stream, m);
     return hipGetLastError();
 }
 
