@@ -66,6 +66,35 @@ __device__ __forceinline__ int amax_bits(i32x4 x, int m) {
     return m;
 }
 
+// The arguments of the two copies, in order of use: they lie in host memory, and the cache lines of a decode step's
+// launch are most of its time (KV8Params whole: 5.3 us, b128 of one token).
+struct KV8CacheArgs {                    // names as in KV8Params
+    struct Base {
+        const int *cu_seqlens_k, *block_table, *cache_batch_idx;
+        int64_t bt_bs;
+        void *k, *v;
+        int64_t k_bs, k_rs, k_hs, v_bs, v_rs, v_hs;
+        int seqlen_k, h_k, d, b;
+    } p;
+    unsigned char *ks, *vs;
+    int64_t ks_bs, ks_rs, ks_hs, vs_bs, vs_rs, vs_hs;
+    int cap, blk, page_rows, num_pages;
+    unsigned page_mul, blk_mul;
+    int page_sh, blk_sh;
+    explicit KV8CacheArgs(const KV8Params &a)
+        : p{a.p.cu_seqlens_k, a.p.block_table, a.p.cache_batch_idx, a.p.bt_bs, (void *)a.p.k, (void *)a.p.v,
+            a.p.k_bs, a.p.k_rs, a.p.k_hs, a.p.v_bs, a.p.v_rs, a.p.v_hs, a.p.seqlen_k, a.p.h_k, a.p.d, a.p.b},
+          ks(a.ks), vs(a.vs), ks_bs(a.ks_bs), ks_rs(a.ks_rs), ks_hs(a.ks_hs), vs_bs(a.vs_bs), vs_rs(a.vs_rs), vs_hs(a.vs_hs),
+          cap(a.cap), blk(a.blk), page_rows(a.page_rows), num_pages(a.num_pages), page_mul(a.page_mul), blk_mul(a.blk_mul),
+          page_sh(a.page_sh), blk_sh(a.blk_sh) {}
+};
+struct KV8New {
+    const int *cu;                       // ragged: (b + 1)
+    const void *k, *v;
+    int64_t k_bs, k_rs, k_hs, v_bs, v_rs, v_hs;
+    int seqlen, n_blocks, n_hgroups;
+};
+
 // One workgroup per (sequence, touched block of tokens, group of heads, K or V).  LPR lanes hold one head's
 // row (8 elements each), so a wave covers 64 / LPR adjacent heads of a token, whose rows are adjacent in
 // memory; the four waves take the block's rows in turn.  The block belongs to this workgroup alone, so its
@@ -73,20 +102,20 @@ __device__ __forceinline__ int amax_bits(i32x4 x, int m) {
 // atomics, and nothing depends on the order of workgroups.
 template <bool BF16, int LPR>
 __global__ void __launch_bounds__(Q_NT)
-kv8_quantize_kernel(const KV8Params a, const int n_blocks, const int n_hgroups) {
-    const KParams &p = a.p;
+kv8_quantize_kernel(const KV8New x_new, const KV8CacheArgs a) {
+    const auto &p = a.p;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    int64_t L = blockIdx.x;
+    unsigned L = blockIdx.x;
     const bool is_v = L & 1; L >>= 1;
-    const int hg = (int)(L % n_hgroups); L /= n_hgroups;
-    const int j = (int)(L % n_blocks);
-    const int bidb = (int)(L / n_blocks);
+    const int hg = (int)(L % x_new.n_hgroups); L /= x_new.n_hgroups;
+    const int j = (int)(L % x_new.n_blocks);
+    const int bidb = (int)(L / x_new.n_blocks);
 
     const int start = kv8_cached(a, bidb);
     int64_t src0;                        // first new token's row
     int n_new;
-    if (a.cu_new) { src0 = a.cu_new[bidb]; n_new = a.cu_new[bidb + 1] - a.cu_new[bidb]; }
-    else { src0 = 0; n_new = p.seqlen_knew; }
+    if (x_new.cu) { src0 = x_new.cu[bidb]; n_new = x_new.cu[bidb + 1] - x_new.cu[bidb]; }
+    else { src0 = 0; n_new = x_new.seqlen; }
     const int end = (int)min((int64_t)start + max(n_new, 0), (int64_t)a.cap);
     const int64_t block0 = kv8_div(start >> 4, a.blk_mul, a.blk_sh) * a.blk + (int64_t)j * a.blk;
     if (block0 >= end || end <= start) return;
@@ -105,10 +134,10 @@ kv8_quantize_kernel(const KV8Params a, const int n_blocks, const int n_hgroups) 
     unsigned char *scale = (is_v ? a.vs : a.ks) + (int64_t)page * (is_v ? a.vs_bs : a.ks_bs) +
                            (int64_t)kv8_div(in_page >> 4, a.blk_mul, a.blk_sh) * (is_v ? a.vs_rs : a.ks_rs) +
                            (int64_t)hsafe * (is_v ? a.vs_hs : a.ks_hs);
-    const int64_t nrs = is_v ? p.vnew_rs : p.knew_rs;
-    const unsigned short *src = (const unsigned short *)(is_v ? p.vnew : p.knew) +
-                                (a.cu_new ? src0 * nrs : (int64_t)bidb * (is_v ? p.vnew_bs : p.knew_bs)) -
-                                (int64_t)start * nrs + (int64_t)hsafe * (is_v ? p.vnew_hs : p.knew_hs) + csafe;   // row of token 0
+    const int64_t nrs = is_v ? x_new.v_rs : x_new.k_rs;
+    const unsigned short *src = (const unsigned short *)(is_v ? x_new.v : x_new.k) +
+                                (x_new.cu ? src0 * nrs : (int64_t)bidb * (is_v ? x_new.v_bs : x_new.k_bs)) -
+                                (int64_t)start * nrs + (int64_t)hsafe * (is_v ? x_new.v_hs : x_new.k_hs) + csafe;   // row of token 0
 
     const bool holds = start > lo;       // the block has tokens already: its scale only grows
     const int e_old = holds ? (int)*scale - 127 : KV8_EMIN;
@@ -165,61 +194,86 @@ hipError_t run_kv8_quantize(const KV8Params &a, hipStream_t stream) {
     const long long blocks = 2LL * p.b * n_blocks * n_hgroups;
     if (blocks > 0x7fffffffLL) return hipErrorInvalidValue;
     const dim3 grid((unsigned)blocks), wg(Q_NT);
-#define VFA_Q(LPR)                                                                                                          \
-    if (p.is_bf16) hipLaunchKernelGGL((kv8_quantize_kernel<true, LPR>), grid, wg, 0, stream, a, n_blocks, n_hgroups);       \
-    else hipLaunchKernelGGL((kv8_quantize_kernel<false, LPR>), grid, wg, 0, stream, a, n_blocks, n_hgroups)
+    const KV8New x{a.cu_new, p.knew, p.vnew, p.knew_bs, p.knew_rs, p.knew_hs, p.vnew_bs, p.vnew_rs, p.vnew_hs,
+                   p.seqlen_knew, n_blocks, n_hgroups};
+    const KV8CacheArgs c(a);
+#define VFA_Q(LPR)                                                                                          \
+    if (p.is_bf16) hipLaunchKernelGGL((kv8_quantize_kernel<true, LPR>), grid, wg, 0, stream, x, c);         \
+    else hipLaunchKernelGGL((kv8_quantize_kernel<false, LPR>), grid, wg, 0, stream, x, c)
     if (lpr == 8) { VFA_Q(8); } else if (lpr == 16) { VFA_Q(16); } else { VFA_Q(32); }
 #undef VFA_Q
     return hipGetLastError();
 }
 
 constexpr int D_NT = 256;
+constexpr int D_CU = 1024;       // offsets of a ragged output that are bisected in LDS
 
-// A workgroup takes `tpw` output rows (tokens): its first threads find each row's sequence (ragged: by
-// bisection of the offsets), page and scale row, then all threads copy 16 codes at a time, adjacent threads
-// adjacent chunks of a token's heads.  Rows behind a sequence's tokens are zeros.
+struct KV8Out {                          // what is read back goes here
+    const int *cu;                       // ragged: (b + 1)
+    int64_t rows;                        // in all
+    void *k, *v;
+    int64_t k_bs, k_rs, k_hs, v_bs, v_rs, v_hs;
+    int seqlen, n_new;                   // dense: rows a sequence; tokens that the call has appended
+    int tpw, cph;                        // rows a workgroup, 8-element chunks of a head's row
+    // for the 16-bit attention kernels: the lengths they are to see
+    int *lens;
+    const int *cu_q;
+    int seqlen_q, ratio, min_rows;
+};
+
+// A workgroup takes `tpw` output rows (tokens): its first threads find each row's sequence (ragged: by bisection of the
+// offsets), page and scale row, then all threads copy 8 codes at a time, so that a wave's store is 1 KiB without gaps
+// (16 codes and two stores each: 188 us against 176 for b32, 500..8192 tokens, h8 d128).  Rows behind a sequence's tokens
+// are zeros.  What is written is twice what is read, so the streams go through the caches (past them: 240 us).
 struct RowOf {
     int64_t k, v, ks, vs, out_k, out_v;   // k < 0: no token here
 };
 
 template <bool BF16>
 __global__ void __launch_bounds__(D_NT)
-kv8_dequantize_kernel(const KV8Params a, const int tpw, const int cph) {
+kv8_dequantize_kernel(const KV8Out o, const KV8CacheArgs a) {
     __shared__ RowOf s_row[64];
-    const KParams &p = a.p;
+    __shared__ int s_cu[D_CU];
+    const auto &p = a.p;
+    const int tpw = o.tpw, cph = o.cph;
     const int tid = threadIdx.x;
     const int64_t first = (int64_t)blockIdx.x * tpw;
     // Read back for the 16-bit attention kernels: sequences that are the decode kernel's have length 0 there, and
     // rows behind a sequence are not read, so not written.
     auto length = [&](int i) -> int {
-        const int n = min(kv8_cached(a, i) + (p.knew ? p.seqlen_knew : 0), a.cap);
-        if (!a.lens_out) return n;
-        const int sq = p.cu_seqlens_q ? p.cu_seqlens_q[i + 1] - p.cu_seqlens_q[i] : p.seqlen_q;
-        return sq * p.h_ratio <= a.min_rows ? 0 : n;
+        const int n = min(kv8_cached(a, i) + o.n_new, a.cap);
+        if (!o.lens) return n;
+        const int sq = o.cu_q ? o.cu_q[i + 1] - o.cu_q[i] : o.seqlen_q;
+        return sq * o.ratio <= o.min_rows ? 0 : n;
     };
-    if (a.lens_out && blockIdx.x == 0)
-        for (int i = tid; i < p.b; i += D_NT) a.lens_out[i] = length(i);
-    if (tid < tpw && first + tid < a.rows_out) {
+    if (o.lens && blockIdx.x == 0)
+        for (int i = tid; i < p.b; i += D_NT) o.lens[i] = length(i);
+    const bool near = o.cu && p.b < D_CU;
+    if (near) {
+        for (int i = tid; i <= p.b; i += D_NT) s_cu[i] = o.cu[i];
+        __syncthreads();
+    }
+    if (tid < tpw && first + tid < o.rows) {
         const int64_t t = first + tid;
         int seq;
         int64_t tok;
         RowOf r;
-        if (a.cu_out) {
+        if (o.cu) {
             int lo = 0, hi = p.b;          // last sequence that starts at or before t
             while (hi - lo > 1) {
                 const int mid = (lo + hi) >> 1;
-                if (a.cu_out[mid] <= t) lo = mid; else hi = mid;
+                if ((near ? s_cu[mid] : o.cu[mid]) <= t) lo = mid; else hi = mid;
             }
             seq = lo;
-            tok = t - a.cu_out[seq];
-            if (t >= a.cu_out[p.b]) tok = a.cap;   // behind the last sequence
-            r.out_k = t * a.ko_rs; r.out_v = t * a.vo_rs;
+            tok = t - (near ? s_cu[seq] : o.cu[seq]);
+            if (t >= (near ? s_cu[p.b] : o.cu[p.b])) tok = a.cap;   // behind the last sequence
+            r.out_k = t * o.k_rs; r.out_v = t * o.v_rs;
         } else {
-            seq = (int)(t / a.seqlen_out);
-            tok = t - (int64_t)seq * a.seqlen_out;
-            r.out_k = seq * a.ko_bs + tok * a.ko_rs; r.out_v = seq * a.vo_bs + tok * a.vo_rs;
+            seq = o.rows <= 0x7fffffff ? (int)((unsigned)t / (unsigned)o.seqlen) : (int)(t / o.seqlen);
+            tok = t - (int64_t)seq * o.seqlen;
+            r.out_k = seq * o.k_bs + tok * o.k_rs; r.out_v = seq * o.v_bs + tok * o.v_rs;
         }
-        r.k = a.lens_out ? -3 : -1; r.v = r.ks = r.vs = 0;
+        r.k = o.lens ? -3 : -1; r.v = r.ks = r.vs = 0;
         if (tok >= 0 && tok < length(seq)) {
             const int page = kv8_page(a, seq, (int)tok);
             if (page >= 0) {
@@ -233,43 +287,50 @@ kv8_dequantize_kernel(const KV8Params a, const int tpw, const int cph) {
         s_row[tid] = r;
     }
     __syncthreads();
-    const int per = p.h_k * cph;                      // chunks of 16 elements of a token
-    const int n = (int)min((int64_t)tpw, a.rows_out - first) * per;
-    for (int i = tid; i < n; i += D_NT) {
-        const int t = i / per, c = i - t * per;
-        const int head = c / cph, col = (c - head * cph) * 16;
+    const int per = p.h_k * cph;                      // chunks of a token
+    const int rows = (int)min((int64_t)tpw, o.rows - first);
+    int t = tid / per, c = tid - t * per;
+    const int t_step = D_NT / per, c_step = D_NT - t_step * per;
+#pragma unroll 2
+    for (; t < rows; t += t_step, c += c_step) {
+        if (c >= per) {
+            c -= per;
+            if (++t >= rows) break;
+        }
+        const int head = c / cph, col = (c - head * cph) * 8;
         const RowOf &r = s_row[t];
         if (r.k == -3) continue;
-        i32x4 k = {0, 0, 0, 0}, v = k;
+        i32x2 k = {0, 0}, v = k;
         float ks = 1.f, vs = 1.f;
         if (r.k >= 0) {
-            k = *(const i32x4 *)((const unsigned char *)p.k + r.k + head * p.k_hs + col);
-            v = *(const i32x4 *)((const unsigned char *)p.v + r.v + head * p.v_hs + col);
+            k = *(const i32x2 *)((const unsigned char *)p.k + r.k + head * p.k_hs + col);
+            v = *(const i32x2 *)((const unsigned char *)p.v + r.v + head * p.v_hs + col);
             ks = e8m0_to_f32(a.ks[r.ks + head * a.ks_hs]);
             vs = e8m0_to_f32(a.vs[r.vs + head * a.vs_hs]);
         } else if (r.k == -2) {
-            k = i32x4{0x7f7f7f7f, 0x7f7f7f7f, 0x7f7f7f7f, 0x7f7f7f7f};
+            k = i32x2{0x7f7f7f7f, 0x7f7f7f7f};
             v = k;
         }
-        unsigned short *ko = (unsigned short *)a.k_out + r.out_k + head * a.ko_hs + col;
-        unsigned short *vo = (unsigned short *)a.v_out + r.out_v + head * a.vo_hs + col;
-        *(i32x4 *)ko = kv8_to16<BF16>(i32x2{k[0], k[1]}, ks);
-        *(i32x4 *)(ko + 8) = kv8_to16<BF16>(i32x2{k[2], k[3]}, ks);
-        *(i32x4 *)vo = kv8_to16<BF16>(i32x2{v[0], v[1]}, vs);
-        *(i32x4 *)(vo + 8) = kv8_to16<BF16>(i32x2{v[2], v[3]}, vs);
+        *(i32x4 *)((unsigned short *)o.k + r.out_k + head * o.k_hs + col) = kv8_to16<BF16>(k, ks);
+        *(i32x4 *)((unsigned short *)o.v + r.out_v + head * o.v_hs + col) = kv8_to16<BF16>(v, vs);
     }
 }
 
 hipError_t run_kv8_dequantize(const KV8Params &a, hipStream_t stream) {
     const KParams &p = a.p;
     if (a.rows_out <= 0) return hipSuccess;
-    const int cph = p.d / 16, per = p.h_k * cph;
-    // enough rows that every thread has a chunk or more, at most the 64 whose places fit in LDS
-    const int tpw = std::min(64, std::max(1, 4 * D_NT / per));
+    const int cph = p.d / 8, per = p.h_k * cph;
+    // rows enough for eight chunks a thread (finding the rows is a chain of loads), down to one where that leaves fewer
+    // than 1024 workgroups; at most the 64 whose places fit in LDS
+    const long long least = std::max(1, D_NT / per), most = std::max(1, 8 * D_NT / per);
+    const int tpw = (int)std::min(64LL, std::max(least, std::min(most, (long long)a.rows_out / 1024)));
     const long long blocks = (a.rows_out + tpw - 1) / tpw;
     if (blocks > 0x7fffffffLL) return hipErrorInvalidValue;
-    if (p.is_bf16) hipLaunchKernelGGL(kv8_dequantize_kernel<true>, dim3((unsigned)blocks), dim3(D_NT), 0, stream, a, tpw, cph);
-    else hipLaunchKernelGGL(kv8_dequantize_kernel<false>, dim3((unsigned)blocks), dim3(D_NT), 0, stream, a, tpw, cph);
+    const KV8Out o{a.cu_out, a.rows_out, a.k_out, a.v_out, a.ko_bs, a.ko_rs, a.ko_hs, a.vo_bs, a.vo_rs, a.vo_hs, a.seqlen_out,
+                   p.knew ? p.seqlen_knew : 0, tpw, cph, a.lens_out, p.cu_seqlens_q, p.seqlen_q, p.h_ratio, a.min_rows};
+    const KV8CacheArgs c(a);
+    if (p.is_bf16) hipLaunchKernelGGL(kv8_dequantize_kernel<true>, dim3((unsigned)blocks), dim3(D_NT), 0, stream, o, c);
+    else hipLaunchKernelGGL(kv8_dequantize_kernel<false>, dim3((unsigned)blocks), dim3(D_NT), 0, stream, o, c);
     return hipGetLastError();
 }
 

@@ -55,21 +55,25 @@ __device__ __forceinline__ int kv8_div(int n, unsigned mul, int shift) {
     return (int)(__umulhi((unsigned)n << 1, mul) >> shift);
 }
 
+// (the helpers take a KV8Params, or a kernel's shorter argument block with the same names)
 // tokens in the cache of sequence bidb before the call
-__device__ __forceinline__ int kv8_cached(const KV8Params &a, int bidb) {
+template <class A>
+__device__ __forceinline__ int kv8_cached(const A &a, int bidb) {
     const int n = a.p.cu_seqlens_k ? a.p.cu_seqlens_k[bidb] : a.p.seqlen_k;
     return min(max(n, 0), a.cap);
 }
 
 // Page that holds token `tok` of sequence bidb (a contiguous cache: its batch row); -1 if the table names
 // none of the pool.  tok < cap.
-__device__ __forceinline__ int kv8_page(const KV8Params &a, int bidb, int tok) {
+template <class A>
+__device__ __forceinline__ int kv8_page(const A &a, int bidb, int tok) {
     int page;
     if (a.p.block_table) page = a.p.block_table[(int64_t)bidb * a.p.bt_bs + kv8_div(tok >> 4, a.page_mul, a.page_sh)];
     else page = a.p.cache_batch_idx ? a.p.cache_batch_idx[bidb] : bidb;
     return (unsigned)page < (unsigned)a.num_pages ? page : -1;
 }
-__device__ __forceinline__ int kv8_row_in_page(const KV8Params &a, int tok) {
+template <class A>
+__device__ __forceinline__ int kv8_row_in_page(const A &a, int tok) {
     return a.p.block_table ? tok - kv8_div(tok >> 4, a.page_mul, a.page_sh) * a.page_rows : tok;
 }
 
