@@ -624,7 +624,11 @@ extern "C" int vfa_kv8_dequantize(const vfa_kv8_params *p) {
 }
 
 // Most (query position, head) rows of a KV head that the decode kernel takes, and the rows from which reading the
-// cache back and the 16-bit kernels are ahead of the prefill kernel over the codes.
+// cache back and the 16-bit kernels are ahead of the prefill kernel over the codes, at head dims up to 128 and above:
+// the codes' conversion is done once, not once for every 128 rows, and those kernels are tuned for long queries.
+// us over the codes / over the cache read back, h32/8 d128: b8 kv2048, 640 rows 86 / 85, 1024 rows 89.5 / 89, 4096 rows
+// 260 / 227; b4 kv8192, 384 rows 88 / 113, 2048 rows 322 / 296.  h8/4 d256: b8 kv2048, 96 rows 47 / 51, 192 rows 85 / 72,
+// 512 rows 132 / 82; b4 kv8192, 96 rows 88 / 104, 192 rows 132 / 120.
 constexpr int VFA_KV8_DECODE_ROWS = 64, VFA_KV8_READ_BACK_ROWS = 1024, VFA_KV8_READ_BACK_ROWS_WIDE = 192;
 
 // How a call is carried out: sequences of few (query position, head) rows by the decode kernel, the others by the

@@ -5,6 +5,10 @@
 // applies the power-of-two scale), so the result is that of the 16-bit cache path on the cache read back,
 // up to the order of sums.
 //
+// Measured (reads alone reach 6.1 to 6.3 TB/s on this card): b128 kv8192 h32/8 d128 fp16 353 us (6.1 TB/s); b48 kv16384 h16
+// d64 274 us (5.9 TB/s); b1 kv65536 h32/8 d128 36 us, of which the loop over the keys is 20 (6.5 TB/s) and the rest the
+// launch, 4.5 us of dependent loads to the first key (arguments, lengths, page ids) and 5.5 us for the merge.
+//
 // HBM-bound: 2 d bytes per key and KV head against 4 d rows flops.  A workgroup is 8 waves; each wave owns
 // one KV head (of heads_per_wg adjacent ones, whose rows are adjacent in memory) and every parts-th step of
 // 32 keys, with a running maximum, sum and output of its own.  Waves share nothing until the end, so the key

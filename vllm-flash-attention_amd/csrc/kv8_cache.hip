@@ -1,7 +1,9 @@
 // Writing tokens to an 8-bit KV cache and reading it back (see vfa_kv8.h for the format).
 //
 // Both are copies: 2 bytes in and 1 out per element, or 1 in and 2 out, bound by HBM (by the launch for a
-// decode step's few tokens).
+// decode step's few tokens).  Measured, h8 d128: prompts of 16 100 tokens written 20.9 us (99 MB, 4.75 TB/s), 139 000
+// tokens read back 176 us (855 MB, 4.85 TB/s), where a 2 GiB copy runs at 4.9 TB/s; one token of 128 sequences written
+// 4.9 us, of which an empty launch is 3.6.
 #include "vfa_kv8.h"
 #include <algorithm>
 

@@ -13,6 +13,10 @@
 // partner of a rotation pair (rd / 16 lanes away, as rd is a multiple of 16) is one exchange of the packed
 // 16-bit words.  A wave stays with one token while it walks that token's heads: angles and weights are
 // loaded once per wave and the rows of adjacent heads are adjacent in memory.
+//
+// Measured, b4 s4096 h32/8 d128 bf16: forward 74 us (336 MB, 4.5 TB/s), backward 115 us (503 MB, 4.4 TB/s) and 4.6 us for
+// the sum of the weights' partials, where a 2 GiB copy runs at 4.9 TB/s.  One token of 64 sequences: 4.5 us, of which an
+// empty launch is 3.6.
 #include "vfa_qk_norm.h"
 #include <algorithm>
 
