@@ -374,6 +374,7 @@ def test_large_and_uneven_batches(b, h, hk, d, cap, num_splits):
     (140, 1, 20, 1, 128, 3000, "bf16", 32),          # 32 rows
     (140, 2, 2, 2, 256, 1600, "fp16", 64),
     (600, 1, 4, 4, 112, 700, "bf16", 16),
+    (300, 2, 8, 4, 64, 1200, "bf16", 16),            # pairs of heads
 ])
 def test_runs_of_keys_across_sequences(b, sq, h, hk, d, cap, dtype, page, equal):
     """Batches that parts of equal length leave much of the chip idle with: a workgroup then has pieces of several
@@ -384,6 +385,47 @@ def test_runs_of_keys_across_sequences(b, sq, h, hk, d, cap, dtype, page, equal)
     lens[3] = lens[70] = 0
     cache = Cache(b, cap, hk, d, 16, page, seed=92)
     _check(cache, lens, _q((b, sq, h, d), dtype, 93), dtype)
+
+
+@pytest.mark.parametrize("h,hk,d,page", [(2, 2, 64, 16), (4, 2, 128, 32), (6, 2, 48, 0), (8, 1, 64, 16), (2, 1, 256, 32)])
+def test_short_ragged_queries(h, hk, d, page):
+    """Single tokens, a few drafted ones and sequences without a query in one ragged batch: the decode kernel alone."""
+    counts, lens = [1, 3, 2, 0, 1, 4, 1], [900, 3, 77, 50, 1, 1500, 0]
+    cache = Cache(len(lens), max(lens), hk, d, 16, page, seed=120)
+    for num_splits in (0, 1, 4):
+        _check(cache, lens, _q((sum(counts), h, d), "bf16", 121), "bf16", ragged=counts, causal=True, num_splits=num_splits)
+
+
+def test_runs_of_keys_over_a_ragged_batch():
+    g = torch.Generator().manual_seed(122)
+    counts = torch.randint(0, 4, (160,), generator=g).tolist()
+    lens = (1500 * (0.7 + 0.3 * torch.rand(160, generator=g))).int().tolist()
+    cache = Cache(160, 1500, 4, 128, 16, 0, seed=123)
+    _check(cache, lens, _q((sum(counts), 4, 128), "fp16", 124), "fp16", ragged=counts, causal=True)
+
+
+@pytest.mark.parametrize("hk,d,b,sq", [(4, 128, 150, 1), (8, 64, 150, 1), (4, 128, 150, 20), (4, 128, 20, 1), (8, 64, 3, 1)])
+def test_long_streams(hk, d, b, sq):
+    """Pools of more than 512 MiB of codes, whose loads go past the caches: parts and runs, heads alone and in pairs."""
+    small = Cache(b, 1600, hk, d, 16, 64, extra_pages=0, seed=125)
+    n = small.codes[0].shape[0]
+    pool = 260 * 2 ** 20 // (64 * hk * d) + 1
+    pool = max(pool, n)
+    ids = torch.randperm(pool, generator=torch.Generator().manual_seed(126))[:n]
+    gpu = []
+    for t, dt in ((small.codes[0], torch.float8_e4m3fn), (small.codes[1], torch.float8_e4m3fn), (small.scales[0], torch.float8_e8m0fnu), (small.scales[1], torch.float8_e8m0fnu)):
+        big = torch.full((pool, *t.shape[1:]), 127, dtype=torch.uint8, device="cuda")
+        big[ids.cuda()] = t.to(torch.uint8).cuda()
+        gpu.append(big.view(dt))
+    wide = 260 * 2 ** 20 // (b * 64 * hk * d) + 1                       # pages a sequence may have
+    table = torch.zeros(b, max(wide, small.per), dtype=torch.int32)
+    table[:, :small.per] = ids[small.table.long()].to(torch.int32)
+    lens = (1600 * (0.6 + 0.4 * torch.rand(b, generator=torch.Generator().manual_seed(127)))).int().tolist()
+    q = _q((b, sq, hk, d), "bf16", 128).cuda()
+    out = _fa().flash_attn_with_quantized_kvcache(q, *gpu, cache_seqlens=torch.tensor(lens, dtype=torch.int32).cuda(), block_table=table.cuda(), causal=True)
+    for i in range(0, b, 1 if b < 10 else 7):
+        want, tol = attend_ref(q[i], small.values(0, i, lens[i]), small.values(1, i, lens[i]), True)
+        _close(out[i], want, tol, "sequence %d" % i)
 
 
 def test_runs_of_keys_with_windows_and_new_tokens():
@@ -468,6 +510,10 @@ def test_scales_at_the_ends_of_their_range():
         same = (k[i].flatten().cpu() == want) | (torch.isnan(k[i].flatten().cpu()) & torch.isnan(want))
         assert bool(same.all()), (e, codes[~same])
     assert torch.isnan(k[3]).all() and torch.equal(k.view(torch.int16), v.view(torch.int16))
+    h, _ = fa.dequantize_kvcache(kc, kc, sc, sc, torch.full((4,), 16, dtype=torch.int32).cuda(), max_seqlen=16, dtype=torch.float16)
+    for i, e in enumerate((-127, -126, 127)):               # fp16 holds none of these: zeros and infinities
+        want, got = (val * 2.0 ** e).to(torch.float16), h[i].flatten().cpu()
+        assert bool(((got == want) | (torch.isnan(got) & torch.isnan(want))).all()), e
     # a token that joins a block at 2^127, and one whose scale is NaN
     x = torch.zeros(4, 1, 1, 16, dtype=torch.bfloat16)
     x[:, :, :, 0] = 2.0 ** 127

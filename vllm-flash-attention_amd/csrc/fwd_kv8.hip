@@ -347,18 +347,18 @@ fwd_kv8_kernel(const KV8Params args, const int n_mblocks) {
         }
     }
 
-    const int k_rs = (int)p.k_rs, v_rs = (int)p.v_rs;
+    const unsigned k_rs = (unsigned)p.k_rs, v_rs = (unsigned)p.v_rs;   // (under 2^27: sixteen rows and a head stay under 2^32)
     // lane offsets inside a tile of 16 keys: K 16 columns of key c, V chunk lane + 64 i
     unsigned koff[NJ], voff[NV / 2];
 #pragma unroll
     for (int j = 0; j < NJ; j++) {
         const int col = (PAIR ? 0 : 64 * j) + 16 * g;
-        koff[j] = (unsigned)(c * k_rs + (PAIR ? j * (int)p.k_hs : 0) + (col < p.d ? col : 0));
+        koff[j] = (unsigned)c * k_rs + (PAIR ? j * (unsigned)p.k_hs : 0u) + (unsigned)(col < p.d ? col : 0);
     }
 #pragma unroll
     for (int i = 0; i < NV / 2; i++) {
         const int ci = lane + 64 * i, vc = ci % CPR * 16 % HD;
-        voff[i] = (unsigned)(ci / CPR * v_rs + (PAIR ? ci % CPR * 16 / HD * (int)p.v_hs : 0) + (vc < p.d ? vc : 0));
+        voff[i] = (unsigned)(ci / CPR) * v_rs + (PAIR ? (unsigned)(ci % CPR * 16 / HD) * (unsigned)p.v_hs : 0u) + (unsigned)(vc < p.d ? vc : 0);
     }
 
     // A step needs eight addresses: of K, V and their scales, for its two tiles.  Lane i of every eight works out

@@ -81,7 +81,8 @@ def flash_attn_with_quantized_kvcache(q, k_cache, v_cache, k_scale, v_scale, k=N
     If k / v (batch_size, seqlen_new, nheads_k, headdim) are given (dense q only) they are written first, as by
     quantize_kvcache, and attended.  The query is used as it is: rotate q and k beforehand (qk_norm_rotary_func).
     causal, window_size, alibi_slopes, num_splits, out as in flash_attn_with_kvcache; softmax_scale > 0.  Returns out,
-    shaped like q; a row that sees no key is zero.  No backward."""
+    shaped like q; a row that sees no key is zero.  An fp16 query over values past fp16's range (a cache that bf16 tokens
+    were written to) sees infinities.  No backward."""
     if (cu_seqlens_q is None) != (max_seqlen_q is None):
         raise ValueError("cu_seqlens_q and max_seqlen_q go together")
     if softmax_scale is None:
