@@ -5,6 +5,7 @@ import torch
 
 from kv8_util import HALF_STEP, TDT, Cache, attend_ref, encode, norm_rotary_ref, write_ref
 from test_gpu_kv8_attention import _check, _close, _q
+from test_gpu_qk_norm import test_forward_and_gradients as _norm_test
 
 pytestmark = pytest.mark.gpu
 
@@ -108,6 +109,16 @@ def test_prompts_decode_steps_and_read_back(h, hk, d, blk, page, dtype):
         assert torch.equal(k16[cu_k[i]:cu_k[i + 1]].double().cpu(), cache.values(0, i, n))
         want, tol = attend_ref(q2[i], cache.values(0, i, n), cache.values(1, i, n), True, dtype=dtype)
         _close(again[i * n_new:(i + 1) * n_new], want, tol, "read back %d" % i)
+
+
+@pytest.mark.parametrize("shape", [(3, 50, 1, 1, 128, 64, False), (2, 33, 4, 1, 64, 32, True), (1, 7, 2, 2, 128, 128, True), (5, 9, 3, 1, 40, 16, False),
+                                   (2, 21, 16, 1, 256, 256, False), (70, 1, 2, 1, 64, 64, False)])
+@pytest.mark.parametrize("given", [False, True])
+def test_norm_of_few_heads(shape, given):
+    """Tokens of so few heads that several share a wave, on one side or on both; the last ones alone."""
+    b, s, h, hk, d, rd, inter = shape
+    for dtype in ("fp16", "bf16"):
+        _norm_test(b, s, h, hk, d, rd, inter, "fp32", "same", given, dtype)
 
 
 def test_training_step_through_the_attention():

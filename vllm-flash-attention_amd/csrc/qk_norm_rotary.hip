@@ -19,6 +19,7 @@
 // empty launch is 3.6.
 #include "vfa_qk_norm.h"
 #include <algorithm>
+#include <type_traits>
 
 namespace vfa {
 
@@ -122,19 +123,29 @@ __device__ __forceinline__ i32x4 from_lane(i32x4 x, int src) {
     return o;
 }
 
-// item -> (token, part): a wave's U passes over 64 / LPR head rows each, of one token of q or of k
+// What a wave works on.  An item is U passes over 64 / LPR head rows each of one token of q or of k (head0: the first
+// pass's first); where a token has half as many heads as a pass has rows, or fewer, it is one pass over several tokens,
+// and all of this is the lane's own (head0: its head; t.h if there is none).
 struct Item {
-    int64_t tok;
     int bi, si, head0, pos;
 };
-__device__ __forceinline__ Item find_item(const QKNormParams &p, int64_t item, int parts, int rows) {
+__device__ __forceinline__ Item at_token(const QKNormParams &p, int64_t tok, int head0) {
     Item it;
-    it.tok = item / parts;
-    it.head0 = (int)(item - it.tok * parts) * rows;
-    it.bi = (int)(it.tok / p.s);
-    it.si = (int)(it.tok - (int64_t)it.bi * p.s);
+    it.head0 = head0;
+    it.bi = (int64_t)p.b * p.s <= 0x7fffffff ? (int)((unsigned)tok / (unsigned)p.s) : (int)(tok / p.s);
+    it.si = (int)(tok - (int64_t)it.bi * p.s);
     it.pos = p.positions ? p.positions[it.bi * p.pos_bs + it.si] : it.si;
     return it;
+}
+__device__ __forceinline__ Item find_item(const QKNormParams &p, int64_t item, int parts, int rows) {
+    const int64_t tok = parts == 1 ? item : item / parts;
+    return at_token(p, tok, (int)(item - tok * parts) * rows);
+}
+// row `j` of an item of 1 << t.toks_sh tokens with `rows` rows
+__device__ __forceinline__ Item find_row(const QKNormParams &p, const QKNormTensor &t, int64_t item, int j, int rows) {
+    const int heads = rows >> t.toks_sh;                      // (a power of two)
+    const int64_t tok = (item << t.toks_sh) + j / heads, all = (int64_t)p.b * p.s;
+    return at_token(p, min(tok, all - 1), tok < all ? j % heads : t.h);
 }
 
 // The first blocks_q workgroups walk q's items, the others k's.
@@ -156,34 +167,38 @@ qk_norm_fwd_kernel(const QKNormParams p, const int64_t items_q, const int64_t it
     for (int i = 0; i < 8; i++) w[i] = wo[i] = 0.f;
     if (col_ok) ld_f<BF16, 8>(t.w, col, p.w_f32, w);
     if (pairs) ld_f<BF16, 8>(t.w, pcol, p.w_f32, wo);
-    for (int64_t item = (int64_t)blk * N_NW + wave; item < items; item += (int64_t)n_blk * N_NW) {
-        const Item it = find_item(p, item, parts, RPW * U);
-        const unsigned short *xp = (const unsigned short *)t.x + it.bi * t.x_bs + it.si * t.x_rs + (col_ok ? col : 0);
-        unsigned short *yp = (unsigned short *)t.y + it.bi * t.y_bs + it.si * t.y_rs + col;
-        i32x4 x[U];
+    auto walk = [&](auto several) __attribute__((always_inline)) {
+        constexpr bool MULTI = decltype(several)::value;
+        constexpr int NU = MULTI ? 1 : U;
+        for (int64_t item = (int64_t)blk * N_NW + wave; item < items; item += (int64_t)n_blk * N_NW) {
+            const Item it = MULTI ? find_row(p, t, item, sub, RPW) : find_item(p, item, parts, RPW * U);
+            auto head_of = [&](int u) __attribute__((always_inline)) { return MULTI ? it.head0 : it.head0 + u * RPW + sub; };
+            const bool pad = it.pos < 0;               // zeros, whatever stands there
+            i32x4 x[NU];
 #pragma unroll
-        for (int u = 0; u < U; u++) {
-            const int head = it.head0 + u * RPW + sub;
-            x[u] = (col_ok && head < t.h) ? *(const i32x4 *)(xp + head * t.x_hs) : i32x4{0, 0, 0, 0};
+            for (int u = 0; u < NU; u++) {
+                const unsigned short *xp = (const unsigned short *)t.x + it.bi * t.x_bs + it.si * t.x_rs + (col_ok ? col : 0);
+                x[u] = (col_ok && head_of(u) < t.h) ? *(const i32x4 *)(xp + head_of(u) * t.x_hs) : i32x4{0, 0, 0, 0};
+            }
+            Turn tr;
+            load_turn<BF16>(p, pad ? 0 : it.pos, ch, lane, tr);
+#pragma unroll
+            for (int u = 0; u < NU; u++) {
+                float f[8], o[8], ss = 0.f;
+                unpack8<BF16>(x[u], f);
+#pragma unroll
+                for (int j = 0; j < 8; j++) ss += f[j] * f[j];
+                const float r = 1.f / sqrtf(row_sum<LPR>(ss) / (float)p.d + p.eps);
+                unpack8<BF16>(from_lane(x[u], tr.partner), o);
+#pragma unroll
+                for (int j = 0; j < 8; j++) { f[j] *= r * w[j]; o[j] *= r * wo[j]; }
+                turn8(p, tr, inside, f, o, 1.f);
+                unsigned short *yp = (unsigned short *)t.y + it.bi * t.y_bs + it.si * t.y_rs + col;
+                if (col_ok && head_of(u) < t.h) *(i32x4 *)(yp + head_of(u) * t.y_hs) = pad ? i32x4{0, 0, 0, 0} : pack8<BF16>(f);
+            }
         }
-        const bool pad = it.pos < 0;               // zeros, whatever stands there
-        Turn tr;
-        load_turn<BF16>(p, pad ? 0 : it.pos, ch, lane, tr);
-#pragma unroll
-        for (int u = 0; u < U; u++) {
-            const int head = it.head0 + u * RPW + sub;
-            float f[8], o[8], ss = 0.f;
-            unpack8<BF16>(x[u], f);
-#pragma unroll
-            for (int i = 0; i < 8; i++) ss += f[i] * f[i];
-            const float r = 1.f / sqrtf(row_sum<LPR>(ss) / (float)p.d + p.eps);
-            unpack8<BF16>(from_lane(x[u], tr.partner), o);
-#pragma unroll
-            for (int i = 0; i < 8; i++) { f[i] *= r * w[i]; o[i] *= r * wo[i]; }
-            turn8(p, tr, inside, f, o, 1.f);
-            if (col_ok && head < t.h) *(i32x4 *)(yp + head * t.y_hs) = pad ? i32x4{0, 0, 0, 0} : pack8<BF16>(f);
-        }
-    }
+    };
+    if (t.toks_sh > 0) walk(std::true_type{}); else walk(std::false_type{});
 }
 
 // Backward.  The first blocks_q workgroups walk q's items, the others k's, so that a workgroup's partial dw
@@ -205,43 +220,48 @@ qk_norm_bwd_kernel(const QKNormParams p, const int64_t items_q, const int64_t it
 #pragma unroll
     for (int i = 0; i < 8; i++) w[i] = acc[i] = 0.f;
     if (col_ok) ld_f<BF16, 8>(t.w, col, p.w_f32, w);
-    for (int64_t item = (int64_t)blk * N_NW + wave; item < items; item += (int64_t)n_blk * N_NW) {
-        const Item it = find_item(p, item, parts, RPW * U);
-        const unsigned short *xp = (const unsigned short *)t.x + it.bi * t.x_bs + it.si * t.x_rs + (col_ok ? col : 0);
-        const unsigned short *gp = (const unsigned short *)t.dy + it.bi * t.dy_bs + it.si * t.dy_rs + (col_ok ? col : 0);
-        unsigned short *yp = (unsigned short *)t.y + it.bi * t.y_bs + it.si * t.y_rs + col;
-        const bool pad = it.pos < 0;
-        i32x4 x[U], g[U];
+    auto walk = [&](auto several) __attribute__((always_inline)) {
+        constexpr bool MULTI = decltype(several)::value;
+        constexpr int NU = MULTI ? 1 : U;
+        for (int64_t item = (int64_t)blk * N_NW + wave; item < items; item += (int64_t)n_blk * N_NW) {
+            const Item it = MULTI ? find_row(p, t, item, sub, RPW) : find_item(p, item, parts, RPW * U);
+            auto head_of = [&](int u) __attribute__((always_inline)) { return MULTI ? it.head0 : it.head0 + u * RPW + sub; };
+            const bool pad = it.pos < 0;               // zeros, whatever stands there
+            i32x4 x[NU], g[NU];
 #pragma unroll
-        for (int u = 0; u < U; u++) {
-            const int head = it.head0 + u * RPW + sub;
-            const bool ok = col_ok && head < t.h && !pad;
-            x[u] = ok ? *(const i32x4 *)(xp + head * t.x_hs) : i32x4{0, 0, 0, 0};
-            g[u] = ok ? *(const i32x4 *)(gp + head * t.dy_hs) : i32x4{0, 0, 0, 0};
-        }
-        Turn tr;
-        load_turn<BF16>(p, pad ? 0 : it.pos, ch, lane, tr);
-#pragma unroll
-        for (int u = 0; u < U; u++) {
-            const int head = it.head0 + u * RPW + sub;
-            float f[8], q[8], o[8];
-            unpack8<BF16>(x[u], f);
-            unpack8<BF16>(g[u], q);
-            unpack8<BF16>(from_lane(g[u], tr.partner), o);
-            turn8(p, tr, inside, q, o, -1.f);             // g = R^T dy
-            float ss = 0.f, sg = 0.f;
-#pragma unroll
-            for (int i = 0; i < 8; i++) { ss += f[i] * f[i]; sg += q[i] * w[i] * f[i]; }
-            const float r = 1.f / sqrtf(row_sum<LPR>(ss) / (float)p.d + p.eps);
-            const float m = row_sum<LPR>(sg) / (float)p.d * r * r;
-#pragma unroll
-            for (int i = 0; i < 8; i++) {
-                if (col_ok && head < t.h && !pad) acc[i] += q[i] * f[i] * r;
-                f[i] = r * (q[i] * w[i] - f[i] * m);
+            for (int u = 0; u < NU; u++) {
+                const unsigned short *xp = (const unsigned short *)t.x + it.bi * t.x_bs + it.si * t.x_rs + (col_ok ? col : 0);
+                const unsigned short *gp = (const unsigned short *)t.dy + it.bi * t.dy_bs + it.si * t.dy_rs + (col_ok ? col : 0);
+                const bool ok = col_ok && head_of(u) < t.h && !pad;
+                x[u] = ok ? *(const i32x4 *)(xp + head_of(u) * t.x_hs) : i32x4{0, 0, 0, 0};
+                g[u] = ok ? *(const i32x4 *)(gp + head_of(u) * t.dy_hs) : i32x4{0, 0, 0, 0};
             }
-            if (t.y && col_ok && head < t.h) *(i32x4 *)(yp + head * t.y_hs) = pad ? i32x4{0, 0, 0, 0} : pack8<BF16>(f);
+            Turn tr;
+            load_turn<BF16>(p, pad ? 0 : it.pos, ch, lane, tr);
+#pragma unroll
+            for (int u = 0; u < NU; u++) {
+                const bool live = col_ok && head_of(u) < t.h;
+                float f[8], q[8], o[8];
+                unpack8<BF16>(x[u], f);
+                unpack8<BF16>(g[u], q);
+                unpack8<BF16>(from_lane(g[u], tr.partner), o);
+                turn8(p, tr, inside, q, o, -1.f);             // g = R^T dy
+                float ss = 0.f, sg = 0.f;
+#pragma unroll
+                for (int j = 0; j < 8; j++) { ss += f[j] * f[j]; sg += q[j] * w[j] * f[j]; }
+                const float r = 1.f / sqrtf(row_sum<LPR>(ss) / (float)p.d + p.eps);
+                const float m = row_sum<LPR>(sg) / (float)p.d * r * r;
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    if (live && !pad) acc[j] += q[j] * f[j] * r;
+                    f[j] = r * (q[j] * w[j] - f[j] * m);
+                }
+                unsigned short *yp = (unsigned short *)t.y + it.bi * t.y_bs + it.si * t.y_rs + col;
+                if (t.y && live) *(i32x4 *)(yp + head_of(u) * t.y_hs) = pad ? i32x4{0, 0, 0, 0} : pack8<BF16>(f);
+            }
         }
-    }
+    };
+    if (t.toks_sh > 0) walk(std::true_type{}); else walk(std::false_type{});
     if (!t.dw) return;
     __shared__ float s_acc[N_NW][LPR * 8];
 #pragma unroll
@@ -293,15 +313,26 @@ qk_norm_dw_kernel(const QKNormParams p) {
 static int lanes_per_row(int d) { return d <= 64 ? 8 : d <= 128 ? 16 : 32; }
 constexpr int N_U = 2;           // passes of a wave over a token's heads
 
+// Parts of a token's heads, and a wave's items on one side.  (b19 s2517 h1/1 d128 forward: one token a pass 57 us, four 16.)
 static int head_parts(const QKNormParams &p, int side) {
     const int rows = 64 / lanes_per_row(p.d) * N_U;
     return (p.t[side].h + rows - 1) / rows;
+}
+static int tokens_shift(const QKNormParams &p, int side) {
+    const int rows = 64 / lanes_per_row(p.d);
+    int sh = 0;
+    while (p.t[side].h << (sh + 1) <= rows) sh++;
+    return sh;
+}
+static int64_t side_items(const QKNormParams &p, int side) {
+    const int sh = tokens_shift(p, side);
+    return (((int64_t)p.b * p.s + (1 << sh) - 1) >> sh) * head_parts(p, side);
 }
 
 // Workgroups, shared out between the sides by their items: enough that every CU has work, few enough that the
 // weights are loaded (and, backward, the partial sums of dw written) seldom.
 void qk_norm_blocks(QKNormParams &p, int cus, bool bwd) {
-    const long long iq = (long long)p.b * p.s * head_parts(p, 0), ik = (long long)p.b * p.s * head_parts(p, 1);
+    const long long iq = side_items(p, 0), ik = side_items(p, 1);
     const long long most = (bwd ? 6LL : 8LL) * cus, all = std::max(1LL, iq + ik);
     auto share = [&](long long items) {
         const long long want = (items + N_NW - 1) / N_NW, part = (most * items + all - 1) / all;
@@ -309,12 +340,13 @@ void qk_norm_blocks(QKNormParams &p, int cus, bool bwd) {
     };
     p.blocks_q = share(iq);
     p.blocks_k = share(ik);
+    for (int side = 0; side < 2; side++) p.t[side].toks_sh = tokens_shift(p, side);
 }
 
 template <bool BF16, int LPR>
 static hipError_t launch(const QKNormParams &p, bool bwd, hipStream_t stream) {
     const int parts_q = head_parts(p, 0), parts_k = head_parts(p, 1);
-    const int64_t items_q = (int64_t)p.b * p.s * parts_q, items_k = (int64_t)p.b * p.s * parts_k;
+    const int64_t items_q = side_items(p, 0), items_k = side_items(p, 1);
     if (!bwd) {
         hipLaunchKernelGGL((qk_norm_fwd_kernel<BF16, LPR, N_U>), dim3((unsigned)(p.blocks_q + p.blocks_k)), dim3(N_NT), 0, stream, p,
                            items_q, items_k, parts_q, parts_k);

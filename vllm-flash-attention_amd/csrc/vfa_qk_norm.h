@@ -11,6 +11,7 @@ struct QKNormTensor {
     void *dw;                    // backward (same type as w), or null
     int64_t x_bs, x_rs, x_hs, dy_bs, dy_rs, dy_hs, y_bs, y_rs, y_hs;
     int h;
+    int toks_sh;                 // a wave's item is the heads of 1 << toks_sh tokens (0: of one token, or a part of them)
 };
 struct QKNormParams {
     QKNormTensor t[2];           // q, k
