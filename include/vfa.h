@@ -269,7 +269,8 @@ int vfa_kv8_dequantize(const vfa_kv8_params *p);
 
 /* Attention of q (dense (b, seqlen_q, h, d), or ragged with cu_seqlens_q) over the cache: a.q, a.out,
  * a.softmax_lse, masks and ALiBi as for vfa_mha_fwd_kvcache.  With a.knew the new tokens (dense) are written
- * first and attended.  a.num_splits: 0 = chosen here, n = at most n parts of a sequence's keys.  Partial results
+ * first and attended.  a.num_splits: 0 = chosen here, 1 = no split, n = the keys in as many parts as n of every
+ * sequence would be (by the lengths: longer sequences get more, at most n + 1).  Partial results
  * -- and for long queries the cache in 16 bits -- go to `workspace` (a.oaccum and a.softmax_lseaccum are not
  * used); nothing in it has to be set. */
 int vfa_kv8_mha_fwd(const vfa_kv8_params *p);

@@ -296,6 +296,37 @@ def test_capture_with_gradients_while_an_eager_graph_holds_a_leaf_is_refused():
         assert all(torch.equal(a, b) for a, b in zip(grads, first))
 
 
+def test_capture_of_views_of_a_held_leaf_is_refused():
+    """The same where the leaf comes as a view: ragged q and k, a slice of a packed projection."""
+    fa = _fa()
+    cos, sin = (t.cuda() for t in _tables(40, 64))
+    base = _norm_leaves(75)
+    w = base[2:]
+    pos = torch.arange(40, dtype=torch.int32).cuda()
+    flat = [t[0].clone().requires_grad_() for t in base[:2]]
+    packed = torch.cat(base[:2], 2)[0].clone().requires_grad_()
+    for q, k in ((flat[0], flat[1]), (flat[0], base[1][0]), (base[0][0], flat[1]), (packed[:, :4], packed[:, 4:])):
+        eager = fa.qk_norm_rotary_func(q, k, *w, cos, sin, positions=pos)
+        torch.cuda.synchronize()
+        with pytest.raises(RuntimeError, match="drop it before capturing"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                fa.qk_norm_rotary_func(q, k, *w, cos, sin, positions=pos)
+        del eager, q, k
+    # dropped: captured and right
+    def step():
+        out = fa.qk_norm_rotary_func(packed[:, :4], packed[:, 4:], *w, cos, sin, positions=pos)
+        return torch.autograd.grad(out, packed, [torch.ones_like(o) for o in out])[0]
+
+    want = step()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = step()
+    for _ in range(3):
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
+
+
 def test_gradient_of_a_gradient_is_refused():
     leaves = [t.requires_grad_() for t in _norm_leaves(73)]
     out = _fa().qk_norm_rotary_func(*leaves, *(t.cuda() for t in _tables(40, 64)))

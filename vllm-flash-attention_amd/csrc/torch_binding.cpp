@@ -1244,7 +1244,8 @@ struct QKNormRotary : torch::autograd::Function<QKNormRotary> {
 
 // A leaf keeps the stream of the first live graph that it is part of, and a backward pass hands its gradient over to
 // that stream.  The default stream cannot take part in a capture: the backward pass would end the process.
-void expect_capturable(const Tensor &x) {
+void expect_capturable(const Tensor &input) {
+    const Tensor x = input.is_view() ? Tensor(input._base()) : input;   // (a ragged or packed input is a view of its leaf)
     if (!x.requires_grad() || !x.is_leaf() || !x.is_cuda()) return;
     const auto leaf = torch::autograd::impl::try_get_grad_accumulator(x);
     const auto stream = leaf ? leaf->stream() : c10::nullopt;
