@@ -312,6 +312,14 @@ def test_capture_of_views_of_a_held_leaf_is_refused():
             with torch.cuda.graph(torch.cuda.CUDAGraph()):
                 fa.qk_norm_rotary_func(q, k, *w, cos, sin, positions=pos)
         del eager, q, k
+    # an input that an eager operation made
+    q = base[0][0].clone().requires_grad_() * 2
+    torch.cuda.synchronize()
+    with pytest.raises(RuntimeError, match="drop it before capturing"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            fa.qk_norm_rotary_func(q, base[1][0], *w, cos, sin, positions=pos)
+    del q
+
     # dropped: captured and right
     def step():
         out = fa.qk_norm_rotary_func(packed[:, :4], packed[:, 4:], *w, cos, sin, positions=pos)

@@ -1242,15 +1242,20 @@ struct QKNormRotary : torch::autograd::Function<QKNormRotary> {
     }
 };
 
-// A leaf keeps the stream of the first live graph that it is part of, and a backward pass hands its gradient over to
-// that stream.  The default stream cannot take part in a capture: the backward pass would end the process.
-void expect_capturable(const Tensor &input) {
-    const Tensor x = input.is_view() ? Tensor(input._base()) : input;   // (a ragged or packed input is a view of its leaf)
-    if (!x.requires_grad() || !x.is_leaf() || !x.is_cuda()) return;
-    const auto leaf = torch::autograd::impl::try_get_grad_accumulator(x);
-    const auto stream = leaf ? leaf->stream() : c10::nullopt;
-    TORCH_CHECK(!stream || stream->id() != 0,
-                "qk_norm_rotary_func: a graph recorded on the default stream still holds an input; drop it before capturing a pass with gradients");
+// A node of a graph keeps the stream that it was recorded on (a leaf: that of the first live graph it is part of), and a
+// backward pass hands its gradient over to that stream.  The default stream cannot take part in a capture: the backward
+// pass would end the process.
+void expect_capturable(const Tensor &x) {
+    if (!x.requires_grad()) return;
+    const auto refuse_default = [](const std::shared_ptr<torch::autograd::Node> &node) {
+        const auto stream = node ? node->stream() : std::nullopt;
+        TORCH_CHECK(!stream || stream->id() != 0,
+                    "qk_norm_rotary_func: a graph recorded on the default stream still holds an input; drop it before capturing a pass with gradients");
+    };
+    refuse_default(x.grad_fn());
+    const Tensor base = x.is_view() ? Tensor(x._base()) : x;   // (a ragged or packed input is a view)
+    if (!base.requires_grad()) return;
+    refuse_default(base.is_leaf() ? torch::autograd::impl::try_get_grad_accumulator(base) : base.grad_fn());
 }
 
 std::vector<Tensor> qk_norm_rotary(const Tensor &q, const Tensor &k, const Tensor &wq, const Tensor &wk, const Tensor &cos, const Tensor &sin,
