@@ -361,6 +361,23 @@ def test_on_another_stream():
     assert torch.equal(out, want)
 
 
+def test_two_streams_at_once():
+    """Calls in flight together, split over the keys and merged, share nothing."""
+    states = [_decode_state(76), _decode_state(77)]
+    want = [_decode_step(_copy(s)) for s in states]
+    streams = [torch.cuda.Stream() for _ in states]
+    copies = [[_copy(s) for _ in range(10)] for s in states]
+    torch.cuda.synchronize()
+    outs = [[], []]
+    for turn in range(10):
+        for i, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                outs[i].append(_decode_step(copies[i][turn]))
+    torch.cuda.synchronize()
+    for o, w in zip(outs, want):
+        assert all(torch.equal(x, w) for x in o)
+
+
 # rows = query positions x heads of a group: 1024 at head dims up to 128 and 192 above go through the cache read back
 LONG = [
     (2, 300, 8, 2, 128, 16, 32, [700, 300], 0),
