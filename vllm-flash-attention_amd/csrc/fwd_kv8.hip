@@ -88,7 +88,8 @@ template <int NR>
 __device__ __forceinline__ int kv8_steps(const KV8Params &a, int i, int q0) {
     const KParams &p = a.p;
     if (i >= p.b) return -1;
-    const int span = p.is_local ? (min(p.wl, a.cap) + min(p.wr, a.cap) + 16 * NR) / A_STEP + 2 : 1 << 30;
+    const int span = p.is_local ? (int)(((int64_t)min(p.wl, a.cap) + min(p.wr, a.cap) + 16 * NR) >> 5) + 2 : 1 << 30;
+    static_assert(A_STEP == 32, "");
     const int len = min(kv8_cached(a, i) + (p.knew ? p.seqlen_knew : 0), a.cap);
     const int rows = (p.cu_seqlens_q ? p.cu_seqlens_q[i + 1] - p.cu_seqlens_q[i] : p.seqlen_q) * p.h_ratio;
     return rows > q0 && !(a.max_rows > 0 && rows > a.max_rows) ? min((len + A_STEP - 1) / A_STEP, span) : -1;
@@ -822,7 +823,7 @@ template <int DP, bool BF16, int NR, bool NT, bool PAIR = false>
 static hipError_t launch_kv8_layout(const KV8Params &a, long long codes, hipStream_t stream) {
     const bool paged = a.p.block_table != nullptr;
     // Runs of steps (see the kernel) cost 2 us more before the first key; worth it where parts of equal length can leave
-    // a good part of the chip idle: two parts a sequence at most, or up to eight of long ones.  b4096 h32/8 d128, 64-row
+    // a good part of the chip idle: two parts a sequence at most, or up to eight of long ones.  kv4096 h32/8 d128, 64-row
     // pages: b129 311 -> 196 us, b65 154 -> 107; b48 kv16384 320 -> 274; b20 42.5 (44 with runs).
     // (In the 128 registers of head dim 64 the loop over pieces spills.)
     if constexpr (DP > 64 || NR > 1)
