@@ -217,11 +217,12 @@ struct KV8Out {                          // what is read back goes here
     int64_t k_bs, k_rs, k_hs, v_bs, v_rs, v_hs;
     int seqlen, n_new;                   // dense: rows a sequence; tokens that the call has appended
     int tpw, cph;                        // rows a workgroup, 8-element chunks of a head's row
-    // for the 16-bit attention kernels: the lengths they are to see
+    // for the 16-bit attention kernels: the lengths they are to see, and the window on the left (-1: none)
     int *lens;
     const int *cu_q;
-    int seqlen_q, ratio, min_rows;
+    int seqlen_q, ratio, min_rows, wl;
 };
+constexpr int D_TILE = 256;              // keys of their largest tile
 
 // A workgroup takes `tpw` output rows (tokens): its first threads find each row's sequence (ragged: by bisection of the
 // offsets), page and scale row, then all threads copy 8 codes at a time, so that a wave's store is 1 KiB without gaps
@@ -241,12 +242,14 @@ kv8_dequantize_kernel(const KV8Out o, const KV8CacheArgs a) {
     const int tid = threadIdx.x;
     const int64_t first = (int64_t)blockIdx.x * tpw;
     // Read back for the 16-bit attention kernels: sequences that are the decode kernel's have length 0 there, and
-    // rows behind a sequence are not read, so not written.
+    // rows behind a sequence are not read, so not written.  Neither are keys in front of the window of the sequence's
+    // first query, but for those in the first tile of a visible one: they are zeros, whatever the cache has there (a
+    // released page, a NaN code), because their weight 0 is multiplied with them.
+    auto queries = [&](int i) -> int { return o.cu_q ? o.cu_q[i + 1] - o.cu_q[i] : o.seqlen_q; };
     auto length = [&](int i) -> int {
         const int n = min(kv8_cached(a, i) + o.n_new, a.cap);
         if (!o.lens) return n;
-        const int sq = o.cu_q ? o.cu_q[i + 1] - o.cu_q[i] : o.seqlen_q;
-        return sq * o.ratio <= o.min_rows ? 0 : n;
+        return min(queries(i), o.seqlen_q) * o.ratio <= o.min_rows ? 0 : n;
     };
     if (o.lens && blockIdx.x == 0)
         for (int i = tid; i < p.b; i += D_NT) o.lens[i] = length(i);
@@ -276,7 +279,11 @@ kv8_dequantize_kernel(const KV8Out o, const KV8CacheArgs a) {
             r.out_k = seq * o.k_bs + tok * o.k_rs; r.out_v = seq * o.v_bs + tok * o.v_rs;
         }
         r.k = o.lens ? -3 : -1; r.v = r.ks = r.vs = 0;
-        if (tok >= 0 && tok < length(seq)) {
+        const int len = tok >= 0 && tok < a.cap ? length(seq) : 0;
+        const int first_key = o.lens && o.wl >= 0 ? max(0, (len - queries(seq)) - o.wl) : 0;
+        if (tok >= 0 && tok < len && tok < first_key) {
+            if (tok >= first_key / D_TILE * D_TILE) r.k = -1;
+        } else if (tok >= 0 && tok < len) {
             const int page = kv8_page(a, seq, (int)tok);
             if (page >= 0) {
                 const int row = kv8_row_in_page(a, (int)tok), blk = kv8_div(row >> 4, a.blk_mul, a.blk_sh);
@@ -329,7 +336,7 @@ hipError_t run_kv8_dequantize(const KV8Params &a, hipStream_t stream) {
     const long long blocks = (a.rows_out + tpw - 1) / tpw;
     if (blocks > 0x7fffffffLL) return hipErrorInvalidValue;
     const KV8Out o{a.cu_out, a.rows_out, a.k_out, a.v_out, a.ko_bs, a.ko_rs, a.ko_hs, a.vo_bs, a.vo_rs, a.vo_hs, a.seqlen_out,
-                   p.knew ? p.seqlen_knew : 0, tpw, cph, a.lens_out, p.cu_seqlens_q, p.seqlen_q, p.h_ratio, a.min_rows};
+                   p.knew ? p.seqlen_knew : 0, tpw, cph, a.lens_out, p.cu_seqlens_q, p.seqlen_q, p.h_ratio, a.min_rows, p.is_local ? p.wl : -1};
     const KV8CacheArgs c(a);
     if (p.is_bf16) hipLaunchKernelGGL(kv8_dequantize_kernel<true>, dim3((unsigned)blocks), dim3(D_NT), 0, stream, o, c);
     else hipLaunchKernelGGL(kv8_dequantize_kernel<false>, dim3((unsigned)blocks), dim3(D_NT), 0, stream, o, c);
