@@ -31,12 +31,13 @@ def _spoil(cache, gpu, i, tokens, how, table):
                 scales[page, row // cache.blk] = 147
 
 
-#     sq, h, hk, d, lens: rows over the cache read back
-SHAPES = [(300, 8, 2, 128, [900, 640]), (1100, 1, 1, 64, [1300, 1500]), (270, 8, 2, 96, [700, 500]), (100, 4, 2, 256, [500, 333]),
-          (200, 2, 2, 160, [500, 333]), (270, 8, 2, 128, [3000, 2011])]
+#     sq, h, hk, d, lens: few rows, rows over the codes, rows over the cache read back
+SHAPES = [(2, 8, 2, 128, [300, 190]), (1, 4, 4, 64, [115, 90]), (60, 8, 2, 128, [330, 190]), (30, 4, 2, 256, [300, 190]), (80, 1, 1, 64, [355, 158]),
+          (300, 8, 2, 128, [900, 640]), (1100, 1, 1, 64, [1300, 1500]), (270, 8, 2, 96, [700, 500]),
+          (100, 4, 2, 256, [500, 333]), (200, 2, 2, 160, [500, 333]), (270, 8, 2, 128, [3000, 2011])]
 
 
-@pytest.mark.parametrize("how", ["page", "code", "large"])
+@pytest.mark.parametrize("how", ["page", "code", "scale", "large"])
 @pytest.mark.parametrize("ragged", [False, True])
 @pytest.mark.parametrize("sq,h,hk,d,lens", SHAPES)
 def test_keys_in_front_of_the_window(sq, h, hk, d, lens, ragged, how):

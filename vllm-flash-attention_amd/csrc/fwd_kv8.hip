@@ -477,6 +477,11 @@ fwd_kv8_kernel(const KV8Params args, const int n_mblocks) {
                 const int key = k0 + (lane + 64 * (i % (NV / 2))) / CPR + 16 * (i / (NV / 2));
                 if (key < vis_lo || key >= vis_hi) w.v[i] = i32x4{0, 0, 0, 0};
             }
+#pragma unroll
+            for (int t = 0; t < 2; t++)               // nor the scale of a tile of such keys (a NaN, a page outside the pool)
+                if (k0 + 16 * t + 16 <= vis_lo || k0 + 16 * t >= vis_hi)
+#pragma unroll
+                    for (int e = 0; e < (PAIR ? 2 : 1); e++) sc[e][2 + t] = 1.f;
         }
 #pragma unroll
         for (int i = 0; i < NV; i++) {

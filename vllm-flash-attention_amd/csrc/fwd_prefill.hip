@@ -328,17 +328,19 @@ fwd_prefill_kernel(const std::conditional_t<LD == 5, KV8Params, KParams> args, c
     auto store_tile8 = [&](int n, auto BUFC) __attribute__((always_inline)) {
         constexpr int BUF = decltype(BUFC)::value;
         if constexpr (KV8) {
+#pragma unroll
+            for (int i = 0; i < NP; i++) vs8[i] |= bad8[i];
             if (n * BN < vis_lo || (n + 1) * BN > vis_hi) {
 #pragma unroll
                 for (int i = 0; i < NP; i++) {
                     const int key = n * BN + (tid + i * NT) / PPR;
-                    if (key < vis_lo || key >= vis_hi) vc8[i] = i32x4{0, 0, 0, 0};
+                    if (key < vis_lo || key >= vis_hi) { vc8[i] = i32x4{0, 0, 0, 0}; vs8[i] = 127u; }   // (the scale may be a NaN)
                 }
             }
 #pragma unroll
             for (int i = 0; i < NP; i++) {
                 const int tr = (tid + i * NT) / PPR, ch = (tid + i * NT) % PPR * 2;
-                const float ks = e8m0_to_f32(ks8[i] | bad8[i]), vs = e8m0_to_f32(vs8[i] | bad8[i]);
+                const float ks = e8m0_to_f32(ks8[i] | bad8[i]), vs = e8m0_to_f32(vs8[i]);
                 char *kd = smem + BUF * Cfg::TILE_BYTES, *vd = smem + (2 + BUF) * Cfg::TILE_BYTES;
 #pragma unroll
                 for (int e = 0; e < 2; e++) {
