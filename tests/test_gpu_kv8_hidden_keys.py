@@ -1,9 +1,10 @@
 """Attention over an 8-bit KV cache where what a row does not see cannot be multiplied by zero: NaN codes and scales, pages
-outside the pool, values past fp16's range.  A key that no row of its sequence sees has no part in any result."""
+outside the pool, values past fp16's range.  A key that no row of its sequence sees has no part in any result, and a row that
+sees no key is zero."""
 import pytest
 import torch
 
-from kv8_util import Cache, attend_ref
+from kv8_util import TDT, Cache, attend_ref
 from test_gpu_kv8_attention import _close, _q
 
 pytestmark = pytest.mark.gpu
@@ -59,3 +60,27 @@ def test_keys_in_front_of_the_window(sq, h, hk, d, lens, ragged, how):
         qi, oi = (q[i], out[i]) if not ragged else (q[:sq], out[:sq]) if i == 0 else (q[sq:], out[sq:])
         want, tol = attend_ref(qi.cuda(), cache.values(0, i, n), cache.values(1, i, n), True, (wl, 0), dtype=dtype)
         _close(oi, want, tol, "sequence %d" % i)
+
+
+#     sq, h, hk, d, lens: more query positions than keys
+SHORT = [(12, 4, 2, 64, [5, 9]), (7, 4, 4, 64, [3, 6]), (16, 8, 2, 128, [9, 2]), (9, 4, 2, 256, [5, 8]),
+         (50, 8, 2, 128, [33, 49]), (150, 2, 2, 64, [20, 149]), (40, 4, 2, 256, [17, 39])]
+
+
+@pytest.mark.parametrize("how", ["page", "code", "large"])
+@pytest.mark.parametrize("num_splits", [1, 3])
+@pytest.mark.parametrize("sq,h,hk,d,lens", SHORT)
+def test_a_row_that_sees_no_key_is_zero(sq, h, hk, d, lens, num_splits, how):
+    dtype = "fp16" if how == "large" else "bf16"
+    cache = Cache(2, max(lens), hk, d, 16, 16, seed=202)
+    gpu, table = cache.gpu(), cache.block_table()
+    for i, n in enumerate(lens):
+        _spoil(cache, gpu, i, [n - 1], how, table)     # a key that the last row sees
+    q = _q((2, sq, h, d), dtype, 203).cuda()
+    lens_gpu = torch.tensor(lens, dtype=torch.int32).cuda()
+    out = _fa().flash_attn_with_quantized_kvcache(q, *gpu, cache_seqlens=lens_gpu, block_table=table, causal=True, num_splits=num_splits)
+    for i, n in enumerate(lens):
+        assert not out[i, :sq - n].any(), "sequence %d: rows that see no key are not zero" % i
+        if how != "large":
+            assert torch.isnan(out[i, sq - 1]).all()
+    assert out.dtype == TDT[dtype]

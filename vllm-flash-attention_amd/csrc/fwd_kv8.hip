@@ -602,9 +602,16 @@ fwd_kv8_kernel(const KV8Params args, const int n_mblocks) {
         }
         const bool none = m_all == -INFINITY && l_all == 0.f;
         const float f = none ? 0.f : __builtin_amdgcn_exp2f((m_run[r] - m_fin) * c2) / l_all;
+        // (a wave that saw no key of this row has nothing to add: its O is a sum of zero weights times V, NaN if V is)
+        const bool saw = ml[((wave * NR + r) * 16 + c) * 2 + 1] != 0.f;
         char *ob = smem + wave * 16 * Cfg::O_ROWB + c * Cfg::O_ROWB + g * 16;
 #pragma unroll
-        for (int db = 0; db < NDB; db++) *(f32x4 *)(ob + db * 64) = o[r][db] * f;
+        for (int db = 0; db < NDB; db++) {
+            f32x4 x = o[r][db] * f;
+#pragma unroll
+            for (int i = 0; i < 4; i++) x[i] = saw ? x[i] : 0.f;
+            *(f32x4 *)(ob + db * 64) = x;
+        }
         const int row = PAIR ? c & 7 : q0 + 16 * r + c;
         if (part == 0 && g == 0 && row < rows)
             lse[stat_at(hk + (PAIR ? c >> 3 : 0), row)] = none ? (is_split ? -INFINITY : INFINITY) : m_all * p.scale + __logf(l_all);

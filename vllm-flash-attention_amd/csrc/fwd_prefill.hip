@@ -923,6 +923,8 @@ fwd_prefill_kernel(const std::conditional_t<LD == 5, KV8Params, KParams> args, c
     const float l_tot = half_swap_sum(l_run);
     const bool bad = (l_tot == 0.f) || (l_tot != l_tot);
     const float inv = (bad ? 1.f : 1.f / l_tot) * (DROP ? p.rp_dropout : 1.f);  // softmax.h:181
+    // (KV8: a row that sees no key is zero; its O is a sum of zero weights times V, NaN if V is)
+    auto result = [&](const float x) __attribute__((always_inline)) -> float { return KV8 && l_tot == 0.f ? 0.f : x * inv; };
     float lse = bad ? (SPLIT ? -INFINITY : INFINITY) : m_run * p.scale + __logf(l_tot);
     if (alibi_lin && !bad) {  // the row constant left out of the linear ALiBi form
         const float slope = alibi * p.scale;
@@ -941,8 +943,8 @@ fwd_prefill_kernel(const std::conditional_t<LD == 5, KV8Params, KParams> args, c
                 for (int g4 = 0; g4 < 4; g4++) {
                     const int col = 32 * db + 8 * g4 + 4 * hh;
                     if (col < p.d)
-                        *(f32x4 *)(dst + col) = f32x4{o[db][4 * g4] * inv, o[db][4 * g4 + 1] * inv,
-                                                      o[db][4 * g4 + 2] * inv, o[db][4 * g4 + 3] * inv};
+                        *(f32x4 *)(dst + col) = f32x4{result(o[db][4 * g4]), result(o[db][4 * g4 + 1]),
+                                                      result(o[db][4 * g4 + 2]), result(o[db][4 * g4 + 3])};
                 }
         }
         return;
@@ -954,8 +956,8 @@ fwd_prefill_kernel(const std::conditional_t<LD == 5, KV8Params, KParams> args, c
 #pragma unroll
         for (int g4 = 0; g4 < 4; g4++) {
             i32x2 w;
-            w[0] = pack2<BF16>(o[db][4 * g4 + 0] * inv, o[db][4 * g4 + 1] * inv);
-            w[1] = pack2<BF16>(o[db][4 * g4 + 2] * inv, o[db][4 * g4 + 3] * inv);
+            w[0] = pack2<BF16>(result(o[db][4 * g4 + 0]), result(o[db][4 * g4 + 1]));
+            w[1] = pack2<BF16>(result(o[db][4 * g4 + 2]), result(o[db][4 * g4 + 3]));
             *(i32x2 *)(ob + r * Cfg::O_ROWB + (32 * db + 8 * g4 + 4 * hh) * 2) = w;
         }
     __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): this wave's own LDS writes
