@@ -1260,6 +1260,8 @@ void expect_capturable(const Tensor &x) {
 
 std::vector<Tensor> qk_norm_rotary(const Tensor &q, const Tensor &k, const Tensor &wq, const Tensor &wk, const Tensor &cos, const Tensor &sin,
                                    const OptTensor &positions, double eps, bool interleaved) {
+    for (const Tensor *x : {&q, &k, &wq, &wk, &cos, &sin})   // (a tensor with a tangent need not require a gradient)
+        TORCH_CHECK(!x->_fw_grad(0).defined(), "qk_norm_rotary_func has no forward-mode derivative");
     // a serving step is a few microseconds: it is not recorded for a backward that cannot come
     if (at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || wq.requires_grad() || wk.requires_grad())) {
         if (q.is_cuda()) {

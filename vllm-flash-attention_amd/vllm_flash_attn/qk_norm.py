@@ -16,8 +16,8 @@ def qk_norm_rotary_func(q, k, q_weight, k_weight, rotary_cos, rotary_sin, positi
     defaults to 0 .. seqlen - 1; a negative position marks padding (output and gradients are zero there), one past the
     tables gives NaN.  A ragged batch is q (total, nheads, headdim), k (total, nheads_k, headdim) with positions (total,).
 
-    Returns (q_out, k_out).  Differentiable in q, k and the weights (not in the tables); gradients are bitwise
-    reproducible.  Can be captured into a graph with its backward, unless a graph recorded on the default stream still
+    Returns (q_out, k_out).  Differentiable in q, k and the weights (not in the tables; an input with a forward-mode
+    tangent is refused); gradients are bitwise reproducible.  Can be captured into a graph with its backward, unless a graph recorded on the default stream still
     holds one of the inputs or what it is a view of (refused: the backward pass would end the process).  headdim is a
     multiple of 8, at most 256.  No counterpart in the reference, whose cache call rotates q and k
     (csrc/flash_attn/src/rotary.h:19-148) but does not norm them."""
