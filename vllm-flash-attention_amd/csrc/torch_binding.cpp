@@ -1047,7 +1047,8 @@ std::vector<Tensor> fwd_kv8(const Tensor &q_, const Tensor &kc, const Tensor &vc
         TORCH_CHECK(o.size(-1) <= 1 || o.stride(-1) == 1, "Output tensor must have contiguous last dimension");
         bool fits = ((uintptr_t)o.data_ptr() & 15) == 0;
         for (int64_t i = 0; i + 1 < o.dim(); i++) fits = fits && stride_of(o, i) % 8 == 0;
-        out = fits ? o : torch::empty(q.sizes(), q.options());
+        // (rows behind the last sequence of a ragged batch stay as they are: they come back with the copy)
+        out = fits ? o : ragged ? o.clone(at::MemoryFormat::Contiguous) : torch::empty(q.sizes(), q.options());
     } else {
         out = torch::empty(q.sizes(), q.options());
     }
