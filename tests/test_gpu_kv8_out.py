@@ -1,5 +1,5 @@
 """The caller's `out` of flash_attn_with_quantized_kvcache: rows behind the last sequence stay as they were, whatever its
-alignment."""
+alignment, and what is returned is the caller's tensor also where there is nothing to compute."""
 import pytest
 import torch
 
@@ -33,3 +33,15 @@ def test_rows_behind_the_last_sequence_stay(counts):
         assert r.data_ptr() == out.data_ptr()
         assert torch.equal(out[:total], want[:total])
         assert bool((out[total:] == 7).all())
+
+
+def test_nothing_to_compute_returns_the_callers_tensor():
+    import vllm_flash_attn as fa
+    cache = Cache(2, 64, 2, 64, 16, 16, seed=222)
+    q = _q((5, 4, 64), "bf16", 223).cuda()
+    kw = dict(cache_seqlens=torch.tensor([64, 9], dtype=torch.int32).cuda(), block_table=cache.block_table(), max_seqlen_q=0,
+              cu_seqlens_q=torch.zeros(3, dtype=torch.int32).cuda())
+    for out in _outs(tuple(q.shape)):
+        r = fa.flash_attn_with_quantized_kvcache(q, *cache.gpu(), out=out, **kw)
+        assert r.data_ptr() == out.data_ptr() and r.stride() == out.stride()
+        assert bool((out == 7).all())

@@ -1057,7 +1057,7 @@ std::vector<Tensor> fwd_kv8(const Tensor &q_, const Tensor &kc, const Tensor &vc
     if (q.numel() == 0 || sq == 0) {
         // no query: the new tokens still enter the cache
         if (k_.has_value() && keep.first.numel() > 0) { P.a.stream = current_stream(); run(vfa_kv8_quantize(&P)); }
-        return {out, lse};
+        return {out_.has_value() ? out_.value() : out, lse};
     }
     P.a.dtype = dt;
     P.a.q = q.data_ptr(); P.a.out = out.data_ptr(); P.a.softmax_lse = lse.data_ptr<float>();
