@@ -61,7 +61,7 @@ EXTRA_FLAGS = {"fwd_kv8.hip": NO_PACKED_FP32, "fwd_prefill_kv8.hip": NO_PACKED_F
                "fwd_prefill_d64.hip": ["-fno-slp-vectorize"]}
 # the dropout translation units are one-line includes of the kernel sources
 EXTRA_DEPS = {"fwd_prefill_drop.hip": ["fwd_prefill.hip"], "bwd_drop.hip": ["bwd.hip"], "bwd_d96.hip": ["bwd.hip"], "fwd_prefill_wide_paged.hip": ["fwd_prefill_wide.hip"], "bwd_dq_ilp.hip": ["bwd.hip"], "fwd_prefill_d64.hip": ["fwd_prefill.hip"], "fwd_prefill_d96.hip": ["fwd_prefill.hip"], "fwd_prefill_pack.hip": ["fwd_prefill.hip"],
-              "fwd_prefill_split.hip": ["fwd_prefill.hip"], "fwd_prefill_kv8.hip": ["fwd_prefill.hip"]}
+              "fwd_prefill_split.hip": ["fwd_prefill.hip"]}
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 HIP_FLAGS = ["--offload-arch=gfx950", "-O3", "-fPIC", "-fvisibility=hidden", "-std=c++17", "-I", INCLUDE, "-I", CSRC]
 

@@ -16,7 +16,6 @@
 //     tiles that need them (wave-uniform test).
 #include "vfa_kernel_params.h"
 #include "vfa_dispatch.h"
-#include "vfa_kv8.h"
 #include <type_traits>
 
 namespace vfa {
@@ -123,10 +122,6 @@ struct PrefillCfg {
 // XOR swizzle places at its slot.  No staging registers, no ds_write, and the wave does not wait
 // for its own loads before the tile's last barrier.  (Out-of-range lanes write zeros.)
 // LD = 0: generic per-row addressing (any strides, any page size).
-// LD = 5: an 8-bit cache (vfa_kv8.h; the kernel's argument is then a KV8Params), contiguous or paged.
-// The codes go through staging registers, 16 of a row per load, and are converted once per workgroup
-// on their way to the 16-bit tile in LDS; from there on the kernel is the same.  The rows of a wave's load
-// lie in one group of 16, so in one page and one block of the scales.
 //
 // DROP: dropout on P (flash_fwd_kernel.h:324-337, dropout.h) with the reference's Philox pattern,
 // and the optional Return_softmax output.  The reference point of the exponentials then follows
@@ -143,14 +138,9 @@ struct PrefillCfg {
 // heads).  For a few query tokens per sequence against a long cache (chunked prefill, draft-token
 // verification): 16 tokens of 4 grouped heads fill half a 128-row block and sweep the keys once,
 // where one block per query head sweeps them four times at an eighth of the rows each.
-__device__ __forceinline__ const KParams &base_params(const KParams &p) { return p; }
-__device__ __forceinline__ const KParams &base_params(const KV8Params &a) { return a.p; }
-
 template <int DP, bool BF16, int NW, int LD, bool DROP, bool SPLIT = false, bool PACK = false, int DV = DP>
 __global__ void __launch_bounds__(NW * 64, (NW == 8 || DP == 256) ? 1 : 2)
-fwd_prefill_kernel(const std::conditional_t<LD == 5, KV8Params, KParams> args, const int n_mblocks) {
-    constexpr bool KV8 = LD == 5;                    // 8-bit codes, converted on their way into LDS
-    const KParams &p = base_params(args);
+fwd_prefill_kernel(const KParams p, const int n_mblocks) {
     static_assert(!PACK || (NW == 4 && !DROP), "packed grouped heads: 4-wave geometry, no dropout");
     constexpr bool DIRECT = LD == 3;                 // contiguous K/V, loaded straight into LDS
     constexpr bool PDIRECT = LD == 4;                // paged K/V (per-page descriptors), loaded straight into LDS
@@ -177,11 +167,8 @@ fwd_prefill_kernel(const std::conditional_t<LD == 5, KV8Params, KParams> args, c
     const int ratio = PACK ? p.pack_gqa : 1;
 
     const BlockInfo bi(p, bidb);
-    int sk_ = bi.sk;
-    if constexpr (KV8) sk_ = min(kv8_cached(args, bidb) + (p.knew ? p.seqlen_knew : 0), args.cap);
-    const int sq = bi.sq, sk = sk_;
-    const int sq_rows = (KV8 ? min(sq, p.seqlen_q) : sq) * ratio;    // rows of this (batch, head): query positions (x grouped heads)
-    if constexpr (KV8) if (sq_rows <= args.min_rows) return;   // the decode kernel's
+    const int sq = bi.sq, sk = bi.sk;
+    const int sq_rows = sq * ratio;    // rows of this (batch, head): query positions (x grouped heads)
     // Philox state: the caller's values, or (under graph capture) read on the device at replay
     // time from the generator's captured state (at::cuda::philox::unpack, flash_fwd_kernel.h:45)
     unsigned long long ph_seed = p.philox_seed, ph_offset = p.philox_offset;
@@ -219,15 +206,9 @@ fwd_prefill_kernel(const std::conditional_t<LD == 5, KV8Params, KParams> args, c
     float *oacc_g = nullptr;
     if constexpr (SPLIT) {
         const int split = blockIdx.y;
-        if constexpr (KV8) {   // the keys this block sees, in equal parts
-            const int per = (max(n_max - n_min, 0) + p.num_splits - 1) / p.num_splits;
-            n_min += split * per;
-            n_max = min(n_max, n_min + per);
-        } else {
-            const int per = (((p.seqlen_k + BN - 1) / BN) + p.num_splits - 1) / p.num_splits;  // from the capacity
-            n_min = max(n_min, split * per);
-            n_max = min(n_max, (split + 1) * per);
-        }
+        const int per = (((p.seqlen_k + BN - 1) / BN) + p.num_splits - 1) / p.num_splits;  // from the capacity
+        n_min = max(n_min, split * per);
+        n_max = min(n_max, (split + 1) * per);
         const int64_t acc_row0 = (((int64_t)split * p.b + bidb) * h_all + head0) * p.seqlen_q;
         lse_g = p.lseaccum + acc_row0;
         oacc_g = p.oaccum + acc_row0 * p.d;
@@ -280,77 +261,6 @@ fwd_prefill_kernel(const std::conditional_t<LD == 5, KV8Params, KParams> args, c
         kg += bi.k_off(p.k_bs, p.k_rs, bidb_cache);
         vg += bi.k_off(p.v_bs, p.v_rs, bidb_cache);
     }
-
-    // KV8: 16-byte pieces of the tile's codes per thread, and the scales of the wave's rows
-    constexpr int NP = KV8 ? CH / 2 : 1, PPR = DP / 16;
-    static_assert(!KV8 || (CH % 2 == 0 && 64 / PPR <= 16), "pieces of a wave lie in one group of 16 rows");
-    i32x4 kc8[NP], vc8[NP];
-    unsigned ks8[NP], vs8[NP], bad8[NP];
-    int pg8[NP];
-    const unsigned char *k_base = (const unsigned char *)p.k + (int64_t)hk * p.k_hs, *v_base = (const unsigned char *)p.v + (int64_t)hk * p.v_hs;
-    const unsigned char *ks_base = nullptr, *vs_base = nullptr;
-    if constexpr (KV8) { ks_base = args.ks + (int64_t)hk * args.ks_hs; vs_base = args.vs + (int64_t)hk * args.vs_hs; }
-    // (a thread's row in its group of 16 and its columns are the same in every piece; columns past the head dim
-    // read column 0: they meet zero columns of Q, or columns of O that are not stored)
-    static_assert(!KV8 || NT / PPR % 16 == 0, "");
-    const int col8 = tid % PPR * 16 < p.d ? tid % PPR * 16 : 0;
-    const unsigned koff8 = (unsigned)(((tid / PPR) & 15) * (int)p.k_rs + col8), voff8 = (unsigned)(((tid / PPR) & 15) * (int)p.v_rs + col8);
-    // keys that some row of the block sees: V of the others must not count, whatever stands there
-    const int vis_lo = p.is_local ? max(0, pos_lo_b + sk - sq - p.wl) : 0;
-    const int vis_hi = (p.is_causal || p.is_local) ? min(sk, pos_hi_b + sk - sq + p.wr) : sk;
-    auto load_pages8 = [&](int n) __attribute__((always_inline)) {
-        if constexpr (KV8) {
-#pragma unroll
-            for (int i = 0; i < NP; i++) {
-                const int g16 = min(n * BN + (((wave * 64 + i * NT) / PPR) & ~15), (sk - 1) & ~15);   // the wave's group of rows
-                if (bt) pg8[i] = bt[kv8_div(g16 >> 4, args.page_mul, args.page_sh)];
-                else pg8[i] = bidb_cache;
-            }
-        }
-    };
-    auto load_tile8 = [&](int n) __attribute__((always_inline)) {
-        if constexpr (KV8) {
-#pragma unroll
-            for (int i = 0; i < NP; i++) {
-                const int g16 = min(n * BN + (((wave * 64 + i * NT) / PPR) & ~15), (sk - 1) & ~15);
-                const int page = __builtin_amdgcn_readfirstlane(pg8[i]);
-                const bool bad = (unsigned)page >= (unsigned)args.num_pages;   // outside the pool: NaN, from the scale
-                const int row = bt ? g16 - kv8_div(g16 >> 4, args.page_mul, args.page_sh) * args.page_rows : g16;
-                const int64_t pg = bad ? 0 : page, blk = kv8_div(row >> 4, args.blk_mul, args.blk_sh);
-                bad8[i] = bad ? 255u : 0u;
-                ks8[i] = ks_base[pg * args.ks_bs + blk * args.ks_rs];
-                vs8[i] = vs_base[pg * args.vs_bs + blk * args.vs_rs];
-                kc8[i] = *(const i32x4 *)(k_base + pg * p.k_bs + (int64_t)row * p.k_rs + koff8);
-                vc8[i] = *(const i32x4 *)(v_base + pg * p.v_bs + (int64_t)row * p.v_rs + voff8);
-            }
-        }
-    };
-    auto store_tile8 = [&](int n, auto BUFC) __attribute__((always_inline)) {
-        constexpr int BUF = decltype(BUFC)::value;
-        if constexpr (KV8) {
-#pragma unroll
-            for (int i = 0; i < NP; i++) vs8[i] |= bad8[i];
-            if (n * BN < vis_lo || (n + 1) * BN > vis_hi) {
-#pragma unroll
-                for (int i = 0; i < NP; i++) {
-                    const int key = n * BN + (tid + i * NT) / PPR;
-                    if (key < vis_lo || key >= vis_hi) { vc8[i] = i32x4{0, 0, 0, 0}; vs8[i] = 127u; }   // (the scale may be a NaN)
-                }
-            }
-#pragma unroll
-            for (int i = 0; i < NP; i++) {
-                const int tr = (tid + i * NT) / PPR, ch = (tid + i * NT) % PPR * 2;
-                const float ks = e8m0_to_f32(ks8[i] | bad8[i]), vs = e8m0_to_f32(vs8[i]);
-                char *kd = smem + BUF * Cfg::TILE_BYTES, *vd = smem + (2 + BUF) * Cfg::TILE_BYTES;
-#pragma unroll
-                for (int e = 0; e < 2; e++) {
-                    const int off = lds_off<DP>(tr, ch + e);
-                    *(i32x4 *)(kd + off) = kv8_to16<BF16>(i32x2{kc8[i][2 * e], kc8[i][2 * e + 1]}, ks);
-                    *(i32x4 *)(vd + off) = kv8_to16<BF16>(i32x2{vc8[i][2 * e], vc8[i][2 * e + 1]}, vs);
-                }
-            }
-        }
-    };
 
     i32x4 kreg[CH], vreg[CH];
     // FAST path state: descriptors and the per-lane byte offset of chunk 0 (out of range for the
@@ -644,11 +554,6 @@ fwd_prefill_kernel(const std::conditional_t<LD == 5, KV8Params, KParams> args, c
         FWD_BLK_STAMP(5);
         __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): this wave's part of the first tile is in LDS
         FWD_BLK_STAMP(6);
-    } else if constexpr (KV8) {
-        load_pages8(n_max - 1);
-        load_tile8(n_max - 1);
-        if (n_max - 2 >= n_min) load_pages8(n_max - 2);
-        store_tile8(n_max - 1, std::integral_constant<int, 0>{});
     } else {
         load_pages(n_max - 1);
         load_tile(n_max - 1);
@@ -674,9 +579,6 @@ fwd_prefill_kernel(const std::conditional_t<LD == 5, KV8Params, KParams> args, c
             } else if constexpr (PDIRECT) {
                 load_tile_pdirect(n - 1, std::integral_constant<int, BUF ^ 1>{});
                 if (n - 2 >= n_min) load_pages(n - 2);
-            } else if constexpr (KV8) {
-                load_tile8(n - 1);
-                if (n - 2 >= n_min) load_pages8(n - 2);
             } else {
                 load_tile(n - 1);
                 if (n - 2 >= n_min) load_pages(n - 2);
@@ -896,7 +798,6 @@ fwd_prefill_kernel(const std::conditional_t<LD == 5, KV8Params, KParams> args, c
         }  // !skip
 
         if constexpr (TO_LDS) __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0) before the barrier
-        else if constexpr (KV8) { if (has_next) store_tile8(n - 1, std::integral_constant<int, BUF ^ 1>{}); }
         else if (has_next) store_tile(std::integral_constant<int, BUF ^ 1>{});
         STAMP(4);
         __syncthreads();
@@ -923,8 +824,6 @@ fwd_prefill_kernel(const std::conditional_t<LD == 5, KV8Params, KParams> args, c
     const float l_tot = half_swap_sum(l_run);
     const bool bad = (l_tot == 0.f) || (l_tot != l_tot);
     const float inv = (bad ? 1.f : 1.f / l_tot) * (DROP ? p.rp_dropout : 1.f);  // softmax.h:181
-    // (KV8: a row that sees no key is zero; its O is a sum of zero weights times V, NaN if V is)
-    auto result = [&](const float x) __attribute__((always_inline)) -> float { return KV8 && l_tot == 0.f ? 0.f : x * inv; };
     float lse = bad ? (SPLIT ? -INFINITY : INFINITY) : m_run * p.scale + __logf(l_tot);
     if (alibi_lin && !bad) {  // the row constant left out of the linear ALiBi form
         const float slope = alibi * p.scale;
@@ -943,8 +842,8 @@ fwd_prefill_kernel(const std::conditional_t<LD == 5, KV8Params, KParams> args, c
                 for (int g4 = 0; g4 < 4; g4++) {
                     const int col = 32 * db + 8 * g4 + 4 * hh;
                     if (col < p.d)
-                        *(f32x4 *)(dst + col) = f32x4{result(o[db][4 * g4]), result(o[db][4 * g4 + 1]),
-                                                      result(o[db][4 * g4 + 2]), result(o[db][4 * g4 + 3])};
+                        *(f32x4 *)(dst + col) = f32x4{o[db][4 * g4] * inv, o[db][4 * g4 + 1] * inv,
+                                                      o[db][4 * g4 + 2] * inv, o[db][4 * g4 + 3] * inv};
                 }
         }
         return;
@@ -956,8 +855,8 @@ fwd_prefill_kernel(const std::conditional_t<LD == 5, KV8Params, KParams> args, c
 #pragma unroll
         for (int g4 = 0; g4 < 4; g4++) {
             i32x2 w;
-            w[0] = pack2<BF16>(result(o[db][4 * g4 + 0]), result(o[db][4 * g4 + 1]));
-            w[1] = pack2<BF16>(result(o[db][4 * g4 + 2]), result(o[db][4 * g4 + 3]));
+            w[0] = pack2<BF16>(o[db][4 * g4 + 0] * inv, o[db][4 * g4 + 1] * inv);
+            w[1] = pack2<BF16>(o[db][4 * g4 + 2] * inv, o[db][4 * g4 + 3] * inv);
             *(i32x2 *)(ob + r * Cfg::O_ROWB + (32 * db + 8 * g4 + 4 * hh) * 2) = w;
         }
     __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): this wave's own LDS writes
@@ -973,13 +872,9 @@ fwd_prefill_kernel(const std::conditional_t<LD == 5, KV8Params, KParams> args, c
     FWD_BLK_STAMP(3);
 }
 
-inline const KParams &host_params(const KParams &p) { return p; }
-inline const KParams &host_params(const KV8Params &a) { return a.p; }
-
 template <int DP, bool BF16, int NW, int LD, bool DROP = false, bool SPLIT = false, bool PACK = false, int DV = DP>
-static hipError_t launch_prefill_impl(const std::conditional_t<LD == 5, KV8Params, KParams> &args, hipStream_t stream) {
+static hipError_t launch_prefill_impl(const KParams &p, hipStream_t stream) {
     using Cfg = PrefillCfg<DP, BF16, NW>;
-    const KParams &p = host_params(args);
     const int n_mblocks = (p.seqlen_q * (PACK ? p.pack_gqa : 1) + Cfg::BM - 1) / Cfg::BM;
     const long long blocks = (long long)n_mblocks * p.b * p.h;   // (PACK: p.h is the KV head count)
     if (blocks <= 0) return hipSuccess;
@@ -987,7 +882,7 @@ static hipError_t launch_prefill_impl(const std::conditional_t<LD == 5, KV8Param
     static std::atomic<uint64_t> lds_set{0};
     if (hipError_t e = set_dyn_lds_once((const void *)kern, Cfg::LDS_BYTES, lds_set); e != hipSuccess) return e;
     hipLaunchKernelGGL(kern, dim3((unsigned)blocks, SPLIT ? (unsigned)p.num_splits : 1u), dim3(Cfg::NT),
-                       Cfg::LDS_BYTES, stream, args, n_mblocks);
+                       Cfg::LDS_BYTES, stream, p, n_mblocks);
     return hipGetLastError();
 }
 
@@ -1062,24 +957,6 @@ hipError_t run_fwd_prefill_pack(const KParams &p_in, hipStream_t stream) {
     if (p.d <= 64) return bf ? launch_pack_s<64, true>(p, stream) : launch_pack_s<64, false>(p, stream);
     if (p.d <= 128) return bf ? launch_pack_s<128, true>(p, stream) : launch_pack_s<128, false>(p, stream);
     return bf ? launch_pack_s<256, true>(p, stream) : launch_pack_s<256, false>(p, stream);
-}
-#elif defined(VFA_KV8_TU)
-// Longer queries over an 8-bit cache, a translation unit of its own (fwd_prefill_kv8.hip): the query heads of
-// a KV head packed into the rows (one head per KV head is a group of one).
-template <int DP, bool BF16>
-static hipError_t launch_kv8_prefill(const KV8Params &a, hipStream_t stream) {
-    return a.p.num_splits > 1 ? launch_prefill_impl<DP, BF16, 4, 5, false, true, true>(a, stream)
-                              : launch_prefill_impl<DP, BF16, 4, 5, false, false, true>(a, stream);
-}
-hipError_t run_fwd_kv8_prefill(const KV8Params &a_in, hipStream_t stream) {
-    KV8Params a = a_in;
-    a.p.pack_gqa = a_in.p.h_ratio;   // the grid walks the KV heads
-    a.p.h = a_in.p.h_k;
-    a.p.h_ratio = 1;
-    const bool bf = a.p.is_bf16;
-    if (a.p.d <= 64) return bf ? launch_kv8_prefill<64, true>(a, stream) : launch_kv8_prefill<64, false>(a, stream);
-    if (a.p.d <= 128) return bf ? launch_kv8_prefill<128, true>(a, stream) : launch_kv8_prefill<128, false>(a, stream);
-    return bf ? launch_kv8_prefill<256, true>(a, stream) : launch_kv8_prefill<256, false>(a, stream);
 }
 #elif defined(VFA_FWD64_TU)
 // The d <= 64 instantiations, a translation unit of their own (fwd_prefill_d64.hip) because they are
