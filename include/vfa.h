@@ -228,7 +228,7 @@ int vfa_dispatch_geometry(const vfa_params *p, int kernel);
  * Common to the three entry points, in `a`: k / v = the codes, contiguous cache (num_pages, seqlen_k, h_k, d)
  * or pages (num_pages, page_block_size, h_k, d) with block_table; strides in BYTES, multiples of 16, base
  * pointers 16-byte aligned; b, h_k, d (a multiple of 16, at most 256); seqlen_k = the most tokens a sequence
- * can have (a contiguous cache: its rows, a multiple of 16; pages: max_blocks * page_block_size);
+ * can have (a contiguous cache: its rows, a multiple of 16; pages: max_blocks * page_block_size; at most 2^30);
  * cu_seqlens_k = (b) int32, tokens in the cache before the call (lengths, not offsets), NULL = seqlen_k;
  * cache_batch_idx (contiguous caches only).  Lengths are cut to [0, seqlen_k]; a page id outside
  * [0, num_pages) is never followed: nothing is written there, and what is read from it is NaN. */

@@ -555,6 +555,7 @@ static int kv8_fill(const vfa_kv8_params *p, vfa::KV8Params &k) {
     VFA_CHECK(!(a.block_table && a.cache_batch_idx), "Paged KVcache does not support cache_batch_idx");
     const int rows = a.block_table ? a.page_block_size : a.seqlen_k;
     VFA_CHECK(p->num_pages > 0 && rows > 0 && a.seqlen_k > 0, "8-bit KV cache: empty cache");
+    VFA_CHECK(a.seqlen_k <= 1 << 30 && rows <= 1 << 30 && a.seqlen_knew <= 1 << 30, "8-bit KV cache: more than 2^30 tokens of a sequence");
     VFA_CHECK(p->scale_block > 0 && p->scale_block % 16 == 0 && rows % p->scale_block == 0,
               "8-bit KV cache: the tokens per scale must be a multiple of 16 that divides the rows of a page");
     VFA_CHECK(a.block_table || a.cache_batch_idx || a.b <= p->num_pages, "8-bit KV cache: batch size exceeds the cache's");

@@ -90,7 +90,7 @@ __device__ __forceinline__ int kv8_steps(const KV8Params &a, int i, int q0) {
     if (i >= p.b) return -1;
     const int span = p.is_local ? (int)(((int64_t)min(p.wl, a.cap) + min(p.wr, a.cap) + 16 * NR) >> 5) + 2 : 1 << 30;
     static_assert(A_STEP == 32, "");
-    const int len = min(kv8_cached(a, i) + (p.knew ? p.seqlen_knew : 0), a.cap);
+    const int len = kv8_total(a, i, p.knew ? p.seqlen_knew : 0);
     const int rows = (p.cu_seqlens_q ? p.cu_seqlens_q[i + 1] - p.cu_seqlens_q[i] : p.seqlen_q) * p.h_ratio;
     return rows > q0 && !(a.max_rows > 0 && rows > a.max_rows) ? min((len + A_STEP - 1) / A_STEP, span) : -1;
 }
@@ -270,7 +270,7 @@ fwd_kv8_kernel(const KV8Params args, const int n_mblocks) {
 
     const BlockInfo bi(p, bidb);
     const int sq = bi.sq;
-    const int sk = min(kv8_cached(a, bidb) + (p.knew ? p.seqlen_knew : 0), a.cap);
+    const int sk = kv8_total(a, bidb, p.knew ? p.seqlen_knew : 0);
     const int rows = min(sq, p.seqlen_q) * ratio;    // (results have places for seqlen_q positions)
     if (q0 >= rows || (a.max_rows > 0 && rows > a.max_rows)) {
         if (runs) continue;
@@ -279,9 +279,9 @@ fwd_kv8_kernel(const KV8Params args, const int n_mblocks) {
     const int pos_lo = q0 / ratio, pos_hi = min(rows - 1, q0 + 16 * NR - 1) / ratio;
 
     // keys that some row of the block sees, and this part of them
-    const bool edge_r = p.is_causal || p.is_local;
-    const int vis_lo = p.is_local ? max(0, pos_lo + sk - sq - p.wl) : 0;
-    const int vis_hi = edge_r ? min(sk, pos_hi + 1 + sk - sq + p.wr) : sk;
+    const Kv8Seen seen(p, sq, sk);
+    const int vis_lo = seen.lo(pos_lo), vis_hi = seen.hi(pos_hi);
+    const int all_lo = seen.lo(pos_hi), all_hi = seen.hi(pos_lo);     // ... and that all of them see
     int n0 = vis_lo / A_STEP, n1 = vis_hi > vis_lo ? (vis_hi + A_STEP - 1) / A_STEP : n0;
     if (is_split) {
         const float per = (float)(n1 - n0) / (float)weight;
@@ -490,13 +490,11 @@ fwd_kv8_kernel(const KV8Params args, const int n_mblocks) {
         }
         load_step(next, w, next + parts);
 
-        bool need = k0 + A_STEP > sk;
-        if (edge_r) need = need || (k0 + A_STEP > pos_lo + 1 + sk - sq + p.wr);
-        if (p.is_local) need = need || (k0 < pos_hi + sk - sq - p.wl);
+        const bool need = k0 + A_STEP > all_hi || k0 < all_lo;
         if (has_alibi) {
 #pragma unroll
             for (int r = 0; r < NR; r++) {
-                const float at = p.is_causal ? 0.f : (float)(pos[r] + sk - sq);
+                const float at = p.is_causal ? 0.f : (float)(seen.shift + pos[r]);
 #pragma unroll
                 for (int t = 0; t < 2; t++)
 #pragma unroll
@@ -509,8 +507,8 @@ fwd_kv8_kernel(const KV8Params args, const int n_mblocks) {
         if (need) {
 #pragma unroll
             for (int r = 0; r < NR; r++) {
-                const int lo = (p.is_local ? max(0, pos[r] + sk - sq - p.wl) : 0) - k0 - 4 * g;
-                const int hi = (edge_r ? min(sk, pos[r] + 1 + sk - sq + p.wr) : sk) - k0 - 4 * g;
+                const int lo = seen.lo(pos[r]) - k0 - 4 * g;
+                const int hi = seen.hi(pos[r]) - k0 - 4 * g;
 #pragma unroll
                 for (int t = 0; t < 2; t++)
 #pragma unroll

@@ -54,15 +54,15 @@ kv8_prefill_kernel(const KV8Params args, const int n_mblocks) {
     const int ratio = p.pack_gqa;
 
     const BlockInfo bi(p, bidb);
-    const int sq = bi.sq, sk = min(kv8_cached(args, bidb) + (p.knew ? p.seqlen_knew : 0), args.cap);
+    const int sq = bi.sq, sk = kv8_total(args, bidb, p.knew ? p.seqlen_knew : 0);
     const int rows = min(sq, p.seqlen_q) * ratio;
     if (rows <= args.min_rows || m_block * BM >= rows) return;   // the decode kernel's, or none
 
     // ---- key tiles of the block: query positions [pos_lo_b, pos_hi_b) ----
     const int pos_lo_b = m_block * BM / ratio, pos_hi_b = min(sq, ((m_block + 1) * BM - 1) / ratio + 1);
-    int n_min = !p.is_local ? 0 : max(0, (pos_lo_b + sk - sq - p.wl) / BN);
-    int n_max = (sk + BN - 1) / BN;
-    if (p.is_causal || p.is_local) n_max = min(n_max, (pos_hi_b + sk - sq + p.wr + BN - 1) / BN);
+    const Kv8Seen seen(p, sq, sk);
+    const int vis_lo = seen.lo(pos_lo_b), vis_hi = seen.hi(pos_hi_b - 1);   // keys that some row of the block sees
+    int n_min = vis_lo / BN, n_max = (vis_hi + BN - 1) / BN;
 
     const int h_all = p.h * ratio, head0 = hk * ratio;           // query heads of the tensors, the group's first
     const unsigned short *qg = (const unsigned short *)p.q + bi.q_off(p.q_bs, p.q_rs, bidb) + (int64_t)head0 * p.q_hs;
@@ -87,7 +87,10 @@ kv8_prefill_kernel(const KV8Params args, const int n_mblocks) {
         return (int64_t)(row % ratio) * p.seqlen_q + row / ratio;
     };
     const int pos_l = (q0w + r) / ratio;                                  // this lane's query position
-    const int pos_lo_w = q0w / ratio, pos_hi_w = (q0w + 31) / ratio + 1;  // the wave's, [lo, hi)
+    // keys that some row of the wave sees, and that all of them see
+    const int pos_lo_w = q0w / ratio, pos_hi_w = (q0w + 31) / ratio;
+    const int some_lo = seen.lo(pos_lo_w), some_hi = q0w >= rows ? 0 : seen.hi(pos_hi_w);
+    const int all_lo = seen.lo(pos_hi_w), all_hi = seen.hi(pos_lo_w);
 
     if (n_max <= n_min) {
         // no visible key: O = 0, LSE = +inf; in a part: O = 0, LSE = -inf
@@ -121,9 +124,6 @@ kv8_prefill_kernel(const KV8Params args, const int n_mblocks) {
     // read column 0: they meet zero columns of Q, or columns of O that are not stored)
     const int col8 = tid % PPR * 16 < p.d ? tid % PPR * 16 : 0;
     const unsigned koff8 = (unsigned)(((tid / PPR) & 15) * (int)p.k_rs + col8), voff8 = (unsigned)(((tid / PPR) & 15) * (int)p.v_rs + col8);
-    // keys that some row of the block sees: V of the others must not count, whatever stands there
-    const int vis_lo = p.is_local ? max(0, pos_lo_b + sk - sq - p.wl) : 0;
-    const int vis_hi = (p.is_causal || p.is_local) ? min(sk, pos_hi_b + sk - sq + p.wr) : sk;
     auto group16 = [&](const int n, const int i) __attribute__((always_inline)) -> int {   // the wave's rows in piece i of tile n
         return min(n * BN + (((wave * 64 + i * NT) / PPR) & ~15), (sk - 1) & ~15);
     };
@@ -153,7 +153,7 @@ kv8_prefill_kernel(const KV8Params args, const int n_mblocks) {
         constexpr int BUF = decltype(BUFC)::value;
 #pragma unroll
         for (int i = 0; i < NP; i++) vs8[i] |= bad8[i];
-        if (n * BN < vis_lo || (n + 1) * BN > vis_hi) {
+        if (n * BN < vis_lo || (n + 1) * BN > vis_hi) {   // V of keys that no row sees must not count, whatever stands there
 #pragma unroll
             for (int i = 0; i < NP; i++) {
                 const int key = n * BN + (tid + i * NT) / PPR;
@@ -199,7 +199,7 @@ kv8_prefill_kernel(const KV8Params args, const int n_mblocks) {
     const bool has_alibi = p.alibi_slopes != nullptr;
     if (has_alibi) alibi = p.alibi_slopes[(int64_t)bidb * p.alibi_bs + head0 + (q0w + r) % ratio] / p.scale;
     const bool alibi_lin = has_alibi && (p.is_causal || (p.is_local && p.wr <= 0));
-    const int cref = pos_lo_b + sk - sq;
+    const int cref = seen.shift + pos_lo_b;
     const float c2 = p.scale_log2;
 
     // per-lane LDS read offsets; buffer, k-step and key block are compile-time constants on top
@@ -233,17 +233,12 @@ kv8_prefill_kernel(const KV8Params args, const int n_mblocks) {
         const char *vb = smem + (2 + BUF) * Cfg::TILE_BYTES;
         const int c0 = n * BN;
         // a wave whose 32 rows see none of this tile's keys only helps with the staging
-        bool skip = q0w >= rows;
-        if (p.is_causal || p.is_local) skip = skip || c0 >= pos_hi_w + sk - sq + p.wr;
-        if (p.is_local) skip = skip || (c0 + BN <= pos_lo_w + sk - sq - p.wl);
-        if (!skip) {
+        if (c0 < some_hi && c0 + BN > some_lo) {
         // ---- S^T = K Q^T: s[kb2][reg] = score(key = c0 + 32 kb2 + (reg & 3) + 8 (reg >> 2) + 4 hh, row q0w + r) ----
         // Vector instructions of a wave run in the shadow of its own MFMAs, so the maximum of the first 32 keys and the
         // exponentials of the first 16, against the current reference point, go with the MFMAs of the second 32 keys.
         // They stand unless the tile needs a mask or moves the reference point (both rare), which redoes them.
-        bool need_mask = c0 + BN > sk;
-        if (p.is_causal || p.is_local) need_mask = need_mask || (c0 + BN > pos_lo_w + 1 + sk - sq + p.wr);
-        if (p.is_local) need_mask = need_mask || (c0 < pos_hi_w - 1 + sk - sq - p.wl);
+        const bool need_mask = c0 + BN > all_hi || c0 < all_lo;
         const bool need = need_mask || has_alibi;
         f32x16 s[2];
         i32x4 pf[4];
@@ -304,8 +299,7 @@ kv8_prefill_kernel(const KV8Params args, const int n_mblocks) {
                     s[kb2][j] = __builtin_fmaf(alibi, (float)(32 * kb2 + (j & 3) + 8 * (j >> 2)), s[kb2][j] + t);
         }
         if (need_mask && !has_alibi && !p.is_local) {
-            const int hi = p.is_causal ? min(sk, pos_l + 1 + sk - sq) : sk;
-            const int lim = hi - c0 - 4 * hh;
+            const int lim = seen.hi(pos_l) - c0 - 4 * hh;
 #pragma unroll
             for (int kb2 = 0; kb2 < 2; kb2++)
 #pragma unroll
@@ -313,8 +307,7 @@ kv8_prefill_kernel(const KV8Params args, const int n_mblocks) {
                     s[kb2][j] = (32 * kb2 + (j & 3) + 8 * (j >> 2) < lim) ? s[kb2][j] : -INFINITY;
         }
         if ((need_mask && (has_alibi || p.is_local)) || (has_alibi && !alibi_lin && !need_mask)) {
-            const int lo = p.is_local ? max(0, pos_l + sk - sq - p.wl) : 0;
-            const int hi = (p.is_causal || p.is_local) ? min(sk, pos_l + 1 + sk - sq + p.wr) : sk;
+            const int lo = seen.lo(pos_l), hi = seen.hi(pos_l);
 #pragma unroll
             for (int kb2 = 0; kb2 < 2; kb2++)
 #pragma unroll
@@ -323,7 +316,7 @@ kv8_prefill_kernel(const KV8Params args, const int n_mblocks) {
                     float x = s[kb2][j];
                     if (has_alibi)
                         x = alibi_lin ? x + alibi * (float)(col - cref)
-                                      : x - alibi * fabsf((float)(pos_l + sk - sq - col));
+                                      : x - alibi * fabsf((float)(seen.shift + pos_l - col));
                     s[kb2][j] = (col >= lo && col < hi) ? x : -INFINITY;
                 }
         }
@@ -375,7 +368,7 @@ kv8_prefill_kernel(const KV8Params args, const int n_mblocks) {
             }
         }
         l_run += (ps[0] + ps[1]) + (ps[2] + ps[3]);
-        }  // !skip
+        }
         if (has_next) store_tile(n - 1, std::integral_constant<int, BUF ^ 1>{});
         __syncthreads();
     };
@@ -395,7 +388,7 @@ kv8_prefill_kernel(const KV8Params args, const int n_mblocks) {
     float lse = bad ? (SPLIT ? -INFINITY : INFINITY) : m_run * p.scale + __logf(l_tot);
     if (alibi_lin && !bad) {  // the row constant left out of the linear form
         const float slope = alibi * p.scale;
-        lse += p.is_causal ? slope * (float)cref : -slope * (float)(pos_l + sk - sq - cref);
+        lse += p.is_causal ? slope * (float)cref : -slope * (float)(seen.shift + pos_l - cref);
     }
     if (hh == 0 && q0w + r < rows) lse_g[stat_off(q0w + r)] = lse;
 

@@ -247,7 +247,7 @@ kv8_dequantize_kernel(const KV8Out o, const KV8CacheArgs a) {
     // released page, a NaN code), because their weight 0 is multiplied with them.
     auto queries = [&](int i) -> int { return o.cu_q ? o.cu_q[i + 1] - o.cu_q[i] : o.seqlen_q; };
     auto length = [&](int i) -> int {
-        const int n = min(kv8_cached(a, i) + o.n_new, a.cap);
+        const int n = kv8_total(a, i, o.n_new);
         if (!o.lens) return n;
         return min(queries(i), o.seqlen_q) * o.ratio <= o.min_rows ? 0 : n;
     };

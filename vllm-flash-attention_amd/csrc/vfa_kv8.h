@@ -63,6 +63,26 @@ __device__ __forceinline__ int kv8_cached(const A &a, int bidb) {
     return min(max(n, 0), a.cap);
 }
 
+// ... and with the call's own (both up to 2^30)
+template <class A>
+__device__ __forceinline__ int kv8_total(const A &a, int bidb, int n_new) {
+    const int n = kv8_cached(a, bidb);
+    return n + min(n_new, a.cap - n);
+}
+// The keys [lo, hi) that a query position sees, aligned at the last query and the last key.  (Positions, lengths and
+// windows go up to 2^30: no sum of two of them is formed that could be more.)
+struct Kv8Seen {
+    int sk, shift, wl, wr;             // shift: sk - sq
+    bool left, right;
+    __device__ __forceinline__ Kv8Seen(const KParams &p, int sq, int sk_)
+        : sk(sk_), shift(sk_ - sq), wl(p.wl), wr(p.wr), left(p.is_local), right(p.is_causal || p.is_local) {}
+    __device__ __forceinline__ int lo(int pos) const { return left ? max(0, shift + pos - wl) : 0; }
+    __device__ __forceinline__ int hi(int pos) const {
+        const int next = shift + pos + 1;
+        return right ? next + min(wr, sk - next) : sk;
+    }
+};
+
 // Page that holds token `tok` of sequence bidb (a contiguous cache: its batch row); -1 if the table names
 // none of the pool.  tok < cap.
 template <class A>
