@@ -64,7 +64,8 @@ def test_keys_in_front_of_the_window(sq, h, hk, d, lens, ragged, how):
 
 #     sq, h, hk, d, lens: more query positions than keys
 SHORT = [(12, 4, 2, 64, [5, 9]), (7, 4, 4, 64, [3, 6]), (16, 8, 2, 128, [9, 2]), (9, 4, 2, 256, [5, 8]),
-         (50, 8, 2, 128, [33, 49]), (150, 2, 2, 64, [20, 149]), (40, 4, 2, 256, [17, 39])]
+         (50, 8, 2, 128, [33, 49]), (150, 2, 2, 64, [20, 149]), (40, 4, 2, 256, [17, 39]),
+         (300, 8, 2, 128, [40, 299]), (1100, 1, 1, 64, [50, 1000]), (270, 8, 2, 96, [100, 3]), (100, 4, 2, 256, [33, 95]), (200, 2, 2, 160, [7, 180])]
 
 
 @pytest.mark.parametrize("how", ["page", "code", "large"])

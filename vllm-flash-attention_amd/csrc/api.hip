@@ -35,7 +35,10 @@ int kv8_heads_per_wg(int d, int h_k, bool pairs);
 bool kv8_pairs(int d, int h_k, int rows, int64_t k_hs, int64_t v_hs);
 int kv8_decode_rows(int d, int rows);
 int kv8_decode_wgs_per_cu(int d, int rows, bool pairs);
-hipError_t run_fwd_kv8_prefill(const KV8Params &a, hipStream_t stream);          // fwd_prefill_kv8.hip
+hipError_t run_kv8_merge(const KParams &p, hipStream_t stream);
+hipError_t run_fwd_kv8_prefill(const KV8Params &a, bool codes, hipStream_t stream);   // fwd_prefill_kv8.hip
+bool kv8_read_back_ok(int64_t seqlen_k, int h_k, int d);
+hipError_t run_fwd_kv8_wide(const KParams &p, hipStream_t stream);               // fwd_prefill_wide_kv8.hip
 hipError_t run_qk_norm_rotary(const QKNormParams &p, bool bwd, hipStream_t stream);   // qk_norm_rotary.hip
 void qk_norm_blocks(QKNormParams &p, int cus, bool bwd);
 }  // namespace vfa
@@ -635,7 +638,7 @@ constexpr int VFA_KV8_DECODE_ROWS = 64, VFA_KV8_READ_BACK_ROWS = 1024, VFA_KV8_R
 // How a call is carried out: sequences of few (query position, head) rows by the decode kernel, the others by the
 // prefill kernel -- over the codes, or over the cache read back into 16 bits first.
 struct Kv8Plan {
-    bool decode, prefill, read_back;
+    bool decode, prefill, read_back, wide;
     int dec_sq, dec_rows;        // most query positions and rows of a sequence of the decode kernel's
     int dec_splits, pre_splits;
     int hpw;                     // decode: KV heads, or pairs of them, of a workgroup
@@ -691,21 +694,24 @@ static int kv8_plan(const vfa_kv8_params *p, Kv8Plan &w) {
     }
     if (w.prefill) {
         const size_t codes = (size_t)a.b * a.seqlen_k * a.h_k * a.d;
-        w.read_back = rows >= (a.d <= 128 ? VFA_KV8_READ_BACK_ROWS : VFA_KV8_READ_BACK_ROWS_WIDE) && codes * 4 <= (size_t)2 << 30;
+        w.read_back = rows >= (a.d <= 128 ? VFA_KV8_READ_BACK_ROWS : VFA_KV8_READ_BACK_ROWS_WIDE) && codes * 4 <= (size_t)2 << 30 &&
+                      vfa::kv8_read_back_ok(a.seqlen_k, a.h_k, a.d);
         w.pre_splits = 1;
+        if (!a.cu_seqlens_q) {
+            // 128-row blocks, two workgroups per CU (over the cache read back above head dim 128: one); split only what
+            // would fill less than half of them (a part's fp32 results cost HBM traffic in proportion to its rows), at
+            // least four 64-key tiles each
+            const long long slots = (w.read_back && a.d > 128 ? 1LL : 2LL) * cus;
+            const long long blocks = (long long)a.b * a.h_k * ((rows + 127) / 128);
+            const long long chunks = ((long long)a.seqlen_k + 255) / 256;
+            long long s = a.num_splits > 0 ? a.num_splits : blocks * 2 > slots ? 1 : slots / blocks;
+            w.pre_splits = (int)std::max(1LL, std::min({s, chunks, 128LL}));
+        }
         if (w.read_back) {
+            w.wide = a.d > 128 && !a.alibi_slopes && w.pre_splits == 1;
             w.k16 = take(codes * 2);
             w.v16 = take(codes * 2);
             w.lens = take((size_t)a.b * sizeof(int));
-            if (!a.cu_seqlens_q)
-                w.pre_splits = a.num_splits > 0 ? a.num_splits : vfa_decode_num_splits(a.b, a.h, a.h_k, a.d, a.seqlen_k, a.seqlen_q, cus);
-        } else if (!a.cu_seqlens_q) {
-            // 128-row blocks, two workgroups per CU; split only what would fill less than half of them (a part's
-            // fp32 results cost HBM traffic in proportion to its rows), at least four 64-key tiles each
-            const long long blocks = (long long)a.b * a.h_k * ((rows + 127) / 128);
-            const long long chunks = ((long long)a.seqlen_k + 255) / 256;
-            long long s = a.num_splits > 0 ? a.num_splits : blocks * 2 > 2LL * cus ? 1 : 2LL * cus / blocks;
-            w.pre_splits = (int)std::max(1LL, std::min({s, chunks, 128LL}));
         }
         if (w.pre_splits > 1) {
             const size_t n = (size_t)w.pre_splits * a.b * a.h * a.seqlen_q;
@@ -765,39 +771,38 @@ extern "C" int vfa_kv8_mha_fwd(const vfa_kv8_params *p) {
     if (a.seqlen_q == 0) return VFA_OK;
     char *ws = (char *)p->workspace;
     k.min_rows = w.dec_rows;
-    if (w.prefill && w.read_back) {
-        vfa::KV8Params r = k;
-        r.k_out = ws + w.k16; r.v_out = ws + w.v16;
-        r.lens_out = (int *)(ws + w.lens);
-        r.ko_hs = r.vo_hs = a.d; r.ko_rs = r.vo_rs = (int64_t)a.h_k * a.d; r.ko_bs = r.vo_bs = r.ko_rs * a.seqlen_k;
-        r.rows_out = (int64_t)a.b * a.seqlen_k; r.seqlen_out = a.seqlen_k;
-        e = vfa::run_kv8_dequantize(r, stream);
-        if (e != hipSuccess) return hip_fail(e, "kv8 dequantize launch");
-        vfa_params q = a;
-        q.k = r.k_out; q.v = r.v_out;
-        q.k_batch_stride = q.v_batch_stride = r.ko_bs; q.k_row_stride = q.v_row_stride = r.ko_rs; q.k_head_stride = q.v_head_stride = a.d;
-        q.cu_seqlens_k = r.lens_out; q.is_seqlens_k_cumulative = 0;
-        q.block_table = nullptr; q.cache_batch_idx = nullptr; q.knew = q.vnew = nullptr;
-        q.total_q = 0;   // (what is left are the long sequences: not packed for the sake of the short ones)
-        q.num_splits = w.pre_splits;
-        q.oaccum = w.pre_splits > 1 ? (float *)(ws + w.pre_o) : nullptr;
-        q.softmax_lseaccum = w.pre_splits > 1 ? (float *)(ws + w.pre_lse) : nullptr;
-        KParams k16;
-        fill_common(&q, k16, q.seqlen_q, q.seqlen_k);
-        k16.k_cumulative = 0;
-        if ((rc = launch_fwd(&q, k16, false))) return rc;
-    } else if (w.prefill) {
+    if (w.prefill) {
         vfa::KV8Params f = k;
         if (w.pre_splits > 1) {
             f.p.num_splits = w.pre_splits;
             f.p.oaccum = (float *)(ws + w.pre_o);
             f.p.lseaccum = (float *)(ws + w.pre_lse);
         }
-        e = vfa::run_fwd_kv8_prefill(f, stream);
-        if (e == hipSuccess && w.pre_splits > 1) e = vfa::run_fwd_combine(f.p, stream);
+        if (w.read_back) {
+            f.k_out = ws + w.k16; f.v_out = ws + w.v16;
+            f.lens_out = (int *)(ws + w.lens);
+            f.ko_hs = f.vo_hs = a.d; f.ko_rs = f.vo_rs = (int64_t)a.h_k * a.d; f.ko_bs = f.vo_bs = f.ko_rs * a.seqlen_k;
+            f.rows_out = (int64_t)a.b * a.seqlen_k; f.seqlen_out = a.seqlen_k;
+            e = vfa::run_kv8_dequantize(f, stream);
+            if (e != hipSuccess) return hip_fail(e, "kv8 dequantize launch");
+        }
+        if (w.wide) {
+            vfa_params q = a;
+            q.k = f.k_out; q.v = f.v_out;
+            q.k_batch_stride = q.v_batch_stride = f.ko_bs; q.k_row_stride = q.v_row_stride = f.ko_rs; q.k_head_stride = q.v_head_stride = a.d;
+            q.cu_seqlens_k = f.lens_out; q.is_seqlens_k_cumulative = 0;
+            q.block_table = nullptr; q.cache_batch_idx = nullptr; q.knew = q.vnew = nullptr;
+            KParams k16;
+            fill_common(&q, k16, q.seqlen_q, q.seqlen_k);
+            k16.k_cumulative = 0;
+            e = vfa::run_fwd_kv8_wide(k16, stream);
+        } else {
+            e = vfa::run_fwd_kv8_prefill(f, !w.read_back, stream);
+        }
+        if (e == hipSuccess && w.pre_splits > 1) e = vfa::run_kv8_merge(f.p, stream);
         if (e != hipSuccess) return hip_fail(e, "kv8 prefill launch");
     }
-    if (w.decode) {   // (after the 16-bit kernels, which write zeros for the sequences that are not theirs)
+    if (w.decode) {   // (after the kernel of head dims above 128, which writes zeros for the sequences that are not its own)
         k.heads_per_wg = w.hpw;
         k.pairs = w.pairs;
         k.max_rows = w.prefill ? w.dec_rows : 0;

@@ -649,7 +649,7 @@ struct Kv8Merge {
     const float *o, *lse;
     float *out_lse;
     unsigned short *out;
-    const int *n_split, *cu_q;
+    const int *n_split, *cu_q;     // n_split: parts of a row's keys; null: num_splits each (prefill kernel)
     int64_t out_bs, out_rs, out_hs;
     int b, h, d, acc_sq, num_splits, seqlen_q, max_rows, ratio, n_mblocks, rows_per_block;
 };
@@ -664,7 +664,7 @@ struct Kv8MergeRow {
         head = bh - bidb * a.h;
         rows = (int64_t)a.b * a.h * a.acc_sq;
         at = row;
-        n = a.n_split[bidb * a.n_mblocks + (pos * a.ratio + head % a.ratio) / a.rows_per_block];
+        n = a.n_split ? a.n_split[bidb * a.n_mblocks + (pos * a.ratio + head % a.ratio) / a.rows_per_block] : a.num_splits;
         const int sq = a.cu_q ? a.cu_q[bidb + 1] - a.cu_q[bidb] : a.seqlen_q;
         if (pos >= sq || (a.max_rows > 0 && sq * a.ratio > a.max_rows) || n <= 1) n = 0;
     }
@@ -799,6 +799,56 @@ kv8_combine_kernel(const Kv8Merge a) {
     }
 }
 
+template <bool BF16>
+static hipError_t launch_merge(const Kv8Merge &m, hipStream_t stream) {
+    const long long rows = (long long)m.b * m.h * m.acc_sq;
+    if (rows > 0x7fffffffLL) return hipErrorInvalidValue;
+    if (m.num_splits <= A_FEW_PARTS) hipLaunchKernelGGL(kv8_combine_few_kernel<BF16>, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, stream, m);
+    else hipLaunchKernelGGL(kv8_combine_kernel<BF16>, dim3((unsigned)rows), dim3(256), 0, stream, m);
+    return hipGetLastError();
+}
+
+// The prefill kernel's parts, up to 8: many rows, so the bytes count and not the latency of a row.  A thread takes 8 columns
+// of a row through all parts, in part order.  (The whole call, wave a row / this: 32768 rows of 2 parts, d128 88.3 / 68.8 us;
+// 8192 of 8 107.4 / 102.7; but 2048 rows of 32 45.1 / 57.4, 1536 of 32 at d256 80.1 / 94.0: those go by the wave or workgroup.)
+template <bool BF16>
+__global__ void __launch_bounds__(256)
+kv8_combine_rows_kernel(const Kv8Merge a) {
+    const int cpr = a.d / 8;
+    const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x, rows = (int64_t)a.b * a.h * a.seqlen_q, row = at / cpr;
+    const int ch = (int)(at - row * cpr);
+    if (row >= rows) return;
+    const float *lse = a.lse + row, *o = a.o + row * a.d + ch * 8;
+    float m = -INFINITY;
+    for (int i = 0; i < a.num_splits; i++) m = fmaxf(m, lse[i * rows]);
+    const float ref = m == -INFINITY ? 0.f : m;
+    float sum = 0.f;
+    f32x4 a0 = {0, 0, 0, 0}, a1 = {0, 0, 0, 0};
+#pragma unroll 4
+    for (int i = 0; i < a.num_splits; i++) {
+        const float w = expf(lse[i * rows] - ref);            // (a part that saw no key of this row: 0, and zeros)
+        const float *src = o + i * rows * a.d;
+        sum += w;
+        a0 += *(const f32x4 *)src * w;
+        a1 += *(const f32x4 *)(src + 4) * w;
+    }
+    const bool none = sum == 0.f;                             // no part saw a key of this row
+    const float f = none ? 0.f : 1.f / sum;
+    const int bh = (int)(row / a.seqlen_q), pos = (int)(row - (int64_t)bh * a.seqlen_q), bidb = bh / a.h, head = bh - bidb * a.h;
+    if (ch == 0) a.out_lse[row] = none ? INFINITY : logf(sum) + ref;
+    kv8_store8<BF16>(a.out + bidb * a.out_bs + (int64_t)head * a.out_hs + (int64_t)pos * a.out_rs + ch * 8, a0 * f, a1 * f);
+}
+hipError_t run_kv8_merge(const KParams &p, hipStream_t stream) {   // (dense queries)
+    const Kv8Merge m{p.oaccum, p.lseaccum, p.lse, (unsigned short *)p.o, nullptr, nullptr, p.o_bs, p.o_rs, p.o_hs,
+                     p.b, p.h, p.d, p.seqlen_q, p.num_splits, p.seqlen_q, 0, p.h_ratio, 1, 1};
+    if (p.num_splits > 8) return p.is_bf16 ? launch_merge<true>(m, stream) : launch_merge<false>(m, stream);
+    const long long blocks = ((long long)p.b * p.h * p.seqlen_q * (p.d / 8) + 255) / 256;
+    if (blocks > 0x7fffffffLL) return hipErrorInvalidValue;
+    if (p.is_bf16) hipLaunchKernelGGL(kv8_combine_rows_kernel<true>, dim3((unsigned)blocks), dim3(256), 0, stream, m);
+    else hipLaunchKernelGGL(kv8_combine_rows_kernel<false>, dim3((unsigned)blocks), dim3(256), 0, stream, m);
+    return hipGetLastError();
+}
+
 // Rows of a decode workgroup (above head dim 128 the accumulators of 32 rows do not fit beside the loads) and
 // row blocks of the launch.
 int kv8_decode_rows(int d, int rows) { return d <= 128 && rows > 16 ? 32 : 16; }
@@ -820,13 +870,9 @@ static hipError_t launch_kv8(const KV8Params &a, hipStream_t stream) {
     hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3(A_NT), lds, stream, a, n_mblocks);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || p.num_splits <= 1) return e;
-    const long long rows = (long long)p.b * p.h * a.acc_sq;
-    if (rows > 0x7fffffffLL) return hipErrorInvalidValue;
     const Kv8Merge m{p.oaccum, p.lseaccum, p.lse, (unsigned short *)p.o, a.n_split, p.cu_seqlens_q, p.o_bs, p.o_rs, p.o_hs,
                      p.b, p.h, p.d, a.acc_sq, p.num_splits, p.seqlen_q, a.max_rows, p.h_ratio, n_mblocks, 16 * NR};
-    if (p.num_splits <= A_FEW_PARTS) hipLaunchKernelGGL(kv8_combine_few_kernel<BF16>, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, stream, m);
-    else hipLaunchKernelGGL(kv8_combine_kernel<BF16>, dim3((unsigned)rows), dim3(256), 0, stream, m);
-    return hipGetLastError();
+    return launch_merge<BF16>(m, stream);
 }
 
 template <int DP, bool BF16, int NR, bool NT, bool PAIR = false>

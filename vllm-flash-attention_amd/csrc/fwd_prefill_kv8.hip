@@ -13,6 +13,9 @@
 // Sums, the running maximum and O are fp32; P is rounded to 16 bits once in front of the second product, whose MFMA takes
 // 16-bit operands (with V exact in 16 bits a relative error of half a step per key, averaged by the sum).
 //
+// CODES = false: over the cache read back into contiguous 16-bit rows (args.k_out / v_out), which go straight into LDS
+// (buffer_load ... lds).  For long queries the conversions are then done once, not once for every 128 rows.
+//
 // MFMA-bound, in the shadow of it the conversions (one per two elements of K and V and 128 rows): b8 kv2048 h32/8 d128,
 // 640 rows 86 us; b4 kv8192, 384 rows 88 us.
 #include "vfa_kv8.h"
@@ -35,13 +38,15 @@ struct Cfg {
 
 // The grid walks (sequence, KV head, row block), with p.h = p.h_k, p.h_ratio = 1 and p.pack_gqa = the group's size.
 // SPLIT: blockIdx.y is a part of the keys, whose result goes to the fp32 partials.
-template <int DP, bool BF16, bool SPLIT>
+// DV <= DP: the products stop at column DV (the tiles keep the layout of DP columns, zero beyond the head dim).
+template <int DP, bool BF16, bool SPLIT, bool CODES, int DV = DP>
 __global__ void __launch_bounds__(kv8p::NT, DP == 256 ? 1 : 2)
 kv8_prefill_kernel(const KV8Params args, const int n_mblocks) {
     using namespace kv8p;
     using Cfg = kv8p::Cfg<DP>;
     const KParams &p = args.p;
-    constexpr int CPR = Cfg::CPR, KS = DP / 16, NDB = DP / 32;   // k-steps of QK^T, 32-column blocks of O
+    static_assert(DV % 32 == 0 && DV <= DP && 2 * DV > DP, "DV");
+    constexpr int CPR = Cfg::CPR, KS = DV / 16, NDB = DV / 32;   // k-steps of QK^T, 32-column blocks of O
     extern __shared__ __attribute__((aligned(16))) char smem[];
 
     const int tid = threadIdx.x;
@@ -110,6 +115,25 @@ kv8_prefill_kernel(const KV8Params args, const int n_mblocks) {
         return;
     }
 
+    // ---- read back: a wave instruction fills 1 KiB of LDS in lane order, RPI rows, so a lane fetches the chunk that the XOR
+    // swizzle places at its slot; the rows of a wave's instructions are RPI * NW apart, which leaves a lane's swizzle as it
+    // is, or (8 apart, d256) alternates between two.  Chunks past the head dim and rows past the sequence are out of the
+    // buffer's range: zeros. ----
+    constexpr int RPI = 64 / CPR, NI = BN / (RPI * NW), NVAR = (RPI * NW) % 16 == 0 ? 1 : 2;
+    static_assert((RPI * NW) % 8 == 0, "swizzle of a lane's rows");
+    const unsigned k_rs2 = (unsigned)args.ko_rs * 2, v_rs2 = (unsigned)args.vo_rs * 2;
+    const auto k16 = __builtin_amdgcn_make_buffer_rsrc((unsigned short *)args.k_out + bidb * args.ko_bs + hk * args.ko_hs, 0,
+                                                       CODES ? 0u : (unsigned)(sk - 1) * k_rs2 + p.d * 2, 0x00020000);
+    const auto v16 = __builtin_amdgcn_make_buffer_rsrc((unsigned short *)args.v_out + bidb * args.vo_bs + hk * args.vo_hs, 0,
+                                                       CODES ? 0u : (unsigned)(sk - 1) * v_rs2 + p.d * 2, 0x00020000);
+    unsigned k_voff[NVAR], v_voff[NVAR];
+#pragma unroll
+    for (int e = 0; e < NVAR; e++) {
+        const int row0 = RPI * wave + lane / CPR, ch = (lane % CPR) ^ swz<DP>(row0 + RPI * NW * e);
+        k_voff[e] = ch * 8 < p.d ? (unsigned)row0 * k_rs2 + ch * 16 : 0x80000000u;
+        v_voff[e] = ch * 8 < p.d ? (unsigned)row0 * v_rs2 + ch * 16 : 0x80000000u;
+    }
+
     // ---- the tile's codes: 16-byte pieces per thread, and the scales of the wave's rows ----
     const int bidb_cache = p.cache_batch_idx ? p.cache_batch_idx[bidb] : bidb;
     const int *bt = p.block_table ? p.block_table + (int64_t)bidb * p.bt_bs : nullptr;
@@ -128,13 +152,28 @@ kv8_prefill_kernel(const KV8Params args, const int n_mblocks) {
         return min(n * BN + (((wave * 64 + i * NT) / PPR) & ~15), (sk - 1) & ~15);
     };
     auto load_pages = [&](const int n) __attribute__((always_inline)) {
+        if constexpr (!CODES) return;
 #pragma unroll
         for (int i = 0; i < NP; i++) {
             if (bt) pg8[i] = bt[kv8_div(group16(n, i) >> 4, args.page_mul, args.page_sh)];
             else pg8[i] = bidb_cache;
         }
     };
-    auto load_tile = [&](const int n) __attribute__((always_inline)) {
+    auto load_tile = [&](const int n, auto BUFC) __attribute__((always_inline)) {
+        if constexpr (!CODES) {
+#ifdef __HIP_DEVICE_COMPILE__   // (loads of 16 bytes to LDS are this target's: the host pass does not take them)
+            constexpr int BUF = decltype(BUFC)::value;
+#pragma unroll
+            for (int i = 0; i < NI; i++) {
+                typedef __attribute__((address_space(3))) void *lds_ptr;
+                const unsigned at = (unsigned)(n * BN + RPI * NW * i);
+                char *to = smem + BUF * Cfg::TILE_BYTES + (wave + NW * i) * 1024;
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(k16, (lds_ptr)to, 16, k_voff[i % NVAR] + at * k_rs2, 0, 0, 0);
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(v16, (lds_ptr)(to + 2 * Cfg::TILE_BYTES), 16, v_voff[i % NVAR] + at * v_rs2, 0, 0, 0);
+            }
+#endif
+            return;
+        }
 #pragma unroll
         for (int i = 0; i < NP; i++) {
             const int g16 = group16(n, i);
@@ -151,6 +190,10 @@ kv8_prefill_kernel(const KV8Params args, const int n_mblocks) {
     };
     auto store_tile = [&](const int n, auto BUFC) __attribute__((always_inline)) {
         constexpr int BUF = decltype(BUFC)::value;
+        if constexpr (!CODES) {
+            __builtin_amdgcn_s_waitcnt(0x0F70);   // vmcnt(0): this wave's part of the tile is in LDS
+            return;
+        }
 #pragma unroll
         for (int i = 0; i < NP; i++) vs8[i] |= bad8[i];
         if (n * BN < vis_lo || (n + 1) * BN > vis_hi) {   // V of keys that no row sees must not count, whatever stands there
@@ -216,7 +259,7 @@ kv8_prefill_kernel(const KV8Params args, const int n_mblocks) {
     constexpr int ROWB = DP * 2;
 
     load_pages(n_max - 1);
-    load_tile(n_max - 1);
+    load_tile(n_max - 1, std::integral_constant<int, 0>{});
     if (n_max - 2 >= n_min) load_pages(n_max - 2);
     store_tile(n_max - 1, std::integral_constant<int, 0>{});
     __syncthreads();
@@ -226,7 +269,7 @@ kv8_prefill_kernel(const KV8Params args, const int n_mblocks) {
         constexpr int BUF = decltype(BUFC)::value;
         const bool has_next = n > n_min;
         if (has_next) {
-            load_tile(n - 1);
+            load_tile(n - 1, std::integral_constant<int, BUF ^ 1>{});
             if (n - 2 >= n_min) load_pages(n - 2);
         }
         const char *kb = smem + BUF * Cfg::TILE_BYTES;
@@ -430,30 +473,36 @@ kv8_prefill_kernel(const KV8Params args, const int n_mblocks) {
     }
 }
 
-template <int DP, bool BF16, bool SPLIT>
+template <int DP, bool BF16, bool SPLIT, bool CODES, int DV>
 static hipError_t launch_kv8_prefill(const KV8Params &a, hipStream_t stream) {
     const KParams &p = a.p;
     const int n_mblocks = (p.seqlen_q * p.pack_gqa + kv8p::BM - 1) / kv8p::BM;
     const long long blocks = (long long)n_mblocks * p.b * p.h;   // (p.h: KV heads)
     if (blocks <= 0) return hipSuccess;
     if (blocks > 0x7fffffffLL) return hipErrorInvalidValue;
-    auto kern = kv8_prefill_kernel<DP, BF16, SPLIT>;
+    auto kern = kv8_prefill_kernel<DP, BF16, SPLIT, CODES, DV>;
     static std::atomic<uint64_t> lds_set{0};
     if (hipError_t e = set_dyn_lds_once((const void *)kern, kv8p::Cfg<DP>::LDS_BYTES, lds_set); e != hipSuccess) return e;
     hipLaunchKernelGGL(kern, dim3((unsigned)blocks, SPLIT ? (unsigned)p.num_splits : 1u), dim3(kv8p::NT), kv8p::Cfg<DP>::LDS_BYTES, stream, a, n_mblocks);
     return hipGetLastError();
 }
-template <int DP>
+template <int DP, bool CODES, int DV = DP>
 static hipError_t launch_kv8_prefill_type(const KV8Params &a, hipStream_t stream) {
-    if (a.p.num_splits > 1) return a.p.is_bf16 ? launch_kv8_prefill<DP, true, true>(a, stream) : launch_kv8_prefill<DP, false, true>(a, stream);
-    return a.p.is_bf16 ? launch_kv8_prefill<DP, true, false>(a, stream) : launch_kv8_prefill<DP, false, false>(a, stream);
+    if (a.p.num_splits > 1) return a.p.is_bf16 ? launch_kv8_prefill<DP, true, true, CODES, DV>(a, stream) : launch_kv8_prefill<DP, false, true, CODES, DV>(a, stream);
+    return a.p.is_bf16 ? launch_kv8_prefill<DP, true, false, CODES, DV>(a, stream) : launch_kv8_prefill<DP, false, false, CODES, DV>(a, stream);
 }
-hipError_t run_fwd_kv8_prefill(const KV8Params &a_in, hipStream_t stream) {
+// codes: over the cache itself; else over what was read back of it, whose rows a 32-bit offset reaches (kv8_read_back_ok)
+hipError_t run_fwd_kv8_prefill(const KV8Params &a_in, bool codes, hipStream_t stream) {
     KV8Params a = a_in;
     a.p.pack_gqa = a_in.p.h_ratio;   // the grid walks the KV heads
     a.p.h = a_in.p.h_k;
     a.p.h_ratio = 1;
-    return a.p.d <= 64 ? launch_kv8_prefill_type<64>(a, stream) : a.p.d <= 128 ? launch_kv8_prefill_type<128>(a, stream) : launch_kv8_prefill_type<256>(a, stream);
+    const int d = a.p.d;
+    if (codes) return d <= 64 ? launch_kv8_prefill_type<64, true>(a, stream) : d <= 128 ? launch_kv8_prefill_type<128, true>(a, stream) : launch_kv8_prefill_type<256, true>(a, stream);
+    if (d <= 64) return launch_kv8_prefill_type<64, false>(a, stream);
+    if (d <= 96) return launch_kv8_prefill_type<128, false, 96>(a, stream);
+    return d <= 128 ? launch_kv8_prefill_type<128, false>(a, stream) : launch_kv8_prefill_type<256, false>(a, stream);
 }
+bool kv8_read_back_ok(int64_t seqlen_k, int h_k, int d) { return (seqlen_k + 256) * h_k * d * 2 < (int64_t)1 << 30; }
 
 }  // namespace vfa

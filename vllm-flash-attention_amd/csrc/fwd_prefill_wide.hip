@@ -548,13 +548,18 @@ fwd_prefill_wide_kernel(const KParams p, const int n_mblocks) {
     const bool bad = (l_tot == 0.f) || (l_tot != l_tot);
     const float inv = bad ? 1.f : 1.f / l_tot;
     if (hh == 0 && q0w + r < sq) lse_g[q0w + r] = bad ? INFINITY : m_run * p.scale + __logf(l_tot);
+#ifdef VFA_KV8_TU   // (a row that sees no key is zero; its O is a sum of zero weights times V, NaN if V is)
+#define WIDE_RESULT(j) (l_tot == 0.f ? 0.f : o_read<db, 4 * g4 + (j)>() * inv)
+#else
+#define WIDE_RESULT(j) (o_read<db, 4 * g4 + (j)>() * inv)
+#endif
     static_for<NDB>([&](auto DB) {
         constexpr int db = decltype(DB)::value;
         static_for<4>([&](auto G4) {
             constexpr int g4 = decltype(G4)::value;
             i32x2 w;
-            w[0] = pack2<BF16>(o_read<db, 4 * g4 + 0>() * inv, o_read<db, 4 * g4 + 1>() * inv);
-            w[1] = pack2<BF16>(o_read<db, 4 * g4 + 2>() * inv, o_read<db, 4 * g4 + 3>() * inv);
+            w[0] = pack2<BF16>(WIDE_RESULT(0), WIDE_RESULT(1));
+            w[1] = pack2<BF16>(WIDE_RESULT(2), WIDE_RESULT(3));
             *(i32x2 *)(ob + r * O_ROWB + (32 * db + 8 * g4 + 4 * hh) * 2) = w;
         });
     });
@@ -594,6 +599,8 @@ static hipError_t launch_wide_fwd(const KParams &p, hipStream_t stream) {
 
 #ifdef VFA_WIDE_PAGED_TU
 hipError_t run_fwd_prefill_wide_paged(const KParams &p, hipStream_t stream) { return launch_wide_fwd<true>(p, stream); }
+#elif defined(VFA_KV8_TU)
+hipError_t run_fwd_kv8_wide(const KParams &p, hipStream_t stream) { return launch_wide_fwd<false>(p, stream); }
 #else
 hipError_t run_fwd_prefill_wide_paged(const KParams &p, hipStream_t stream);   // fwd_prefill_wide_paged.hip
 

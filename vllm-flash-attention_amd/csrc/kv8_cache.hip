@@ -217,12 +217,12 @@ struct KV8Out {                          // what is read back goes here
     int64_t k_bs, k_rs, k_hs, v_bs, v_rs, v_hs;
     int seqlen, n_new;                   // dense: rows a sequence; tokens that the call has appended
     int tpw, cph;                        // rows a workgroup, 8-element chunks of a head's row
-    // for the 16-bit attention kernels: the lengths they are to see, and the window on the left (-1: none)
+    // for the attention kernels over what is read back: the lengths they are to see, and the window on the left (-1: none)
     int *lens;
     const int *cu_q;
     int seqlen_q, ratio, min_rows, wl;
 };
-constexpr int D_TILE = 256;              // keys of their largest tile
+constexpr int D_TILE = 64;               // keys of a tile of those kernels
 
 // A workgroup takes `tpw` output rows (tokens): its first threads find each row's sequence (ragged: by bisection of the
 // offsets), page and scale row, then all threads copy 8 codes at a time, so that a wave's store is 1 KiB without gaps
@@ -241,7 +241,7 @@ kv8_dequantize_kernel(const KV8Out o, const KV8CacheArgs a) {
     const int tpw = o.tpw, cph = o.cph;
     const int tid = threadIdx.x;
     const int64_t first = (int64_t)blockIdx.x * tpw;
-    // Read back for the 16-bit attention kernels: sequences that are the decode kernel's have length 0 there, and
+    // Read back for the attention kernels: sequences that are the decode kernel's have length 0 there, and
     // rows behind a sequence are not read, so not written.  Neither are keys in front of the window of the sequence's
     // first query, but for those in the first tile of a visible one: they are zeros, whatever the cache has there (a
     // released page, a NaN code), because their weight 0 is multiplied with them.
