@@ -258,8 +258,9 @@ typedef struct vfa_kv8_params {
 /* Write new tokens at positions cu_seqlens_k[i] .. of every sequence.  A block's scale is the least power of
  * two with max |x| <= 448 * scale over the tokens written to it (not under 2^-126); tokens that join a block
  * which holds some already can only raise it, and what the block holds is then re-encoded.  A block that is
- * written from its first token on starts anew.  Rounding is to nearest even; NaN and the infinities become
- * NaN codes and do not count for the scale.  Rows behind the new tokens stay as they are.  Two sequences must
+ * written from its first token on starts anew.  Rounding is to nearest even, but from a scale of 2^8 (fp16) or
+ * 2^120 (bf16) on codes stop at 240: the next would stand for 2^16 or 2^128, which the tokens' type does not
+ * have.  NaN and the infinities become NaN codes and do not count for the scale.  Rows behind the new tokens stay as they are.  Two sequences must
  * not write to one block. */
 int vfa_kv8_quantize(const vfa_kv8_params *p);
 
@@ -269,10 +270,16 @@ int vfa_kv8_dequantize(const vfa_kv8_params *p);
 
 /* Attention of q (dense (b, seqlen_q, h, d), or ragged with cu_seqlens_q) over the cache: a.q, a.out,
  * a.softmax_lse, masks and ALiBi as for vfa_mha_fwd_kvcache.  With a.knew the new tokens (dense) are written
- * first and attended.  a.num_splits: 0 = chosen here, 1 = no split, n = the keys in as many parts as n of every
- * sequence would be (by the lengths: longer sequences get more, at most n + 1).  Partial results
- * -- and for long queries the cache in 16 bits -- go to `workspace` (a.oaccum and a.softmax_lseaccum are not
- * used); nothing in it has to be set. */
+ * first and attended.  A key that no row of its sequence sees has no part in any result, whatever stands there,
+ * and a row that sees no key is zero; a NaN or an infinity in V of a key that some row sees can reach the
+ * sequence's other rows too (0 * NaN).
+ * a.num_splits: 0 = chosen here, 1 = no split, n = the keys in as many parts as n of every sequence would be (by the
+ * lengths: longer sequences get more, at most n + 1); with more than 64 (query position, head) rows per KV head
+ * n equal parts of what a block of rows sees, at most one per 256 tokens of seqlen_k, and none in a ragged batch.
+ * How a call is carried out, and its workspace, go by seqlen_k and not by the lengths, which only the device
+ * knows: a block table should not be much wider than its longest sequence.
+ * Partial results -- and for long queries the cache in 16 bits -- go to `workspace` (a.oaccum and
+ * a.softmax_lseaccum are not used); nothing in it has to be set. */
 int vfa_kv8_mha_fwd(const vfa_kv8_params *p);
 
 /* Bytes of workspace that vfa_kv8_mha_fwd needs for these arguments (of the pointers only whether they are

@@ -628,11 +628,16 @@ extern "C" int vfa_kv8_dequantize(const vfa_kv8_params *p) {
 }
 
 // Most (query position, head) rows of a KV head that the decode kernel takes, and the rows from which reading the
-// cache back and the 16-bit kernels are ahead of the prefill kernel over the codes, at head dims up to 128 and above:
-// the codes' conversion is done once, not once for every 128 rows, and those kernels are tuned for long queries.
-// us over the codes / over the cache read back, h32/8 d128: b8 kv2048, 640 rows 86 / 85, 1024 rows 89.5 / 89, 4096 rows
-// 260 / 227; b4 kv8192, 384 rows 88 / 113, 2048 rows 322 / 296.  h8/4 d256: b8 kv2048, 96 rows 47 / 51, 192 rows 85 / 72,
-// 512 rows 132 / 82; b4 kv8192, 96 rows 88 / 104, 192 rows 132 / 120.
+// cache back into 16 bits first is ahead of the prefill kernel over the codes, at head dims up to 128 and above: the codes'
+// conversion is then done once, not once for every 128 rows (and above 128 the hand-pipelined kernel takes the rows).
+// us by the decode / by the prefill kernel: h32/8 d128 b32 kv4096, 36 rows 83 / 93, 64 rows 97 / 96, 96 rows 142 / 106; b2 kv32768,
+// 36 rows 48 / 51, 64 rows 53 / 54, 96 rows 66 / 58; h8/2 d256 b16 kv4096, 36 rows 34 / 68, 64 rows 40 / 72; h16/4 d64 b32
+// kv4096, 36 rows 38 / 36, 64 rows 45 / 37.
+// us over the codes / over the cache read back: h32/8 d128 b8 kv2048, 640 rows 85 / 78, 1024 rows 88 / 89, 1536 rows 131 / 117,
+// 4096 rows 254 / 222; b4 kv8192, 384 rows 86 / 101, 1024 rows 178 / 175, 2048 rows 317 / 283; h32/8 d64 b8 kv2048, 1024 rows
+// 53 / 57, 2048 rows 90 / 87; h8/4 d256 b8 kv2048, 96 rows 46 / 53, 192 rows 81 / 59, 512 rows 123 / 81.  Under a window, b4
+// kv16384 h32/8 d128: 127 keys, 4096 rows 37 / 49; 1023 keys, 1024 rows 46 / 54, 4096 rows 104 / 98; 4095 keys 1024 rows 103 / 104,
+// 4096 rows 334 / 288.
 constexpr int VFA_KV8_DECODE_ROWS = 64, VFA_KV8_READ_BACK_ROWS = 1024, VFA_KV8_READ_BACK_ROWS_WIDE = 192;
 
 // How a call is carried out: sequences of few (query position, head) rows by the decode kernel, the others by the
@@ -656,7 +661,9 @@ static int kv8_plan(const vfa_kv8_params *p, Kv8Plan &w) {
     const int ratio = a.h / a.h_k, cus = num_cus();
     const long long rows = (long long)a.seqlen_q * ratio;
     w.prefill = rows > VFA_KV8_DECODE_ROWS;
-    // beside longer ones only sequences of one 16-row block (of one query position, if that is more rows)
+    // Beside longer ones only sequences of one 16-row block (of one query position, if that is more rows).  us with 16 / 32 /
+    // 64 as the limit, seven of eight sequences short: h32/8 d128 b16 kv8192 beside 512 positions, 16 rows each 491 / 493 / 522,
+    // 20 rows 737 / 493 / 522, 64 rows 741 / 758 / 519; beside 64 positions, 16 rows 340 / 344 / 378, 20 rows 271 / 356 / 392.
     w.dec_rows = !w.prefill ? VFA_KV8_DECODE_ROWS : ratio <= 16 ? 16 : ratio <= 32 ? 32 : VFA_KV8_DECODE_ROWS;
     // a dense batch is all one kind; of a ragged one with long members only the lengths on the device know
     w.decode = !w.prefill || (a.cu_seqlens_q && ratio <= w.dec_rows);

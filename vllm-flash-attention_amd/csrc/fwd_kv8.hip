@@ -18,6 +18,9 @@
 //   * S^T = K Q^T by 16x16x32 MFMAs with the key on the accumulator's rows and the query row on the lane.  A
 //     lane's K operand is 16 consecutive codes of one key: two k-steps, loaded straight from memory to
 //     registers (which columns a k-step takes is free as long as Q agrees);
+//   * P is rounded to 16 bits in front of the second product, whose MFMA takes 16-bit operands (V is exact in them): at most
+//     half a step per key, 2^-8 in bf16 and 2^-11 in fp16 of the weight, which the sum over keys averages out; its sum l
+//     is taken in fp32 before that.  Against 64 bits the error is up to 6 % above that of a P kept in fp32.
 //   * P^T of 32 keys is, in the registers it is computed in, the B operand of O^T += V^T P^T if V^T takes its
 //     keys in the order {4g .. 4g+3, 16+4g .. 16+4g+3} for lane group g: ds_read_b64_tr_b8 reads any 8 rows,
 //     so V goes through a wave-private LDS image as codes and comes back transposed, to be converted there.

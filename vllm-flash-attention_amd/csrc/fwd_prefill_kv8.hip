@@ -19,6 +19,7 @@
 // MFMA-bound, in the shadow of it the conversions (one per two elements of K and V and 128 rows): b8 kv2048 h32/8 d128,
 // 640 rows 86 us; b4 kv8192, 384 rows 88 us.
 #include "vfa_kv8.h"
+#include <algorithm>
 #include <type_traits>
 
 namespace vfa {
@@ -36,7 +37,8 @@ struct Cfg {
 };
 }  // namespace kv8p
 
-// The grid walks (sequence, KV head, row block), with p.h = p.h_k, p.h_ratio = 1 and p.pack_gqa = the group's size.
+// The grid walks (sequence, KV head, row block), with p.h = p.h_k, p.pack_gqa = the group's size and p.h_ratio = the row
+// blocks of a (sequence, KV head) that stand next to each other in the launch (n_mblocks: such runs of them).
 // SPLIT: blockIdx.y is a part of the keys, whose result goes to the fp32 partials.
 // DV <= DP: the products stop at column DV (the tiles keep the layout of DP columns, zero beyond the head dim).
 template <int DP, bool BF16, bool SPLIT, bool CODES, int DV = DP>
@@ -56,6 +58,8 @@ kv8_prefill_kernel(const KV8Params args, const int n_mblocks) {
 
     int bidb, hk, m_block;
     map_block(p, n_mblocks, 32 * (DP == 256 ? 1 : 2), bidb, hk, m_block);
+    m_block = m_block * p.h_ratio + p.h_ratio - 1 - hk % p.h_ratio;
+    hk /= p.h_ratio;
     const int ratio = p.pack_gqa;
 
     const BlockInfo bi(p, bidb);
@@ -473,11 +477,19 @@ kv8_prefill_kernel(const KV8Params args, const int n_mblocks) {
     }
 }
 
+// Of a ragged batch the short sequences' workgroups leave at once.  With the row blocks of different sequences in turn the
+// workgroups that stay are a fixed number apart, and the dispatcher, which goes round the chip's parts, gives them to the
+// same few; all blocks of a sequence next to each other reach every part.  (h32/8 d128 b16 kv8192, a quarter of the
+// sequences up to 1024 queries: in turn 631 us, runs of 2 / 4 / 8 370 / 365 / 363, all 364; prompts b16 up to 4096 795, 795 /
+// 607 / 606, 616; h16/16 b16 up to 2048 177, 176 / 181 / 183, 176; d64 b32 up to 2048 232, 233 / 197 / 195, 195.)
+static int row_block_run(const KParams &p, int n_mblocks) { return p.cu_seqlens_q ? std::max(1, n_mblocks) : 1; }
 template <int DP, bool BF16, bool SPLIT, bool CODES, int DV>
-static hipError_t launch_kv8_prefill(const KV8Params &a, hipStream_t stream) {
-    const KParams &p = a.p;
-    const int n_mblocks = (p.seqlen_q * p.pack_gqa + kv8p::BM - 1) / kv8p::BM;
-    const long long blocks = (long long)n_mblocks * p.b * p.h;   // (p.h: KV heads)
+static hipError_t launch_kv8_prefill(KV8Params a, hipStream_t stream) {
+    KParams &p = a.p;
+    const int all = (p.seqlen_q * p.pack_gqa + kv8p::BM - 1) / kv8p::BM;
+    p.h_ratio = row_block_run(p, all);
+    const int n_mblocks = (all + p.h_ratio - 1) / p.h_ratio;
+    const long long blocks = (long long)n_mblocks * p.h_ratio * p.b * p.h;   // (p.h: KV heads)
     if (blocks <= 0) return hipSuccess;
     if (blocks > 0x7fffffffLL) return hipErrorInvalidValue;
     auto kern = kv8_prefill_kernel<DP, BF16, SPLIT, CODES, DV>;
@@ -496,7 +508,6 @@ hipError_t run_fwd_kv8_prefill(const KV8Params &a_in, bool codes, hipStream_t st
     KV8Params a = a_in;
     a.p.pack_gqa = a_in.p.h_ratio;   // the grid walks the KV heads
     a.p.h = a_in.p.h_k;
-    a.p.h_ratio = 1;
     const int d = a.p.d;
     if (codes) return d <= 64 ? launch_kv8_prefill_type<64, true>(a, stream) : d <= 128 ? launch_kv8_prefill_type<128, true>(a, stream) : launch_kv8_prefill_type<256, true>(a, stream);
     if (d <= 64) return launch_kv8_prefill_type<64, false>(a, stream);

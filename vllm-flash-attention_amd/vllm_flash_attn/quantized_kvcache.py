@@ -39,8 +39,9 @@ def quantize_kvcache(k, v, k_cache, v_cache, k_scale, v_scale, cache_seqlens: Un
 
     A block's scale is the least power of two that brings the largest magnitude written to it to at most 448 times the
     scale (2^-126 at least).  Tokens that join a block which holds some already can only raise its scale; what it holds
-    is then re-encoded.  A block written from its first token on starts anew.  Values are rounded to nearest even;
-    NaN and infinities become NaN and do not count for the scale.  Tokens past the capacity are dropped; rows behind
+    is then re-encoded.  A block written from its first token on starts anew.  Values are rounded to nearest even, but
+    from a scale of 2^8 (fp16) or 2^120 (bf16) on to at most 240 times the scale: the next code would stand for 2^16 or
+    2^128, which the type does not have.  NaN and infinities become NaN and do not count for the scale.  Tokens past the capacity are dropped; rows behind
     the new tokens stay as they are.  Two sequences of one call must not write to the same block."""
     if cu_seqlens is not None and max_seqlen is None:
         raise ValueError("max_seqlen is required with cu_seqlens")
@@ -80,9 +81,13 @@ def flash_attn_with_quantized_kvcache(q, k_cache, v_cache, k_scale, v_scale, k=N
 
     If k / v (batch_size, seqlen_new, nheads_k, headdim) are given (dense q only) they are written first, as by
     quantize_kvcache, and attended.  The query is used as it is: rotate q and k beforehand (qk_norm_rotary_func).
-    causal, window_size, alibi_slopes, num_splits, out as in flash_attn_with_kvcache; softmax_scale > 0.  Returns out,
-    shaped like q; a row that sees no key is zero.  An fp16 query over values past fp16's range (a cache that bf16 tokens
-    were written to) sees infinities.  No backward."""
+    causal, window_size, alibi_slopes, num_splits, out as in flash_attn_with_kvcache, but num_splits does not cut the
+    keys of a ragged batch's longer queries; softmax_scale > 0.  Returns out, shaped like q; rows of a ragged batch behind
+    its last sequence stay as they are in `out`.  A row that sees no key is zero, and a key that no row of its sequence sees
+    has no part in any result, whatever stands there; a NaN or an infinity in v of a key that some row sees can make the
+    sequence's other rows NaN too.  An fp16 query over values past fp16's range (a cache that bf16 tokens were written to)
+    sees infinities.  How the work is cut up goes by the width of block_table: one not much wider than the longest sequence
+    is fastest.  No backward."""
     if (cu_seqlens_q is None) != (max_seqlen_q is None):
         raise ValueError("cu_seqlens_q and max_seqlen_q go together")
     if softmax_scale is None:
