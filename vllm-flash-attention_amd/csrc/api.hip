@@ -547,6 +547,17 @@ extern "C" int vfa_dispatch_geometry(const vfa_params *p, int kernel) {
 // 8-bit KV cache
 static bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
 
+// The window as it is given: a negative side has no end.  (fill_common ends it at the capacity, and takes a side of the
+// capacity or more for endless: with more queries than keys neither is the same.)
+static void kv8_window(const vfa_params &a, KParams &k) {
+    constexpr int far = 1 << 30;
+    const int wl = a.window_size_left, wr = a.is_causal ? 0 : a.window_size_right;
+    k.is_causal = wl < 0 && wr == 0;
+    k.is_local = (wl >= 0 || wr >= 0) && !k.is_causal;
+    k.wl = wl < 0 ? far : std::min(wl, far);
+    k.wr = wr < 0 ? far : std::min(wr, far);
+}
+
 static int kv8_fill(const vfa_kv8_params *p, vfa::KV8Params &k) {
     VFA_CHECK(p != nullptr, "null params");
     const vfa_params &a = p->a;
@@ -568,6 +579,7 @@ static int kv8_fill(const vfa_kv8_params *p, vfa::KV8Params &k) {
     for (int64_t r : {a.k_row_stride, a.v_row_stride, p->k_scale_row_stride, p->v_scale_row_stride})
         VFA_CHECK(r >= 0 && r < (int64_t)1 << 27, "8-bit KV cache: row strides must be under 128 MiB");
     fill_common(&a, k.p, a.seqlen_q, a.seqlen_k);
+    kv8_window(a, k.p);
     k.p.k_cumulative = 0;
     k.ks = (unsigned char *)p->k_scale; k.vs = (unsigned char *)p->v_scale;
     k.ks_bs = p->k_scale_batch_stride; k.ks_rs = p->k_scale_row_stride; k.ks_hs = p->k_scale_head_stride;
@@ -662,8 +674,9 @@ static int kv8_plan(const vfa_kv8_params *p, Kv8Plan &w) {
     const long long rows = (long long)a.seqlen_q * ratio;
     w.prefill = rows > VFA_KV8_DECODE_ROWS;
     // Beside longer ones only sequences of one 16-row block (of one query position, if that is more rows).  us with 16 / 32 /
-    // 64 as the limit, seven of eight sequences short: h32/8 d128 b16 kv8192 beside 512 positions, 16 rows each 491 / 493 / 522,
-    // 20 rows 737 / 493 / 522, 64 rows 741 / 758 / 519; beside 64 positions, 16 rows 340 / 344 / 378, 20 rows 271 / 356 / 392.
+    // 64 as the limit, seven of eight sequences short: h32/8 d128 b16 kv8192 beside 512 positions, 16 rows each 308 / 312 / 339,
+    // 20 rows 567 / 311 / 339, 64 rows 577 / 590 / 339; beside 64 positions, 16 rows 341 / 346 / 380, 20 rows 271 / 359 / 393;
+    // h8/2 d256 b16 kv4096 beside 128 positions 152 / 154 / 165 and 156 / 154 / 166.
     w.dec_rows = !w.prefill ? VFA_KV8_DECODE_ROWS : ratio <= 16 ? 16 : ratio <= 32 ? 32 : VFA_KV8_DECODE_ROWS;
     // a dense batch is all one kind; of a ragged one with long members only the lengths on the device know
     w.decode = !w.prefill || (a.cu_seqlens_q && ratio <= w.dec_rows);
@@ -801,6 +814,7 @@ extern "C" int vfa_kv8_mha_fwd(const vfa_kv8_params *p) {
             q.block_table = nullptr; q.cache_batch_idx = nullptr; q.knew = q.vnew = nullptr;
             KParams k16;
             fill_common(&q, k16, q.seqlen_q, q.seqlen_k);
+            kv8_window(a, k16);
             k16.k_cumulative = 0;
             e = vfa::run_fwd_kv8_wide(k16, stream);
         } else {
