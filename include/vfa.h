@@ -269,7 +269,8 @@ int vfa_kv8_quantize(const vfa_kv8_params *p);
 int vfa_kv8_dequantize(const vfa_kv8_params *p);
 
 /* Attention of q (dense (b, seqlen_q, h, d), or ragged with cu_seqlens_q) over the cache: a.q, a.out,
- * a.softmax_lse, masks and ALiBi as for vfa_mha_fwd_kvcache.  With a.knew the new tokens (dense) are written
+ * a.softmax_lse, masks and ALiBi as for vfa_mha_fwd_kvcache, but the LSE is that of the scores with the bias
+ * -slope * |distance| in every mode, and a negative side of the window has no end.  With a.knew the new tokens (dense) are written
  * first and attended.  A key that no row of its sequence sees has no part in any result, whatever stands there,
  * and a row that sees no key is zero; a NaN or an infinity in V of a key that some row sees can reach the
  * sequence's other rows too (0 * NaN).

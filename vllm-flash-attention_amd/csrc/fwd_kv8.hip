@@ -497,14 +497,13 @@ fwd_kv8_kernel(const KV8Params args, const int n_mblocks) {
         if (has_alibi) {
 #pragma unroll
             for (int r = 0; r < NR; r++) {
-                const float at = p.is_causal ? 0.f : (float)(seen.shift + pos[r]);
+                // (by the distance, in the causal case too: slope * key, equal up to a constant of the row, is large over
+                // a long cache, and with it the rounding of every score)
+                const int at = seen.shift + pos[r] - (k0 + 4 * g);
 #pragma unroll
                 for (int t = 0; t < 2; t++)
 #pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const float key = (float)(k0 + 16 * t + 4 * g + i);
-                        s[r][t][i] += slope[r] * (p.is_causal ? key : -fabsf(at - key));
-                    }
+                    for (int i = 0; i < 4; i++) s[r][t][i] -= slope[r] * fabsf((float)(at - 16 * t - i));
             }
         }
         if (need) {

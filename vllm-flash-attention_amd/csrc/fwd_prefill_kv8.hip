@@ -241,7 +241,8 @@ kv8_prefill_kernel(const KV8Params args, const int n_mblocks) {
     float l_run = 0.f;        // running sum, partial per lane half
 
     // ALiBi in linear form where every visible key has col <= row + sk - sq: the bias -slope |row + sk - sq - col| is then
-    // slope * col plus a constant of the row, which cancels in the softmax and returns in the LSE.  cref keeps magnitudes small.
+    // slope * (col - cref) plus a constant of the row, which cancels in the softmax and returns in the LSE; cref, the block's
+    // first diagonal column, keeps magnitudes small.
     float alibi = 0.f;
     const bool has_alibi = p.alibi_slopes != nullptr;
     if (has_alibi) alibi = p.alibi_slopes[(int64_t)bidb * p.alibi_bs + head0 + (q0w + r) % ratio] / p.scale;
@@ -433,10 +434,7 @@ kv8_prefill_kernel(const KV8Params args, const int n_mblocks) {
     // (a row that sees no key is zero; its O is a sum of zero weights times V, NaN if V is)
     auto result = [&](const float x) __attribute__((always_inline)) -> float { return l_tot == 0.f ? 0.f : x * inv; };
     float lse = bad ? (SPLIT ? -INFINITY : INFINITY) : m_run * p.scale + __logf(l_tot);
-    if (alibi_lin && !bad) {  // the row constant left out of the linear form
-        const float slope = alibi * p.scale;
-        lse += p.is_causal ? slope * (float)cref : -slope * (float)(seen.shift + pos_l - cref);
-    }
+    if (alibi_lin && !bad) lse -= alibi * p.scale * (float)(seen.shift + pos_l - cref);   // the row constant left out of the linear form
     if (hh == 0 && q0w + r < rows) lse_g[stat_off(q0w + r)] = lse;
 
     if constexpr (SPLIT) {
