@@ -16,8 +16,9 @@
 // CODES = false: over the cache read back into contiguous 16-bit rows (args.k_out / v_out), which go straight into LDS
 // (buffer_load ... lds).  For long queries the conversions are then done once, not once for every 128 rows.
 //
-// MFMA-bound, in the shadow of it the conversions (one per two elements of K and V and 128 rows): b8 kv2048 h32/8 d128,
-// 640 rows 86 us; b4 kv8192, 384 rows 88 us.
+// MFMA-bound, in the shadow of it the conversions (one per two elements of K and V and 128 rows).  The whole call, h32/8
+// d128: over the codes b8 kv2048 640 rows 85 us, b4 kv8192 384 rows 86 us; read back b8 kv2048 4096 rows 222 us, b4 kv4096
+// 16384 rows 571 us.
 #include "vfa_kv8.h"
 #include <algorithm>
 #include <type_traits>
