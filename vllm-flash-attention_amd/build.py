@@ -27,12 +27,14 @@ LIB = os.path.join(HERE, "libvfa_hip.so")
 HIP_SOURCES = ["api.hip", "fwd_prefill.hip", "fwd_splitkv.hip", "bwd.hip", "fwd_prefill_drop.hip",
                "bwd_drop.hip", "fwd_prefill_split.hip", "bwd_dkdv_w64.hip", "fwd_prefill_persist.hip", "bwd_dq_persist.hip",
                "bwd_dkdv_wide.hip", "fwd_prefill_wide.hip", "bwd_dq_ilp.hip", "fwd_prefill_d64.hip", "fwd_prefill_pack.hip", "fwd_prefill_d96.hip", "bwd_d96.hip", "fwd_prefill_wide_paged.hip",
-               "fwd_kv8.hip", "fwd_prefill_kv8.hip", "fwd_prefill_wide_kv8.hip", "kv8_cache.hip", "qk_norm_rotary.hip"]
+               "fwd_kv8.hip", "fwd_prefill_kv8.hip", "fwd_prefill_kv8_rows.hip", "fwd_prefill_wide_kv8.hip", "kv8_cache.hip", "qk_norm_rotary.hip"]
 # The development library (libvfa_hip_dev.so, -DVFA_DEV) adds the kernels no shipped dispatch takes
 # and the kernel-variant switches (vfa_debug_set_tuning) that select them; the A/B tools and the
 # tests that check a shipped kernel against its alternative load it.  The product never does.
 DEV_SOURCES = HIP_SOURCES + ["fwd_prefill_w64.hip", "bwd_dkdv_persist.hip"]
 DEV_LIB = os.path.join(HERE, "libvfa_hip_dev.so")
+# No kernel variant of these can be switched: both libraries take the same objects.
+SHARED_SOURCES = ["fwd_kv8.hip", "fwd_prefill_kv8.hip", "fwd_prefill_kv8_rows.hip", "fwd_prefill_wide_kv8.hip", "kv8_cache.hip", "qk_norm_rotary.hip"]
 # No packed fp32 vector instructions (v_pk_{add,mul,fma}_f32): some of their forms have given wrong
 # results on gfx950 now and then, without an error.  (hipcc's host pass warns that it does not know the
 # feature: harmless.)  On every object of the operators around the 8-bit KV cache, which launch no kernel from another.  The
@@ -42,7 +44,7 @@ DEV_LIB = os.path.join(HERE, "libvfa_hip_dev.so")
 NO_PACKED_FP32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 # Kernels built for one wave per SIMD (up to 512 registers): MFMA results that vector instructions
 # consume must be allocated in the arch VGPRs, not forced into the accumulator half of the file.
-EXTRA_FLAGS = {"fwd_kv8.hip": NO_PACKED_FP32, "fwd_prefill_kv8.hip": NO_PACKED_FP32, "kv8_cache.hip": NO_PACKED_FP32, "qk_norm_rotary.hip": NO_PACKED_FP32,
+EXTRA_FLAGS = {"fwd_kv8.hip": NO_PACKED_FP32, "fwd_prefill_kv8.hip": NO_PACKED_FP32, "fwd_prefill_kv8_rows.hip": NO_PACKED_FP32, "kv8_cache.hip": NO_PACKED_FP32, "qk_norm_rotary.hip": NO_PACKED_FP32,
                "fwd_prefill_wide_kv8.hip": NO_PACKED_FP32 + ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
                "bwd_dkdv_w64.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
                "bwd_dkdv_wide.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
@@ -62,7 +64,7 @@ EXTRA_FLAGS = {"fwd_kv8.hip": NO_PACKED_FP32, "fwd_prefill_kv8.hip": NO_PACKED_F
                # longer sequences +4 %)
                "fwd_prefill_d64.hip": ["-fno-slp-vectorize"]}
 # the dropout translation units are one-line includes of the kernel sources
-EXTRA_DEPS = {"fwd_prefill_drop.hip": ["fwd_prefill.hip"], "bwd_drop.hip": ["bwd.hip"], "bwd_d96.hip": ["bwd.hip"], "fwd_prefill_wide_paged.hip": ["fwd_prefill_wide.hip"], "fwd_prefill_wide_kv8.hip": ["fwd_prefill_wide.hip"], "bwd_dq_ilp.hip": ["bwd.hip"], "fwd_prefill_d64.hip": ["fwd_prefill.hip"], "fwd_prefill_d96.hip": ["fwd_prefill.hip"], "fwd_prefill_pack.hip": ["fwd_prefill.hip"],
+EXTRA_DEPS = {"fwd_prefill_drop.hip": ["fwd_prefill.hip"], "bwd_drop.hip": ["bwd.hip"], "bwd_d96.hip": ["bwd.hip"], "fwd_prefill_wide_paged.hip": ["fwd_prefill_wide.hip"], "fwd_prefill_wide_kv8.hip": ["fwd_prefill_wide.hip"], "fwd_prefill_kv8_rows.hip": ["fwd_prefill_kv8.hip"], "bwd_dq_ilp.hip": ["bwd.hip"], "fwd_prefill_d64.hip": ["fwd_prefill.hip"], "fwd_prefill_d96.hip": ["fwd_prefill.hip"], "fwd_prefill_pack.hip": ["fwd_prefill.hip"],
               "fwd_prefill_split.hip": ["fwd_prefill.hip"]}
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 HIP_FLAGS = ["--offload-arch=gfx950", "-O3", "-fPIC", "-fvisibility=hidden", "-std=c++17", "-I", INCLUDE, "-I", CSRC]
@@ -80,6 +82,10 @@ def _headers():
         os.path.join(INCLUDE, "vfa.h")]
 
 
+def _object(src, objdir):
+    return os.path.join(OBJ if src in SHARED_SOURCES else objdir, src.replace(".hip", ".o"))
+
+
 def _compile_jobs(sources, objdir, defines, force):
     """hipcc command lines of the objects of one library that are out of date."""
     os.makedirs(objdir, exist_ok=True)
@@ -87,7 +93,9 @@ def _compile_jobs(sources, objdir, defines, force):
     jobs = []
     for src in sources:
         s = os.path.join(CSRC, src)
-        o = os.path.join(objdir, src.replace(".hip", ".o"))
+        if src in SHARED_SOURCES and objdir != OBJ:
+            continue
+        o = _object(src, objdir)
         if force or _newer(o, [s] + hdrs + [os.path.join(CSRC, e) for e in EXTRA_DEPS.get(src, [])]):
             jobs.append([HIPCC] + HIP_FLAGS + EXTRA_FLAGS.get(src, []) + list(defines) + ["-c", s, "-o", o])
     return jobs
@@ -97,7 +105,7 @@ def _run_jobs(jobs):
     if not jobs:
         return
     # the translation units that take longest first (they bound the wall time of a cold build)
-    slow = ("fwd_prefill_wide", "bwd.hip", "bwd_d96", "fwd_prefill.hip", "fwd_prefill_d96", "fwd_prefill_pack", "bwd_dq_ilp", "bwd_drop")
+    slow = ("fwd_prefill_kv8", "fwd_prefill_wide", "fwd_kv8", "bwd.hip", "bwd_d96", "fwd_prefill.hip", "fwd_prefill_d96", "fwd_prefill_pack", "bwd_dq_ilp", "bwd_drop")
     jobs = sorted(jobs, key=lambda c: next((i for i, k in enumerate(slow) if k in c[-3]), len(slow)))
     with ThreadPoolExecutor(max_workers=min(8, len(jobs))) as ex:
         for r in ex.map(lambda c: subprocess.run(c, capture_output=True, text=True), jobs):
@@ -107,7 +115,7 @@ def _run_jobs(jobs):
 
 
 def _link(lib, sources, objdir, rebuilt, force):
-    objs = [os.path.join(objdir, s.replace(".hip", ".o")) for s in sources]
+    objs = [_object(s, objdir) for s in sources]
     if force or rebuilt or _newer(lib, objs):
         subprocess.check_call([HIPCC, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", lib] + objs)
     return lib
@@ -125,6 +133,7 @@ def build_hip(force=False):
 
 def build_dev(force=False):
     """libvfa_hip_dev.so: every kernel and the development switches (see DEV_SOURCES)."""
+    _run_jobs(_compile_jobs(SHARED_SOURCES, OBJ, [], force))
     return _build_lib(DEV_LIB, DEV_SOURCES, os.path.join(OBJ, "dev"), ["-DVFA_DEV"], force)
 
 
@@ -156,7 +165,7 @@ def build_variant(name, defines, sources):
             subprocess.check_call([HIPCC] + HIP_FLAGS + EXTRA_FLAGS.get(src, []) + ["-DVFA_DEV"] + list(defines) +
                                   ["-c", os.path.join(CSRC, src), "-o", o])
         else:
-            o = os.path.join(OBJ, "dev", src.replace(".hip", ".o"))
+            o = _object(src, os.path.join(OBJ, "dev"))
         objs.append(o)
     out = os.path.join(OBJ, "libvfa_%s.so" % name)
     subprocess.check_call([HIPCC, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", out] + objs)

@@ -36,7 +36,8 @@ bool kv8_pairs(int d, int h_k, int rows, int64_t k_hs, int64_t v_hs);
 int kv8_decode_rows(int d, int rows);
 int kv8_decode_wgs_per_cu(int d, int rows, bool pairs);
 hipError_t run_kv8_merge(const KParams &p, hipStream_t stream);
-hipError_t run_fwd_kv8_prefill(const KV8Params &a, bool codes, hipStream_t stream);   // fwd_prefill_kv8.hip
+hipError_t run_fwd_kv8_prefill(const KV8Params &a, hipStream_t stream);          // fwd_prefill_kv8.hip
+hipError_t run_fwd_kv8_prefill_rows(const KV8Params &a, hipStream_t stream);     // fwd_prefill_kv8_rows.hip
 bool kv8_read_back_ok(int64_t seqlen_k, int h_k, int d);
 hipError_t run_fwd_kv8_wide(const KParams &p, hipStream_t stream);               // fwd_prefill_wide_kv8.hip
 hipError_t run_qk_norm_rotary(const QKNormParams &p, bool bwd, hipStream_t stream);   // qk_norm_rotary.hip
@@ -818,7 +819,7 @@ extern "C" int vfa_kv8_mha_fwd(const vfa_kv8_params *p) {
             k16.k_cumulative = 0;
             e = vfa::run_fwd_kv8_wide(k16, stream);
         } else {
-            e = vfa::run_fwd_kv8_prefill(f, !w.read_back, stream);
+            e = w.read_back ? vfa::run_fwd_kv8_prefill_rows(f, stream) : vfa::run_fwd_kv8_prefill(f, stream);
         }
         if (e == hipSuccess && w.pre_splits > 1) e = vfa::run_kv8_merge(f.p, stream);
         if (e != hipSuccess) return hip_fail(e, "kv8 prefill launch");

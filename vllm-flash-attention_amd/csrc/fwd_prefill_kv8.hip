@@ -502,17 +502,24 @@ static hipError_t launch_kv8_prefill_type(const KV8Params &a, hipStream_t stream
     if (a.p.num_splits > 1) return a.p.is_bf16 ? launch_kv8_prefill<DP, true, true, CODES, DV>(a, stream) : launch_kv8_prefill<DP, false, true, CODES, DV>(a, stream);
     return a.p.is_bf16 ? launch_kv8_prefill<DP, true, false, CODES, DV>(a, stream) : launch_kv8_prefill<DP, false, false, CODES, DV>(a, stream);
 }
-// codes: over the cache itself; else over what was read back of it, whose rows a 32-bit offset reaches (kv8_read_back_ok)
-hipError_t run_fwd_kv8_prefill(const KV8Params &a_in, bool codes, hipStream_t stream) {
-    KV8Params a = a_in;
-    a.p.pack_gqa = a_in.p.h_ratio;   // the grid walks the KV heads
-    a.p.h = a_in.p.h_k;
-    const int d = a.p.d;
-    if (codes) return d <= 64 ? launch_kv8_prefill_type<64, true>(a, stream) : d <= 128 ? launch_kv8_prefill_type<128, true>(a, stream) : launch_kv8_prefill_type<256, true>(a, stream);
-    if (d <= 64) return launch_kv8_prefill_type<64, false>(a, stream);
-    if (d <= 96) return launch_kv8_prefill_type<128, false, 96>(a, stream);
-    return d <= 128 ? launch_kv8_prefill_type<128, false>(a, stream) : launch_kv8_prefill_type<256, false>(a, stream);
+static KV8Params packed(KV8Params a) {   // the grid walks the KV heads
+    a.p.pack_gqa = a.p.h_ratio;
+    a.p.h = a.p.h_k;
+    return a;
+}
+#ifdef VFA_KV8_ROWS_TU
+// over what was read back, whose rows a 32-bit offset reaches (kv8_read_back_ok)
+hipError_t run_fwd_kv8_prefill_rows(const KV8Params &a, hipStream_t stream) {
+    if (a.p.d <= 64) return launch_kv8_prefill_type<64, false>(packed(a), stream);
+    if (a.p.d <= 96) return launch_kv8_prefill_type<128, false, 96>(packed(a), stream);
+    return a.p.d <= 128 ? launch_kv8_prefill_type<128, false>(packed(a), stream) : launch_kv8_prefill_type<256, false>(packed(a), stream);
 }
 bool kv8_read_back_ok(int64_t seqlen_k, int h_k, int d) { return (seqlen_k + 256) * h_k * d * 2 < (int64_t)1 << 30; }
+#else
+hipError_t run_fwd_kv8_prefill(const KV8Params &a, hipStream_t stream) {
+    if (a.p.d <= 64) return launch_kv8_prefill_type<64, true>(packed(a), stream);
+    return a.p.d <= 128 ? launch_kv8_prefill_type<128, true>(packed(a), stream) : launch_kv8_prefill_type<256, true>(packed(a), stream);
+}
+#endif
 
 }  // namespace vfa
