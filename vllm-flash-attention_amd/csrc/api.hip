@@ -552,7 +552,8 @@ static bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
 // capacity or more for endless: with more queries than keys neither is the same.)
 static void kv8_window(const vfa_params &a, KParams &k) {
     constexpr int far = 1 << 30;
-    const int wl = a.window_size_left, wr = a.is_causal ? 0 : a.window_size_right;
+    // (a single query is the last: nothing is behind it)
+    const int wl = a.window_size_left, wr = a.seqlen_q == 1 ? -1 : a.is_causal ? 0 : a.window_size_right;
     k.is_causal = wl < 0 && wr == 0;
     k.is_local = (wl >= 0 || wr >= 0) && !k.is_causal;
     k.wl = wl < 0 ? far : std::min(wl, far);
